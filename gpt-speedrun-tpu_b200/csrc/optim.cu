@@ -323,6 +323,215 @@ __global__ void __launch_bounds__(1024) adamw_end_kernel(const double* __restric
   if (!isfinite(grad_norm) || (loss && !isfinite(*loss))) g_optim_error = kErrNonFinite;
 }
 
+// ------------------------------------------------------------------ 8-bit moments
+// The same update with both moments in 8 bits. 64 consecutive elements (a
+// block) share one exponent byte E per moment, the largest magnitude's; a
+// magnitude code holds its exponent relative to E in 4 bits and the mantissa's
+// leading bits below it:
+//   m: sign, 4 exponent bits, 3 mantissa bits;  r = sqrt(v): 4 + 4 bits,
+//   value = 2^(E - 127 - 15 + exponent) (1 + mantissa / 8 or / 16), code 0 = 0,
+//   E = 255 marks a block that held a NaN or an infinity (it decodes to NaN).
+// Floating codes, because the update is m / r element by element: with a step
+// size common to a block, elements far below its largest would get moments off
+// by many times their size. r and not v, because r's range is half as wide and
+// r is what the update divides by. An m below the range becomes 0 and an r
+// below it the smallest code, so rounding never enlarges |m / r| without bound.
+// The bits below a code are rounded by adding random bits and cutting: with
+// beta2 = 0.95 an r whose gradients vanish falls by 2.5% a step, less than half
+// a unit of the code, and rounding to nearest would hold it up for ever. The
+// random bits are a hash of (seed, step, element), so a step is a function of
+// its inputs. Moments enter the update unrounded; every operation up to the
+// codes is rounded by itself (no contraction), so that a restatement with
+// separate operations yields the same codes.
+// Bound by HBM: parameters, gradient, codes and the bf16 copy move 18.06 bytes
+// per parameter, where fp32 moments need 30.
+constexpr int kQBlock = 64;
+
+// The finalizer of MurmurHash3 (32 bits; Appleby, public domain).
+__device__ __forceinline__ uint32_t mix32(uint32_t h) {
+  h = (h ^ (h >> 16)) * 0x85EBCA6Bu;
+  h = (h ^ (h >> 13)) * 0xC2B2AE35u;
+  return h ^ (h >> 16);
+}
+__device__ __forceinline__ uint32_t dither_bits(int64_t e, uint32_t key) {
+  return mix32((uint32_t)e * 0x9E3779B1u + (uint32_t)(e >> 32) * 0x85EBCA77u + key);
+}
+
+// Magnitude of a code with M mantissa bits under block exponent E.
+template <int M>
+__device__ __forceinline__ float q8_decode(int code, int E) {
+  const float x = __int_as_float((code << (23 - M)) + ((E - 15) << 23));
+  return E == 255 ? __int_as_float(0x7fffffff) : code == 0 ? 0.f : x;
+}
+// Block exponent for a largest magnitude with these bits: the one above if the
+// top code would not reach it. At least 16, so that the smallest code is a
+// normal number.
+template <int M>
+__device__ __forceinline__ int q8_exponent(int top_bits) {
+  const int e = (top_bits + ((1 << (23 - M)) - 1)) >> 23;
+  return e >= 255 ? 255 : max(e, 16);
+}
+template <int M>
+__device__ __forceinline__ int q8_encode(int bits, int dither, int E, int low) {
+  const int c = (bits + dither - ((E - 15) << 23)) >> (23 - M);
+  return min(max(c, low), (16 << M) - 1);
+}
+
+__global__ void __launch_bounds__(256) adamw8_kernel(
+    float* __restrict__ p, uint8_t* __restrict__ mq, uint8_t* __restrict__ me,
+    uint8_t* __restrict__ vq, uint8_t* __restrict__ ve, const float* __restrict__ g, int64_t begin,
+    int64_t end, const gptb200_tensor_group* __restrict__ groups, int ngroups,
+    const gptb200_adamw_config cfg, const AdamScalars* __restrict__ sc, uint32_t seed,
+    bf16* __restrict__ pbf, double* __restrict__ part) {
+  extern __shared__ gptb200_tensor_group sg[];
+  __shared__ double red[8];
+  for (int i = threadIdx.x; i < ngroups; i += blockDim.x) sg[i] = groups[i];
+  __syncthreads();
+  const AdamScalars s = *sc;
+  const uint32_t key = mix32(mix32((uint32_t)s.step) ^ seed);
+  const float b1 = cfg.beta1, b2 = cfg.beta2;
+  const float omb1 = 1.0f - b1, omb2 = 1.0f - b2;
+  const float inv1 = 1.0f / s.bc1, inv2 = 1.0f / sqrtf(s.bc2);
+  double acc = 0.0;
+  float accf = 0.f;
+  int cnt = 0, gi = 0;
+  // Sixteen lanes share a block, four elements each.
+  const int64_t stride = (int64_t)gridDim.x * blockDim.x * 4;
+  const int64_t stop = (end + kQBlock - 1) / kQBlock * kQBlock;  // whole blocks: shuffles below
+  for (int64_t e0 = begin + ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 4;
+       e0 - 4 * (threadIdx.x & 31) < stop; e0 += stride) {
+    const bool in = e0 < end;
+    gi = in ? find_group(sg, ngroups, gi, e0) : -1;
+    const bool live = gi >= 0;  // else padding between tensors, or past the end
+    const gptb200_tensor_group& G = sg[live ? gi : 0];
+    const int n = live ? (int)min((int64_t)4, min(end, G.offset + G.size) - e0) : 0;
+    float P[4] = {0.f, 0.f, 0.f, 0.f}, Gr[4] = {0.f, 0.f, 0.f, 0.f};
+    uint32_t mc = 0, vc = 0;
+    int em = 16, ev = 16;
+    if (n == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(p + e0);
+      const float4 b = __ldcs(reinterpret_cast<const float4*>(g + e0));
+      P[0] = a.x, P[1] = a.y, P[2] = a.z, P[3] = a.w;
+      Gr[0] = b.x, Gr[1] = b.y, Gr[2] = b.z, Gr[3] = b.w;
+    } else {
+      for (int j = 0; j < n; ++j) {
+        P[j] = p[e0 + j];
+        Gr[j] = g[e0 + j];
+      }
+    }
+    if (live) {
+      mc = *reinterpret_cast<const uint32_t*>(mq + e0);
+      vc = *reinterpret_cast<const uint32_t*>(vq + e0);
+      em = me[e0 / kQBlock];
+      ev = ve[e0 / kQBlock];
+    }
+    const float lr = s.lr * G.lr_mult;
+    const float eps = cfg.eps * cfg.eps_horizon_scale * G.eps_mult;
+    const float wd = G.decay ? cfg.weight_decay * cfg.wd_horizon_scale * G.wd_mult : 0.f;
+    float M[4], R[4];
+    int mtop = 0, vtop = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      accf += Gr[j] * Gr[j];
+      const float gr = __fmul_rn(Gr[j], s.gscale);
+      const int c = (mc >> (8 * j)) & 255;
+      const float mag = q8_decode<3>(c & 127, em);
+      const float r = q8_decode<4>((vc >> (8 * j)) & 255, ev);
+      M[j] = __fadd_rn(__fmul_rn(b1, c & 128 ? -mag : mag), __fmul_rn(omb1, gr));
+      R[j] = __fsqrt_rn(
+          __fadd_rn(__fmul_rn(b2, __fmul_rn(r, r)), __fmul_rn(omb2, __fmul_rn(gr, gr))));
+      if (j >= n) M[j] = R[j] = 0.f;
+      mtop = max(mtop, __float_as_int(fabsf(M[j])));
+      vtop = max(vtop, __float_as_int(fabsf(R[j])));
+      const float adam = (M[j] * inv1) / (R[j] * inv2 + eps);
+      P[j] = P[j] - lr * (adam + wd * P[j]);
+    }
+    if (n == 4) {
+      *reinterpret_cast<float4*>(p + e0) = make_float4(P[0], P[1], P[2], P[3]);
+      if (pbf)
+        *reinterpret_cast<uint2*>(pbf + e0) =
+            make_uint2(pack_bf16x2(P[0], P[1]), pack_bf16x2(P[2], P[3]));
+    } else {
+      for (int j = 0; j < n; ++j) {
+        p[e0 + j] = P[j];
+        if (pbf) pbf[e0 + j] = __float2bfloat16(P[j]);
+      }
+    }
+    // the block's exponents: the 16 lanes' largest magnitudes (as integers, so
+    // that a NaN or an infinity is larger than every number)
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      mtop = max(mtop, __shfl_xor_sync(0xffffffffu, mtop, o));
+      vtop = max(vtop, __shfl_xor_sync(0xffffffffu, vtop, o));
+    }
+    em = q8_exponent<3>(mtop);
+    ev = q8_exponent<4>(vtop);
+    mc = vc = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t h = dither_bits(e0 + j, key);
+      const int mb = __float_as_int(M[j]), rb = __float_as_int(R[j]) & 0x7fffffff;
+      int cm = q8_encode<3>(mb & 0x7fffffff, (h >> 16) << 4, em, 0);
+      const int cv = q8_encode<4>(rb, (h & 0xffff) << 3, ev, rb != 0);
+      if (mb < 0 && cm) cm |= 128;
+      mc |= (uint32_t)cm << (8 * j);
+      vc |= (uint32_t)cv << (8 * j);
+    }
+    if (live) {
+      *reinterpret_cast<uint32_t*>(mq + e0) = mc;
+      *reinterpret_cast<uint32_t*>(vq + e0) = vc;
+    }
+    // one lane of each block writes its exponents: the first that holds a tensor's element
+    const unsigned any = __ballot_sync(0xffffffffu, live) >> (threadIdx.x & 16) & 0xffff;
+    if (live && (threadIdx.x & 15) == __ffs(any) - 1) {
+      me[e0 / kQBlock] = (uint8_t)em;
+      ve[e0 / kQBlock] = (uint8_t)ev;
+    }
+    if (gi < 0) gi = 0;
+    if (++cnt == 16) {
+      acc += accf;
+      accf = 0.f;
+      cnt = 0;
+    }
+  }
+  if (!part) return;
+  acc += accf;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (int w = 0; w < 8; ++w) t += red[w];
+    part[blockIdx.x] = t;
+  }
+}
+
+// The values that codes stand for (each fits bf16 exactly).
+__global__ void __launch_bounds__(256) adamw8_values_kernel(
+    const uint8_t* __restrict__ mq, const uint8_t* __restrict__ me,
+    const uint8_t* __restrict__ vq, const uint8_t* __restrict__ ve, int64_t n,
+    bf16* __restrict__ m, bf16* __restrict__ r) {
+  for (int64_t e = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8; e < n;
+       e += (int64_t)gridDim.x * blockDim.x * 8) {
+    const uint2 mc = *reinterpret_cast<const uint2*>(mq + e);
+    const uint2 vc = *reinterpret_cast<const uint2*>(vq + e);
+    const int em = me[e / kQBlock], ev = ve[e / kQBlock];
+    float a[8], b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = ((j < 4 ? mc.x : mc.y) >> (8 * (j & 3))) & 255;
+      const float mag = q8_decode<3>(c & 127, em);
+      a[j] = c & 128 ? -mag : mag;
+      b[j] = q8_decode<4>(((j < 4 ? vc.x : vc.y) >> (8 * (j & 3))) & 255, ev);
+    }
+    *reinterpret_cast<uint4*>(m + e) = make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]),
+                                                  pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
+    *reinterpret_cast<uint4*>(r + e) = make_uint4(pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3]),
+                                                  pack_bf16x2(b[4], b[5]), pack_bf16x2(b[6], b[7]));
+  }
+}
+
 }  // namespace gptb200
 
 using namespace gptb200;
@@ -437,6 +646,110 @@ extern "C" int gptb200_adamw_end(int32_t n_slots, const gptb200_adamw_config* cf
   auto part = reinterpret_cast<const double*>(reinterpret_cast<char*>(workspace) + kSlotsOffset);
   adamw_end_kernel<<<1, 1024, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
       part, n_slots * kRangeBlocks, step, *cfg, loss, history);
+  GPTB200_CHECK_LAUNCH();
+  return 0;
+}
+
+// ------------------------------------------------------------------ 8-bit moments (entry points)
+static int adamw8_check(const gptb200_adamw8_state* state, const void* params, const void* grads,
+                        const gptb200_tensor_group* groups, int32_t n_groups,
+                        const gptb200_adamw_config* cfg, const void* params_bf16,
+                        const void* workspace) {
+  if (!state || !state->m || !state->m_exp || !state->v || !state->v_exp || !params || !grads ||
+      !groups || !cfg || !workspace || n_groups <= 0)
+    return GPTB200_EINVAL;
+  if (n_groups > 4096) return GPTB200_EUNSUPPORTED;
+  if (((reinterpret_cast<uintptr_t>(params) | reinterpret_cast<uintptr_t>(grads) |
+        reinterpret_cast<uintptr_t>(state->m) | reinterpret_cast<uintptr_t>(state->v) |
+        reinterpret_cast<uintptr_t>(workspace)) & 15) ||
+      (params_bf16 && (reinterpret_cast<uintptr_t>(params_bf16) & 7)))
+    return GPTB200_ESHAPE;
+  return 0;
+}
+
+// Updates elements [begin, end); part: kRangeBlocks sums of squared gradients, or null.
+static int adamw8_launch(float* params, const gptb200_adamw8_state& q, const float* grads,
+                         int64_t begin, int64_t end, const gptb200_tensor_group* groups,
+                         int32_t n_groups, const gptb200_adamw_config& cfg, const AdamScalars* sc,
+                         uint32_t seed, void* params_bf16, double* part, cudaStream_t st) {
+  const size_t smem = (size_t)n_groups * sizeof(gptb200_tensor_group);
+  if (smem > 40 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(adamw8_kernel,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return -static_cast<int>(e);
+  }
+  adamw8_kernel<<<kRangeBlocks, 256, smem, st>>>(
+      params, q.m, q.m_exp, q.v, q.v_exp, grads, begin, end, groups, n_groups, cfg, sc, seed,
+      reinterpret_cast<bf16*>(params_bf16), part);
+  GPTB200_CHECK_LAUNCH();
+  return 0;
+}
+
+extern "C" int gptb200_adamw8_step(float* params, const gptb200_adamw8_state* state,
+                                   const float* grads, int64_t n,
+                                   const gptb200_tensor_group* groups, int32_t n_groups,
+                                   const gptb200_adamw_config* cfg, int32_t* step,
+                                   const float* loss, float* history, void* params_bf16,
+                                   uint32_t seed, void* workspace, void* stream) {
+  const int s = adamw8_check(state, params, grads, groups, n_groups, cfg, params_bf16, workspace);
+  if (s) return s;
+  if (!step || n <= 0) return GPTB200_EINVAL;
+  auto st = reinterpret_cast<cudaStream_t>(stream);
+  char* ws = reinterpret_cast<char*>(workspace);
+  AdamScalars* sc = reinterpret_cast<AdamScalars*>(ws + kScalarsOffset);
+  if (cfg->grad_clip > 0.f) {  // clipping needs the global norm first
+    double* part = reinterpret_cast<double*>(ws);
+    sqnorm_partial_kernel<<<kNormBlocks, kNormThreads, 0, st>>>(grads, n, part);
+    GPTB200_CHECK_LAUNCH();
+    adamw_scalars_kernel<<<1, 1024, 0, st>>>(part, kNormBlocks, *cfg, step, loss, history, sc);
+    GPTB200_CHECK_LAUNCH();
+    return adamw8_launch(params, *state, grads, 0, n, groups, n_groups, *cfg, sc, seed,
+                         params_bf16, nullptr, st);
+  }
+  // without clipping the gradients are read once: the update also sums their squares
+  int e = gptb200_adamw_begin(cfg, step, workspace, stream);
+  if (e) return e;
+  e = adamw8_launch(params, *state, grads, 0, n, groups, n_groups, *cfg, sc, seed, params_bf16,
+                    reinterpret_cast<double*>(ws + kSlotsOffset), st);
+  if (e) return e;
+  return gptb200_adamw_end(1, cfg, step, loss, history, workspace, stream);
+}
+
+extern "C" int gptb200_adamw8_update_range(float* params, const gptb200_adamw8_state* state,
+                                           const float* grads, int64_t begin, int64_t end,
+                                           const gptb200_tensor_group* groups, int32_t n_groups,
+                                           const gptb200_adamw_config* cfg, int32_t slot,
+                                           void* params_bf16, uint32_t seed, void* workspace,
+                                           void* stream) {
+  const int s = adamw8_check(state, params, grads, groups, n_groups, cfg, params_bf16, workspace);
+  if (s) return s;
+  if (begin < 0 || end <= begin || begin % kQBlock || end % kQBlock || slot < 0 ||
+      slot >= kMaxSlots)
+    return GPTB200_EINVAL;
+  if (cfg->grad_clip > 0.f) return GPTB200_EUNSUPPORTED;
+  char* ws = reinterpret_cast<char*>(workspace);
+  return adamw8_launch(params, *state, grads, begin, end, groups, n_groups, *cfg,
+                       reinterpret_cast<const AdamScalars*>(ws + kScalarsOffset), seed,
+                       params_bf16,
+                       reinterpret_cast<double*>(ws + kSlotsOffset) + (int64_t)slot * kRangeBlocks,
+                       reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int gptb200_adamw8_values(const gptb200_adamw8_state* state, int64_t n, void* m,
+                                     void* v_root, void* stream) {
+  if (!state || !state->m || !state->m_exp || !state->v || !state->v_exp || !m || !v_root ||
+      n <= 0)
+    return GPTB200_EINVAL;
+  if (n % kQBlock || ((reinterpret_cast<uintptr_t>(state->m) | reinterpret_cast<uintptr_t>(state->v) |
+                       reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v_root)) & 15))
+    return GPTB200_ESHAPE;
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int blocks = (int)std::min<int64_t>((n / 8 + 255) / 256, (int64_t)sms * 8);
+  adamw8_values_kernel<<<blocks, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      state->m, state->m_exp, state->v, state->v_exp, n, reinterpret_cast<bf16*>(m),
+      reinterpret_cast<bf16*>(v_root));
   GPTB200_CHECK_LAUNCH();
   return 0;
 }

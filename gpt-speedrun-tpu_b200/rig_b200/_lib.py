@@ -70,6 +70,10 @@ class AdamWConfig(ctypes.Structure):
     ]
 
 
+class AdamW8State(ctypes.Structure):
+    _fields_ = [("m", c_vp), ("m_exp", c_vp), ("v", c_vp), ("v_exp", c_vp)]
+
+
 EPI_BF16 = 0
 EPI_BIAS_GELU = 1
 EPI_DGELU = 2
@@ -77,6 +81,9 @@ EPI_F32 = 3
 EPI_F32_ATOMIC = 4
 EPI_BIAS_ROPE = 5
 EPI_F32_SPLITK = 6
+
+DTYPE_BF16 = 0
+DTYPE_F32 = 1
 
 DEVERR_GEMM = 1
 DEVERR_ATTENTION = 2
@@ -100,6 +107,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "gptb200_rms_norm_bwd_workspace_size": (c_size, [c_i64, c_i64]),
     "gptb200_rms_norm_bwd": (
         c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_f32, c_i64, c_i64, c_vp, c_vp]),
+    "gptb200_layer_norm_fwd": (
+        c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_f32, c_int, c_vp]),
+    "gptb200_layer_norm_bwd_workspace_size": (c_size, [c_i64, c_i64]),
+    "gptb200_layer_norm_bwd": (
+        c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_f32, c_i64, c_i64,
+                c_i64, c_i64, c_i64, c_int, c_vp, c_vp]),
     "gptb200_embedding_fwd": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp]),
     "gptb200_embedding_bwd_workspace_size": (c_size, [c_i64, c_i64, c_i64]),
     "gptb200_embedding_bwd": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp]),
@@ -167,6 +180,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "gptb200_adamw_end": (
         c_int, [ctypes.c_int32, ctypes.POINTER(AdamWConfig), c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "gptb200_adamw8_step": (
+        c_int,
+        [c_vp, ctypes.POINTER(AdamW8State), c_vp, c_i64, c_vp, ctypes.c_int32,
+         ctypes.POINTER(AdamWConfig), c_vp, c_vp, c_vp, c_vp, ctypes.c_uint32, c_vp, c_vp],
+    ),
+    "gptb200_adamw8_update_range": (
+        c_int,
+        [c_vp, ctypes.POINTER(AdamW8State), c_vp, c_i64, c_i64, c_vp, ctypes.c_int32,
+         ctypes.POINTER(AdamWConfig), ctypes.c_int32, c_vp, ctypes.c_uint32, c_vp, c_vp],
+    ),
+    "gptb200_adamw8_values": (c_int, [ctypes.POINTER(AdamW8State), c_i64, c_vp, c_vp, c_vp]),
     "gptb200_cast_bf16": (c_int, [c_vp, c_vp, c_i64, c_vp]),
     "gptb200_mix_uint64": (ctypes.c_uint64, [ctypes.c_uint64]),
     "gptb200_permute_bounded": (

@@ -1,7 +1,8 @@
 """Layer building blocks with the signatures of the reference's rig/nn.py.
 
 `rms_norm` (rig/nn.py:26-33), `apply_rotary` (:36-52) and `linear` (:55-56)
-are differentiable (torch.autograd) wrappers over the libgptb200 kernels; `normal`,
+are differentiable (torch.autograd) wrappers over the libgptb200 kernels, and so
+is `layer_norm`, which the reference lacks; `normal`,
 `parameter_count` and `flatten_arrays` are the reference's host helpers
 (:20-23, :59-77). Inputs are CUDA tensors; there is no CPU path.
 """
@@ -57,6 +58,48 @@ def rms_norm(x: torch.Tensor, scale: torch.Tensor, dtype: Any = torch.bfloat16) 
     if dtype != torch.bfloat16:
         raise TypeError("the B200 kernels compute rms_norm in bfloat16")
     return _RmsNorm.apply(x.to(torch.bfloat16), scale)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, scale, bias, eps):
+        shape = x.shape
+        x2 = x.reshape(-1, shape[-1])
+        if x2.stride(1) != 1:
+            x2 = x2.contiguous()
+        w = scale.to(x.dtype).contiguous()
+        b = None if bias is None else bias.to(x.dtype).contiguous()
+        y = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
+        mean, rstd = torch.empty(2, x2.shape[0], dtype=torch.float32, device=x.device).unbind()
+        ops.layer_norm_fwd(x2, w, b, y, mean, rstd, eps)
+        ctx.save_for_backward(x2, w, mean, rstd)
+        ctx.dtypes = (scale.dtype, None if bias is None else bias.dtype)
+        return y.reshape(shape)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x2, w, mean, rstd = ctx.saved_tensors
+        shape = dy.shape
+        dy2 = dy.reshape(x2.shape).to(x2.dtype).contiguous()
+        dx = torch.empty(x2.shape, dtype=x2.dtype, device=x2.device)
+        dscale, dbias = torch.zeros(2, x2.shape[1], dtype=torch.float32, device=x2.device).unbind()
+        ops.layer_norm_bwd(x2, w, mean, rstd, dy2, None, dx, dscale, dbias)
+        sd, bd = ctx.dtypes
+        return dx.reshape(shape), dscale.to(sd), None if bd is None else dbias.to(bd), None
+
+
+def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """(x - mean) / sqrt(var + eps) * scale + bias over the last dimension.
+
+    bf16 or fp32 x (scale and bias are used in x's dtype), fp32 statistics, one
+    rounding of the result; differentiable in x, scale and bias."""
+
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"layer_norm takes bfloat16 or float32, got {x.dtype}")
+    if x.dim() < 1 or tuple(scale.shape) != (x.shape[-1],):
+        raise ValueError(f"scale must be [{x.shape[-1] if x.dim() else 0}], got {tuple(scale.shape)}")
+    return _LayerNorm.apply(x, scale, bias, eps)
 
 
 _ROPE_TABLES: dict[tuple, tuple[torch.Tensor, torch.Tensor]] = {}

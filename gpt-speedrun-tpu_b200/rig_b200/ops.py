@@ -207,6 +207,77 @@ def rms_norm_bwd(x, scale, rstd, dy, dx_in, dx_out, dscale, dx_colsum=None, cols
     return dx_out
 
 
+# ----------------------------------------------------------------- layer norm
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+
+
+def _norm_args(x, vectors: dict, rows: dict, stats: dict) -> int:
+    """Checks layer norm's tensors against x [rows, d]; returns x's dtype code."""
+
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"layer norm takes bfloat16 or float32 rows, got {x.dtype}")
+    if x.dim() != 2:
+        raise ValueError(f"layer norm takes 2-D rows, got {tuple(x.shape)}")
+    n, d = x.shape
+    wanted = [(vectors, (d,), x.dtype), (rows, (n, d), x.dtype), (stats, None, F32)]
+    for tensors, shape, dtype in wanted:
+        for name, t in tensors.items():
+            if t is None:
+                continue
+            want = shape if shape is not None else ((n,) if name in ("mean", "rstd") else (d,))
+            if tuple(t.shape) != want or t.dtype != dtype:
+                raise ValueError(f"{name} must be {dtype} {want}, got {t.dtype} {tuple(t.shape)}")
+            if (t.dim() == 1 and not t.is_contiguous()) or (t.dim() == 2 and t.stride(1) != 1 and d > 1):
+                raise ValueError(f"{name} must have unit inner stride, got {tuple(t.stride())}")
+    return _DTYPES[x.dtype]
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Row stride in elements (a single row may carry any stride)."""
+
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def layer_norm_fwd(x, scale, bias, y, mean, rstd, eps: float = 1e-5):
+    """y = (x - mean) * rstd * scale + bias over the rows of x (bf16 or fp32,
+    any row stride); mean and rstd (fp32 [rows]) are written for the backward.
+    bias may be None. y may be x."""
+
+    _cuda(x, scale, bias, y, mean, rstd)
+    code = _norm_args(x, dict(scale=scale, bias=bias), dict(x=x, y=y), dict(mean=mean, rstd=rstd))
+    call("gptb200_layer_norm_fwd", x.data_ptr(), scale.data_ptr(), _ptr(bias), y.data_ptr(),
+         mean.data_ptr(), rstd.data_ptr(), x.shape[0], x.shape[1], _row_stride(x), _row_stride(y),
+         float(eps), code, _stream())
+    return y, mean, rstd
+
+
+def layer_norm_bwd_workspace_size(rows: int, d: int) -> int:
+    return int(_lib.load().gptb200_layer_norm_bwd_workspace_size(rows, d))
+
+
+def layer_norm_bwd(x, scale, mean, rstd, dy, dx_in, dx_out, dscale, dbias=None, dx_colsum=None,
+                   colsum_alpha=1.0, workspace=None):
+    """dx_out = dx_in + d(layer_norm)/dx . dy; dscale +=; dbias +=; dx_colsum +=
+    alpha * colsum(dx_out). dx_in, dbias and dx_colsum may be None."""
+
+    _cuda(x, scale, mean, rstd, dy, dx_in, dx_out, dscale, dbias, dx_colsum, workspace)
+    code = _norm_args(x, dict(scale=scale), dict(x=x, dy=dy, dx_in=dx_in, dx_out=dx_out),
+                      dict(mean=mean, rstd=rstd, dscale=dscale, dbias=dbias, dx_colsum=dx_colsum))
+    rows, d = x.shape
+    if dx_in is not None and _row_stride(dx_in) != _row_stride(dx_out):
+        raise ValueError("dx_in and dx_out must share strides")
+    size = layer_norm_bwd_workspace_size(rows, d)
+    if workspace is None:
+        workspace = _scratch(size, x.device)
+    elif workspace.numel() * workspace.element_size() < size:
+        raise ValueError(f"the workspace needs {size} bytes")
+    call("gptb200_layer_norm_bwd", x.data_ptr(), scale.data_ptr(), mean.data_ptr(),
+         rstd.data_ptr(), dy.data_ptr(), _ptr(dx_in), dx_out.data_ptr(), dscale.data_ptr(),
+         _ptr(dbias), _ptr(dx_colsum), float(colsum_alpha), rows, d, _row_stride(x),
+         _row_stride(dy), _row_stride(dx_out), code, _ptr(workspace), _stream())
+    return dx_out
+
+
 # ----------------------------------------------------------------- embedding
 def embedding_fwd(tokens: torch.Tensor, table: torch.Tensor, out: torch.Tensor):
     _cuda(tokens, table, out)
@@ -433,6 +504,73 @@ def adamw_end(n_slots, cfg, step, loss, history, workspace):
     _cuda(step, loss, history, workspace)
     call("gptb200_adamw_end", int(n_slots), ctypes.byref(cfg), step.data_ptr(), _ptr(loss),
          _ptr(history), workspace.data_ptr(), _stream())
+
+
+ADAMW8_BLOCK = 64  # elements that share one exponent byte
+
+
+def adamw8_state(n: int, device) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The zero state of n elements: (m codes, m exponents, v codes, v exponents)."""
+
+    blocks = (int(n) + ADAMW8_BLOCK - 1) // ADAMW8_BLOCK
+    return tuple(torch.zeros(k, dtype=torch.uint8, device=device)
+                 for k in (blocks * ADAMW8_BLOCK, blocks) * 2)
+
+
+def _adamw8(state, n: int, floats: dict) -> _lib.AdamW8State:
+    """Checks a state and the flat buffers that go with it."""
+
+    _cuda(*state, *(t for t, _ in floats.values()))
+    blocks = (n + ADAMW8_BLOCK - 1) // ADAMW8_BLOCK
+    for t, size in zip(state, (blocks * ADAMW8_BLOCK, blocks) * 2, strict=True):
+        if t.dtype != torch.uint8 or t.numel() < size or not t.is_contiguous():
+            raise ValueError(f"an 8-bit state of {n} elements is contiguous uint8 arrays of "
+                             f"{blocks * ADAMW8_BLOCK} codes and {blocks} exponents")
+    for name, (t, dtype) in floats.items():
+        if t is not None and (t.dtype != dtype or t.numel() != n or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous {dtype} of {n} elements")
+    return _lib.AdamW8State(*(t.data_ptr() for t in state))
+
+
+def adamw8_step(params, state, grads, groups_dev, n_groups, cfg, step, loss, history, params_bf16,
+                seed, workspace):
+    """`adamw_step` with both moments in 8 bits (`adamw8_state`, updated in place).
+
+    The rounding of the new moments draws on (seed, step, element): the same
+    inputs give the same codes. workspace: `adamw_workspace`."""
+
+    _cuda(groups_dev, step, loss, history, workspace)
+    q = _adamw8(state, params.numel(), dict(params=(params, F32), grads=(grads, F32),
+                                            params_bf16=(params_bf16, BF16)))
+    call("gptb200_adamw8_step", params.data_ptr(), ctypes.byref(q), grads.data_ptr(),
+         params.numel(), groups_dev.data_ptr(), n_groups, ctypes.byref(cfg), step.data_ptr(),
+         _ptr(loss), _ptr(history), _ptr(params_bf16), int(seed) & 0xFFFFFFFF,
+         workspace.data_ptr(), _stream())
+
+
+def adamw8_update_range(params, state, grads, begin, end, groups_dev, n_groups, cfg, slot,
+                        params_bf16, seed, workspace):
+    """`adamw_update_range` with 8-bit moments; begin and end are multiples of 64."""
+
+    _cuda(groups_dev, workspace)
+    q = _adamw8(state, params.numel(), dict(params=(params, F32), grads=(grads, F32),
+                                            params_bf16=(params_bf16, BF16)))
+    if not 0 <= begin < end <= state[0].numel():
+        raise ValueError(f"[{begin}, {end}) is outside the {state[0].numel()} elements")
+    call("gptb200_adamw8_update_range", params.data_ptr(), ctypes.byref(q), grads.data_ptr(),
+         int(begin), int(end), groups_dev.data_ptr(), n_groups, ctypes.byref(cfg), int(slot),
+         _ptr(params_bf16), int(seed) & 0xFFFFFFFF, workspace.data_ptr(), _stream())
+
+
+def adamw8_values(state) -> tuple[torch.Tensor, torch.Tensor]:
+    """(m, sqrt(v)) that a state's codes stand for, as bf16 (exact)."""
+
+    n = state[0].numel()
+    q = _adamw8(state, n, {})
+    m = torch.empty(n, dtype=BF16, device=state[0].device)
+    root = torch.empty_like(m)
+    call("gptb200_adamw8_values", ctypes.byref(q), n, m.data_ptr(), root.data_ptr(), _stream())
+    return m, root
 
 
 def device_error(clear: bool = True) -> int:

@@ -138,6 +138,34 @@ int gptb200_rms_norm_bwd(const void* x, const void* scale, const float* rstd, co
                          float colsum_alpha, int64_t rows, int64_t d, void* workspace,
                          void* stream);
 
+/* ------------------------------------------------------------------ layer norm
+ * y = (x - mean) * rstd * scale + bias, rstd = 1 / sqrt(var + eps), statistics
+ * in fp32 (the variance about the mean), one rounding at the end. x, y, scale
+ * and bias have element type `dtype`; bias may be NULL; rows have unit inner
+ * stride and row strides of x_stride / y_stride elements (>= d). mean, rstd:
+ * fp32 [rows], saved for the backward. Any d from 1 to 16384; rows of 8-element
+ * multiples on 16-byte boundaries take the 16-byte path. No reference
+ * counterpart (the rig's models use rms_norm). */
+#define GPTB200_DTYPE_BF16 0
+#define GPTB200_DTYPE_F32 1
+int gptb200_layer_norm_fwd(const void* x, const void* scale, const void* bias, void* y,
+                           float* mean, float* rstd, int64_t rows, int64_t d, int64_t x_stride,
+                           int64_t y_stride, float eps, int dtype, void* stream);
+
+/* Backward of layer_norm. dx_out = dx_in (residual-stream gradient, NULL for
+ * zero, may alias dx_out) + d(layer_norm)/dx . dy, rounded once; dscale and
+ * dbias (fp32 [d], dbias may be NULL) are accumulated into, as is dx_colsum
+ * (fp32 [d] or NULL) with colsum_alpha times the column sums of dx_out before
+ * its rounding. dx_in and dx_out share dx_stride. The column sums add per-block
+ * partials (in `workspace`, gptb200_layer_norm_bwd_workspace_size bytes) in a
+ * fixed order: repeated calls give bit-identical results. */
+size_t gptb200_layer_norm_bwd_workspace_size(int64_t rows, int64_t d);
+int gptb200_layer_norm_bwd(const void* x, const void* scale, const float* mean, const float* rstd,
+                           const void* dy, const void* dx_in, void* dx_out, float* dscale,
+                           float* dbias, float* dx_colsum, float colsum_alpha, int64_t rows,
+                           int64_t d, int64_t x_stride, int64_t dy_stride, int64_t dx_stride,
+                           int dtype, void* workspace, void* stream);
+
 /* ------------------------------------------------------------------ embedding
  * out[i, :] = bf16(table[tokens[i], :]); Replaces recipes/reference/train.py:1107
  * (`params["token_embedding"][tokens].astype(dtype)`). table bf16 [vocab, d].
@@ -397,6 +425,41 @@ int gptb200_adamw_update_range(float* params, float* m, float* v, const float* g
                                void* params_bf16, void* workspace, void* stream);
 int gptb200_adamw_end(int32_t n_slots, const gptb200_adamw_config* cfg, const int32_t* step,
                       const float* loss, float* history, void* workspace, void* stream);
+
+/* The update with both Adam moments in 8 bits (no reference counterpart; the
+ * rule of gptb200_adamw_step otherwise). 64 consecutive elements of the flat
+ * buffers share one exponent byte E per moment: a code is the value's exponent
+ * relative to E in 4 bits and its leading mantissa bits,
+ *   m:      sign, 4 exponent bits, 3 mantissa bits (0: zero),
+ *   v_root: 4 exponent bits, 4 mantissa bits of sqrt(v) (0: zero),
+ *   |value| = 2^(E - 142 + exponent) * (1 + mantissa / 8 or / 16);
+ * E = 255: the block held a NaN or an infinity. Bits below a code are rounded
+ * with random bits hashed from (seed, step, element), so the same inputs give
+ * the same codes. All four arrays zero is the initial state. Code arrays hold
+ * n rounded up to 64 bytes and are 16-byte aligned; exponent arrays one byte
+ * per 64 elements. Workspace: gptb200_adamw_workspace_size. */
+typedef struct gptb200_adamw8_state {
+  uint8_t* m;
+  uint8_t* m_exp;
+  uint8_t* v;
+  uint8_t* v_exp;
+} gptb200_adamw8_state;
+int gptb200_adamw8_step(float* params, const gptb200_adamw8_state* state, const float* grads,
+                        int64_t n, const gptb200_tensor_group* groups, int32_t n_groups,
+                        const gptb200_adamw_config* cfg, int32_t* step, const float* loss,
+                        float* history, void* params_bf16, uint32_t seed, void* workspace,
+                        void* stream);
+/* One bucket, between gptb200_adamw_begin and gptb200_adamw_end; begin and end
+ * are multiples of 64. */
+int gptb200_adamw8_update_range(float* params, const gptb200_adamw8_state* state,
+                                const float* grads, int64_t begin, int64_t end,
+                                const gptb200_tensor_group* groups, int32_t n_groups,
+                                const gptb200_adamw_config* cfg, int32_t slot, void* params_bf16,
+                                uint32_t seed, void* workspace, void* stream);
+/* The values the codes stand for, m and sqrt(v), as bf16 [n] (exact); n a
+ * multiple of 64. */
+int gptb200_adamw8_values(const gptb200_adamw8_state* state, int64_t n, void* m, void* v_root,
+                          void* stream);
 
 /* fp32 -> bf16 copy of n elements (the compute-dtype cast of train.py's
  * `weight.astype(dtype)`). */
