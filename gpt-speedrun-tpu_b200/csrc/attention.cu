@@ -32,6 +32,25 @@
 // of the unrotated inputs.
 // Every mbarrier wait is bounded (common.cuh). Semantics follow
 // rig/kernels/tpu_flash_attention.py:171-207 (fp32 statistics, bf16 P).
+//
+// Both kernels take a MODE. kClassic is the plain causal attention above; the
+// others run the score-modified attention (gptb200_score_attention_fwd/bwd),
+//   s'_ij = cap tanh(scale q_i.k_j / cap) - slope_h |i - j|,
+// with key/value heads shared by heads / kv_heads query heads, a per-sequence
+// prefix whose keys every query sees, and segment ids whose negative values
+// mark padding (a row that sees nothing gets o = 0, lse = -inf and no
+// gradients). What they add to the softmax warps:
+//  * tanh. The exponentials already fill the MUFU pipe (one per score, 16 per
+//    clock and SM, against 512 clocks of MMA per 128 x 128 scores), so tanh
+//    runs on the FMA pipe: z P(z^2) with five terms, relative error 7e-6, where
+//    a warp's scores have |z| <= 1; only a warp that holds a larger one takes
+//    1 - 2 / (1 + e^(2z)), two more MUFU operations per score.
+//  * the bias. Linear in the key up to the query, so it is one packed FMA for
+//    two scores; |i - j| itself only near the diagonal and in the prefix.
+// The mask tests, the block lists and the loads stay as in kClassic. In the
+// backward an item is a key tile of a key/value head: it walks the query tiles
+// of every query head that shares it, so dK and dV of the group add up in TMEM,
+// in a fixed order.
 #include <algorithm>
 #include <atomic>
 #include <mutex>
@@ -48,9 +67,16 @@ constexpr int HD = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// Score modes of the kernels (bits of a MODE > kClassic: 1 general, 2 cap, 4 bias).
+enum { kClassic = 0, kGeneral = 1, kCap = 2, kBias = 4 };
+
 struct AttnParams {
-  int B, H, T;
+  int B, H, T;         // H: query heads
+  int KVH, group;      // key/value heads, query heads per key/value head (MODE > kClassic)
   float scale;
+  float cap;           // tanh cap of the scaled scores (kCap)
+  const float* slopes; // [H] distance slopes (kBias)
+  const int* prefix;   // [B] keys every query sees, or null (MODE > kClassic)
   // output / saved tensors
   bf16* o;
   int64_t osb, osh, ost;
@@ -168,6 +194,44 @@ __device__ __forceinline__ void sched_finish(unsigned* sched) {
   }
 }
 
+// ------------------------------------------------------------------ scores
+// tanh(z) / z in u = z^2 on |z| <= 1: minimax in relative error (7e-6) by
+// reweighted least squares over Chebyshev points.
+#define GPTB200_TANH_COEFS \
+  {0.999993085861206f, -0.3329806327819824f, 0.13036808371543884f, -0.04481752589344978f, \
+   0.009036410599946976f}
+
+GPTB200_DEV float2 tanh_small2(float2 z) {
+  constexpr float c[5] = GPTB200_TANH_COEFS;
+  const float2 u = fmul2(z, z);
+  float2 a = ffma2(u, make_float2(c[4], c[4]), make_float2(c[3], c[3]));
+  a = ffma2(u, a, make_float2(c[2], c[2]));
+  a = ffma2(u, a, make_float2(c[1], c[1]));
+  a = ffma2(u, a, make_float2(c[0], c[0]));
+  return fmul2(z, a);
+}
+// Any z: 1 - 2 / (1 + e^(2z)), an absolute error of a few 2^-24.
+GPTB200_DEV float tanh_any(float z) {
+  return fmaf(-2.f, __fdividef(1.f, 1.f + ex2(2.f * kLog2e * z)), 1.f);
+}
+
+// Padding (a negative id) never equals another id: queries carry -2, keys -1.
+template <bool GENERAL>
+GPTB200_DEV int seg_query_id(int v) {
+  return GENERAL && v < 0 ? -2 : v;
+}
+template <bool GENERAL>
+GPTB200_DEV int seg_key_id(int v) {
+  return GENERAL && v < 0 ? -1 : v;
+}
+// Range of a chunk's ids: a chunk of padding alone meets nothing, and a chunk
+// with some padding keeps -1 in its range, so that it is never a single id.
+template <bool GENERAL>
+GPTB200_DEV int2 seg_chunk(int mn, int mx) {
+  if (GENERAL && mn < 0) return mx < 0 ? make_int2(INT_MAX, INT_MIN) : make_int2(-1, mx);
+  return make_int2(mn, mx);
+}
+
 // ------------------------------------------------------------------ forward
 // Persistent: one CTA per SM walks work items (pair of 128-query tiles pr,
 // batch*head bh), item = bh * npair + (npair-1-pr), handed out by next_item.
@@ -186,7 +250,10 @@ constexpr int kFwdItemUsers = 2 + 8;   // both MMA threads, the 8 softmax warps
 // Item slot written by the TMA warp: pair, batch*head, key blocks the pair
 // visits (tile 0 the first n0 of them), whether tile 1 lies inside the sequence.
 struct FwdItem {
-  int pr, bh, nkv, n0, has1, pad0, pad1, pad2;
+  int pr, bh, nkv, n0, has1;
+  int nch;     // chunks of the segment table (MODE > kClassic)
+  int prefix;  // keys every query sees (MODE > kClassic)
+  int pad;
 };
 
 template <bool SEG>
@@ -205,11 +272,12 @@ struct FwdSmem {
   static constexpr int TOTAL = BAR + 256;
 };
 
-template <bool SEG>
+template <bool SEG, int MODE>
 __global__ void __launch_bounds__(kFwdThreads, 1)
     attn_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const AttnParams p) {
   using L = FwdSmem<SEG>;
+  constexpr bool GENERAL = MODE != kClassic;
   extern __shared__ __align__(1024) uint8_t smem_fwd[];
   uint8_t* sm = smem_fwd;
   if (smem_u32(sm) & 1023) {  // the layout needs 1024-byte aligned tiles: give up, flagged
@@ -309,7 +377,57 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       const int has1 = q0 + FQ < p.T;
       const int dmax = has1 ? d0 + 1 : d0;
       int nkv = dmax + 1, n0 = d0 + 1;
-      if constexpr (SEG) {
+      int hk = h, pf = 0, nch = 0;
+      if constexpr (GENERAL) {
+        hk = h / p.group;
+        if (p.prefix) {  // the prefix's blocks are seen by both tiles
+          pf = min(max(p.prefix[b], 0), p.T);
+          nkv = max(nkv, (pf + FK - 1) / FK);
+          n0 = max(n0, (pf + FK - 1) / FK);
+        }
+      }
+      if constexpr (SEG && GENERAL) {
+        // As below, over the blocks up to the diagonal or the prefix's end. A
+        // tile's diagonal block stays in the list even if nothing meets there
+        // (padding alone), so that every tile has a block and writes its rows.
+        const int* segrow = p.seg + (int64_t)b * p.T;
+        int2* tab = segtab_of(slot);
+        nch = min((p.T + kSegChunk - 1) / kSegChunk, 2 * nkv);
+        for (int c = 0; c < nch; ++c) {
+          int mn = INT_MAX, mx = INT_MIN;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int t = c * kSegChunk + u * 32 + lane;
+            if (t < p.T) {
+              const int v = segrow[t];
+              mn = min(mn, v);
+              mx = max(mx, v);
+            }
+          }
+          mn = __reduce_min_sync(0xffffffffu, mn);
+          mx = __reduce_max_sync(0xffffffffu, mx);
+          if (lane == 0) tab[c] = seg_chunk<true>(mn, mx);
+        }
+        __syncwarp();
+        if (lane == 0) {
+          int* bl = reinterpret_cast<int*>(sm + L::BLOCKS) + slot * (kMaxSegChunks / 2);
+          const int2 qr0 = seg_range(tab, nch, 2 * d0, 2);
+          const int2 qr1 = seg_range(tab, nch, 2 * d0 + 2, 2);
+          int n = 0, n_le0 = 0;
+          for (int j = 0; j < nkv; ++j) {
+            const int2 kr = seg_range(tab, nch, 2 * j, 2);
+            if (j == d0 || j == dmax || (j < n0 && rng_meet(kr, qr0)) ||
+                (has1 && rng_meet(kr, qr1))) {
+              bl[n++] = j;
+              if (j < n0) ++n_le0;
+            }
+          }
+          nkv = n;
+          n0 = n_le0;
+        }
+        nkv = __shfl_sync(0xffffffffu, nkv, 0);
+        n0 = __shfl_sync(0xffffffffu, n0, 0);
+      } else if constexpr (SEG) {
         // The key blocks 0..dmax either query tile can see, in order. Both
         // tiles walk this one list (tile 0 its prefix up to d0); a block only
         // the other tile needs is fully masked for a tile, at most costing its
@@ -355,7 +473,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         n0 = __shfl_sync(0xffffffffu, n0, 0);
       }
       if (lane == 0) {
-        items[slot] = FwdItem{pr, bh, nkv, n0, has1, 0, 0, 0};
+        items[slot] = FwdItem{pr, bh, nkv, n0, has1, nch, pf, 0};
         mbar_arrive(&item_full[slot]);
         if ((ok = mbar_wait(&q_empty[slot], ((ii >> 1) & 1) ^ 1, abort_flag, err))) {
           uint8_t* qd = sm + L::Q + slot * 2 * Q_BYTES;
@@ -368,8 +486,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           if (!(ok = mbar_wait(&kv_empty[s], ((gk / kKvStages) & 1) ^ 1, abort_flag, err))) break;
           mbar_arrive_expect_tx(&kv_full[s], 2 * KV_BYTES);
           const int key0 = kblock(slot, j) * FK;
-          tma_load_4d(sm + L::K + s * KV_BYTES, &tmK, &kv_full[s], 0, key0, h, b);
-          tma_load_4d(sm + L::V + s * KV_BYTES, &tmV, &kv_full[s], 0, key0, h, b);
+          tma_load_4d(sm + L::K + s * KV_BYTES, &tmK, &kv_full[s], 0, key0, hk, b);
+          tma_load_4d(sm + L::V + s * KV_BYTES, &tmV, &kv_full[s], 0, key0, hk, b);
         }
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
@@ -475,9 +593,15 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       const int qrow = q0 + x * FQ + r;
       const int* segrow = SEG ? p.seg + (int64_t)b * p.T : nullptr;
       const int2* segtab = SEG ? segtab_of(slot) : nullptr;
-      const int nch = min((p.T + kSegChunk - 1) / kSegChunk, 2 * (d0 + inf.has1 + 1));
+      const int nch = GENERAL ? inf.nch
+                              : min((p.T + kSegChunk - 1) / kSegChunk, 2 * (d0 + inf.has1 + 1));
       // this row's segment id (rows past T take an id no key has)
-      const int sq = segrow ? (qrow < p.T ? segrow[qrow] : INT_MIN) : 0;
+      const int sq = segrow ? (qrow < p.T ? seg_query_id<GENERAL>(segrow[qrow])
+                                          : (GENERAL ? -2 : INT_MIN))
+                            : 0;
+      // the last key this row sees under the causal and the prefix mask
+      const int last = GENERAL ? max(qrow, inf.prefix - 1) : qrow;
+      const float slope2 = (MODE & kBias) ? p.slopes[h] * kLog2e : 0.f;
       const int2 qrng = segrow ? seg_range(segtab, nch, 2 * (d0 + x), 2) : make_int2(0, 0);
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < nb && ok; ++j) {
@@ -485,7 +609,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         if (!(ok = mbar_wait(&s_full[x], jj & 1, abort_flag, err))) break;
         tc_fence_after();
         const int jb = kblock(slot, j);
-        const bool diag = (jb == d0 + x);  // keys past the query (and past T) are masked
+        // keys past the query (and past T) are masked
+        const bool diag = GENERAL ? jb * FK + FK - 1 > max(q0 + x * FQ, inf.prefix - 1)
+                                  : (jb == d0 + x);
+        const int rl = GENERAL ? last - jb * FK : r;  // last visible key of this block
         // Per-element segment test unless keys and queries all share one id;
         // the block's key ids then come through shared memory (double-buffered,
         // one mbarrier handshake across the warpgroup).
@@ -493,7 +620,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         const int* ks = kseg + (nseg & 1) * FK;
         if (segmask) {
           const int key = jb * FK + r;
-          kseg[(nseg & 1) * FK + r] = key < p.T ? segrow[key] : INT_MAX;
+          kseg[(nseg & 1) * FK + r] =
+              key < p.T ? seg_key_id<GENERAL>(segrow[key]) : (GENERAL ? -1 : INT_MAX);
           mbar_arrive(&kseg_full[2 * x + (nseg & 1)]);
           if (!(ok = mbar_wait(&kseg_full[2 * x + (nseg & 1)], (nseg >> 1) & 1, abort_flag, err)))
             break;
@@ -508,12 +636,73 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[x]);
+        auto visible = [&](int i) { return (!diag || i <= rl) && (!segmask || ks[i] == sq); };
+        // Capped and biased scores, in units of log2, in place of the raw ones.
+        if constexpr ((MODE & (kCap | kBias)) != 0) {
+          const float k = (MODE & kCap) ? p.scale / p.cap : 1.f;
+          const float a = (MODE & kCap) ? p.cap * kLog2e : c;
+          // key - query at this block's first key
+          const float at0 = (float)(jb * FK - qrow);
+          const float base = slope2 * at0;
+          const bool ahead = jb * FK + FK - 1 > q0 + x * FQ;  // some key is past some query
+          auto bias2 = [&](float2 y, int i, auto two_sided) {
+            if constexpr (!(MODE & kBias)) return y;
+            if constexpr (decltype(two_sided)::value)
+              return make_float2(fmaf(-slope2, fabsf(at0 + (float)i), y.x),
+                                 fmaf(-slope2, fabsf(at0 + (float)(i + 1)), y.y));
+            else
+              return fadd2(y, ffma2(make_float2(slope2, slope2),
+                                    make_float2((float)i, (float)(i + 1)),
+                                    make_float2(base, base)));
+          };
+          auto modify = [&](auto small, auto two_sided) {
+#pragma unroll
+            for (int i = 0; i < FK; i += 2) {
+              float2 y = make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+              if constexpr ((MODE & kCap) != 0) {
+                y = fmul2(y, make_float2(k, k));
+                if constexpr (decltype(small)::value)
+                  y = tanh_small2(y);
+                else
+                  y = make_float2(tanh_any(y.x), tanh_any(y.y));
+              }
+              y = bias2(fmul2(y, make_float2(a, a)), i, two_sided);
+              v[i] = __float_as_uint(y.x);
+              v[i + 1] = __float_as_uint(y.y);
+            }
+          };
+          bool large = false;
+          if constexpr ((MODE & kCap) != 0) {
+            if (diag || segmask) {  // hidden scores do not choose the form of tanh
+#pragma unroll
+              for (int i = 0; i < FK; ++i)
+                if (!visible(i)) v[i] = 0;
+            }
+            float t8[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) t8[u] = 0.f;
+#pragma unroll
+            for (int i = 0; i < FK; i += 2)
+              t8[(i >> 1) & 7] = fmax3(t8[(i >> 1) & 7], fabsf(__uint_as_float(v[i])),
+                                       fabsf(__uint_as_float(v[i + 1])));
+            const float top = fmaxf(fmax3(t8[0], t8[1], t8[2]),
+                                    fmax3(t8[3], t8[4], fmaxf(t8[5], fmaxf(t8[6], t8[7]))));
+            large = __any_sync(0xffffffffu, top * k > 1.f);
+          }
+          const std::true_type yes;
+          const std::false_type no;
+          if (large)
+            modify(no, yes);
+          else if ((MODE & kBias) && ahead)
+            modify(yes, yes);
+          else
+            modify(yes, no);
+        }
         // Row max of the raw scores (c > 0 commutes with the max), eight
         // independent chains; on the diagonal block keys past the query are out.
         float m8[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) m8[u] = -INFINITY;
-        auto visible = [&](int i) { return (!diag || i <= r) && (!segmask || ks[i] == sq); };
         if (diag || segmask) {
 #pragma unroll
           for (int i = 0; i < FK; i += 2)
@@ -525,8 +714,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             m8[(i >> 1) & 7] =
                 fmax3(m8[(i >> 1) & 7], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
         }
+        const float unit = (MODE & (kCap | kBias)) ? 1.f : c;  // of v in log2
         const float mx =
-            fmaxf(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], fmaxf(m8[5], fmaxf(m8[6], m8[7])))) * c;
+            fmaxf(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], fmaxf(m8[5], fmaxf(m8[6], m8[7])))) * unit;
         // The rescale decision is made per warp: the TMEM loads/stores of O are
         // warp-collective and must not run in a divergent branch. Rows whose
         // max did not move rescale by exactly 1.
@@ -542,13 +732,19 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         // P = exp2(s*c - m) packed to bf16 pairs in registers (the S registers
         // die as P is produced); four packed partial row sums.
         const float2 c2 = make_float2(c, c), nm2 = make_float2(-m_used, -m_used);
+        const auto shifted = [&](float2 y) {
+          if constexpr ((MODE & (kCap | kBias)) != 0)
+            return fadd2(y, nm2);
+          else
+            return ffma2(y, c2, nm2);
+        };
         float2 acc[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) acc[u] = make_float2(0.f, 0.f);
         uint32_t pk[FK / 2];
 #pragma unroll
         for (int i = 0; i < FK; i += 2) {
-          const float2 t = ffma2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), c2, nm2);
+          const float2 t = shifted(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
           float p0 = ex2(t.x), p1 = ex2(t.y);
           if (diag || segmask) {
             if (!visible(i)) p0 = 0.f;
@@ -586,7 +782,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       if (ok && nb > 0) {
         if (!(ok = mbar_wait(&pv_done[x], (jx + nb - 1) & 1, abort_flag, err))) break;
         tc_fence_after();
-        const float inv = 1.f / l;
+        // a row that sees no key: zeros, lse -inf
+        const float inv = GENERAL && l == 0.f ? 0.f : 1.f / l;
         float o[32];
         bf16* orow = p.o + b * p.osb + h * p.osh + (int64_t)qrow * p.ost;
 #pragma unroll
@@ -604,7 +801,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             }
           }
         }
-        if (qrow < p.T) p.lse[(int64_t)bh * p.T + qrow] = (m_used + __log2f(l)) * kLn2;
+        if (qrow < p.T)
+          p.lse[(int64_t)bh * p.T + qrow] =
+              GENERAL && l == 0.f ? -INFINITY : (m_used + __log2f(l)) * kLn2;
       }
       if (!ok) break;
       tc_fence_before();
@@ -651,8 +850,11 @@ constexpr int kBwdItemUsers = 2 + kBwdSmWarps + 4;
 // tiles (always even: an odd count gets one tile past the sequence end, whose
 // rows load as zeros and carry no probability, so query pairs never straddle
 // two items).
+// MODE > kClassic: bh counts key/value heads and the list is walked once per
+// query head of the group, nq1 tiles each (nq = group * nq1); tile indexes
+// count from position qb, 0 where the key tile reaches into the prefix.
 struct BwdItem {
-  int kt, bh, nq, pad;
+  int kt, bh, nq, nq1, qb, prefix, pad0, pad1;
 };
 
 template <bool SEG>
@@ -670,19 +872,20 @@ struct BwdSmem {
   static constexpr int ITEM = STAT + kQStages * kStatBytes;  // 2 BwdItem slots
   // segment ids only: per slot, (min, max) id per 64-position chunk from k0
   // and the list of query tiles that can see the key tile
-  static constexpr int SEGTAB = ITEM + 32;
+  static constexpr int SEGTAB = ITEM + 64;
   static constexpr int QLIST = SEGTAB + (SEG ? 2 * kMaxSegChunks * 8 : 0);
   static constexpr int BAR = QLIST + (SEG ? 2 * kMaxSegChunks * 4 : 0);
   // the dynamic shared memory base is 1024-byte aligned (checked at entry)
   static constexpr int TOTAL = BAR + 272;
 };
 
-template <bool SEG, int GROUPS>
+template <bool SEG, int GROUPS, int MODE>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attn_bwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
                 const __grid_constant__ CUtensorMap tmDQ, const AttnParams p) {
   using L = BwdSmem<SEG>;
+  constexpr bool GENERAL = MODE != kClassic;
   constexpr int kQS = L::kQStages;
   constexpr int kBwdSmGroups = GROUPS;
   constexpr int kBwdGroupWarps = kBwdSmWarps / kBwdSmGroups;
@@ -715,7 +918,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   BwdItem* items = reinterpret_cast<BwdItem*>(sm + L::ITEM);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int BH = p.B * p.H;
+  const int heads = GENERAL ? p.KVH : p.H;
+  const int BH = p.B * heads;
   const int n_items = ((p.T + BT - 1) / BT) * BH;  // item = bh * nkt + kt
   int* err = &g_attn_error;
   // query tile (64-position index past k0) of list entry `it` of the item in `slot`
@@ -783,11 +987,50 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       const int nkt = (p.T + BT - 1) / BT;
       const int bh = item / nkt, kt = item - bh * nkt;
-      const int b = bh / p.H, h = bh - b * p.H;
+      const int b = bh / heads, h = bh - b * heads;
       const int k0 = kt * BT;
-      const int nq_all = (p.T - k0 + BQ - 1) / BQ;  // 64-query tiles from the diagonal on
+      int qb = k0, pf = 0;
+      if constexpr (GENERAL) {
+        if (p.prefix) {
+          pf = min(max(p.prefix[b], 0), p.T);
+          if (k0 < pf) qb = 0;  // queries before the diagonal see the prefix's keys
+        }
+      }
+      const int nq_all = (p.T - qb + BQ - 1) / BQ;  // 64-query tiles from the diagonal on
       int nq = nq_all;
-      if constexpr (SEG) {
+      if constexpr (SEG && GENERAL) {
+        // as below, from position qb; without a visible tile two tiles past the
+        // sequence end remain, which leave dK and dV zero
+        const int* segrow = p.seg + (int64_t)b * p.T;
+        int2* tab = segtab_of(slot);
+        const int nch = (p.T + kSegChunk - 1) / kSegChunk - qb / kSegChunk;
+        for (int c = 0; c < nch; ++c) {
+          int mn = INT_MAX, mx = INT_MIN;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int t = qb + c * kSegChunk + u * 32 + lane;
+            if (t < p.T) {
+              const int v = segrow[t];
+              mn = min(mn, v);
+              mx = max(mx, v);
+            }
+          }
+          mn = __reduce_min_sync(0xffffffffu, mn);
+          mx = __reduce_max_sync(0xffffffffu, mx);
+          if (lane == 0) tab[c] = seg_chunk<true>(mn, mx);
+        }
+        __syncwarp();
+        if (lane == 0) {
+          int* ql = reinterpret_cast<int*>(sm + L::QLIST) + slot * kMaxSegChunks;
+          const int2 kr = seg_range(tab, nch, (k0 - qb) / kSegChunk, 2);
+          int n = 0;
+          for (int it = 0; it < nq_all; ++it)
+            if (rng_meet(seg_range(tab, nch, it, 1), kr)) ql[n++] = it;
+          while ((n & 1) || n == 0) ql[n++] = nq_all;
+          nq = n;
+        }
+        nq = __shfl_sync(0xffffffffu, nq, 0);
+      } else if constexpr (SEG) {
         // (min, max) segment id per 64-position chunk from k0, then the query
         // tiles whose ids can meet this key tile's, in order
         const int* segrow = p.seg + (int64_t)b * p.T;
@@ -825,8 +1068,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       } else {
         nq += nq & 1;
       }
+      const int nq1 = nq;
+      if constexpr (GENERAL) nq *= p.group;
       if (lane == 0) {
-        items[slot] = BwdItem{kt, bh, nq, 0};
+        items[slot] = BwdItem{kt, bh, nq, nq1, qb, pf, 0, 0};
         mbar_arrive(&item_full[slot]);
         const int kvs = ii & 1;
         ok = mbar_wait(&kv_empty[kvs], ((ii >> 1) & 1) ^ 1, abort_flag, err);
@@ -838,17 +1083,26 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-      const float* Lg = p.lse + (int64_t)bh * p.T;
-      const float* Dg = p.delta + (int64_t)bh * p.T;
-      for (int it = 0; ok && it < nq; ++it, ++g) {
+      // query head: the key/value head's own, or the first of its group
+      int hq = GENERAL ? h * p.group : h;
+      const float* Lg = p.lse + ((int64_t)b * p.H + hq) * p.T;
+      const float* Dg = p.delta + ((int64_t)b * p.H + hq) * p.T;
+      int ql = 0;  // entry of the head's list
+      for (int it = 0; ok && it < nq; ++it, ++ql, ++g) {
+        if (GENERAL && ql == nq1) {  // the group's next head
+          ql = 0;
+          ++hq;
+          Lg += p.T;
+          Dg += p.T;
+        }
         const int s = g % kQS;
-        const int qq = k0 + qtile(slot, it) * BQ;
+        const int qq = qb + qtile(slot, ql) * BQ;
         if (lane == 0) {
           ok = mbar_wait(&q_empty[s], ((g / kQS) & 1) ^ 1, abort_flag, err);
           if (ok) {
             mbar_arrive_expect_tx(&q_full[s], 2 * BQ_BYTES);
-            tma_load_4d(sm + L::Q + s * BQ_BYTES, &tmQ, &q_full[s], 0, qq, h, b);
-            tma_load_4d(sm + L::DO + s * BQ_BYTES, &tmDO, &q_full[s], 0, qq, h, b);
+            tma_load_4d(sm + L::Q + s * BQ_BYTES, &tmQ, &q_full[s], 0, qq, hq, b);
+            tma_load_4d(sm + L::DO + s * BQ_BYTES, &tmDO, &q_full[s], 0, qq, hq, b);
           }
         }
         if (!(ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0)) break;
@@ -986,20 +1240,33 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const BwdItem inf = items[slot];
       if (inf.nq < 0) break;  // no more items
       const int nq = inf.nq;
-      const int b = inf.bh / p.H;
+      const int b = inf.bh / heads;
       const int k0 = inf.kt * BT;
       const int key = k0 + r;
+      const int qoff = GENERAL ? inf.qb - k0 : 0;  // first query tile relative to the keys
+      // this key's row is seen by every query of its sequence
+      const bool open = GENERAL && key < inf.prefix;
+      int ql = wg, hq = GENERAL ? (inf.bh - b * heads) * p.group : 0;
       const int* segrow = SEG ? p.seg + (int64_t)b * p.T : nullptr;
       const int2* segtab = SEG ? segtab_of(slot) : nullptr;
-      const int nch = (p.T + kSegChunk - 1) / kSegChunk - 2 * inf.kt;
+      const int nch = (p.T + kSegChunk - 1) / kSegChunk -
+                      (GENERAL ? inf.qb / kSegChunk : 2 * inf.kt);
       // this key row's segment id (rows past T take an id no query has)
-      const int sk = segrow ? (key < p.T ? segrow[key] : INT_MAX) : 0;
-      const int2 krng = segrow ? seg_range(segtab, nch, 0, 2) : make_int2(0, 0);
-      for (int it = wg; it < nq; it += kBwdSmGroups) {
+      const int sk = segrow ? (key < p.T ? seg_key_id<GENERAL>(segrow[key])
+                                         : (GENERAL ? -1 : INT_MAX))
+                            : 0;
+      const int2 krng =
+          segrow ? seg_range(segtab, nch, -qoff / kSegChunk, 2) : make_int2(0, 0);
+      for (int it = wg; it < nq; it += kBwdSmGroups, ql += kBwdSmGroups) {
+        if (GENERAL && ql >= inf.nq1) {  // the group's next head
+          ql -= inf.nq1;
+          ++hq;
+        }
         const int gt = g + it;  // running tile index
         const int bb = gt % 3;
         const uint32_t tb = tBuf(bb);
-        const int qt = qtile(slot, it);  // query tile index (64 positions) past k0
+        const int qt = qtile(slot, GENERAL ? ql : it);  // query tile index (64 positions) past k0
+        const float slope2 = (MODE & kBias) ? p.slopes[hq] * kLog2e : 0.f;
         if (!(ok = mbar_wait(&s_full[bb], (gt / 3) & 1, abort_flag, err))) break;
         if (!(ok = mbar_wait(&q_full[gt % kQS], (gt / kQS) & 1, abort_flag, err))) break;
         // The dS^T ring slot of this tile was last read by the dQ MMA of the
@@ -1020,8 +1287,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tmem_ld16_nw(tb + lane_off + cg * 16, sraw);
         tmem_ld16_nw(tb + 64 + lane_off + cg * 16, draw);
         tmem_wait_ld();
-        const int qbase = qt * BQ + cg * 16;  // query index relative to k0
-        const bool diag = (qt < 2);           // key r > query masks only near the diagonal
+        const int qbase = qoff + qt * BQ + cg * 16;  // query index relative to k0
+        // key r > query masks only near (with a prefix, before) the diagonal
+        const bool diag = GENERAL ? qoff + qt * BQ < BT : (qt < 2);
         const int tail = p.T - k0 - qbase;    // columns j >= tail lie past the sequence end
         const bool mask = diag || tail < 16;
         // per-element segment test unless this key tile and query tile share one id
@@ -1031,21 +1299,68 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         // tests run only on tiles that need them and the segment test only
         // when the tiles' ids differ.
         uint32_t pk[8], dk[8];
+        // tanh's short form needs |z| <= 1 of this warp's scores
+        const float kcap = (MODE & kCap) ? p.scale / p.cap : 0.f;
+        bool large = false;
+        if constexpr ((MODE & kCap) != 0) {
+          if (mask || segmask) {  // hidden scores do not choose the form
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if ((diag && !open && r > qbase + j) || j >= tail ||
+                  (SEG && segmask && (stat_seg[j] != sk || stat_seg[j] < 0)))
+                sraw[j] = 0;
+          }
+          float top = 0.f;
+#pragma unroll
+          for (int j = 0; j < 16; j += 2)
+            top = fmax3(top, fabsf(__uint_as_float(sraw[j])), fabsf(__uint_as_float(sraw[j + 1])));
+          large = __any_sync(0xffffffffu, top * kcap > 1.f);
+        }
         auto softmax_cols = [&](auto mask_tag) {
           constexpr bool kMask = decltype(mask_tag)::value;
-          const float2 c2 = make_float2(c, c);
+          const float2 c2 = (MODE & kCap) ? make_float2(p.cap * kLog2e, p.cap * kLog2e)
+                                          : make_float2(c, c);
           const float2 nlog2e = make_float2(-kLog2e, -kLog2e);
           const float2 m1 = make_float2(-1.f, -1.f);
 #pragma unroll
           for (int j4 = 0; j4 < 4; ++j4) {
             const float4 l4 = reinterpret_cast<const float4*>(stat)[j4];
             const float4 d4 = reinterpret_cast<const float4*>(stat + 64)[j4];
-            const float2 x01 = ffma2(make_float2(__uint_as_float(sraw[4 * j4]),
-                                                 __uint_as_float(sraw[4 * j4 + 1])),
-                                     c2, fmul2(make_float2(l4.x, l4.y), nlog2e));
-            const float2 x23 = ffma2(make_float2(__uint_as_float(sraw[4 * j4 + 2]),
-                                                 __uint_as_float(sraw[4 * j4 + 3])),
-                                     c2, fmul2(make_float2(l4.z, l4.w), nlog2e));
+            float2 s01 = make_float2(__uint_as_float(sraw[4 * j4]), __uint_as_float(sraw[4 * j4 + 1]));
+            float2 s23 = make_float2(__uint_as_float(sraw[4 * j4 + 2]),
+                                     __uint_as_float(sraw[4 * j4 + 3]));
+            [[maybe_unused]] float2 slope01, slope23;  // d s' / d (scaled score)
+            if constexpr ((MODE & kCap) != 0) {
+              const float2 k2 = make_float2(kcap, kcap), one = make_float2(1.f, 1.f);
+              s01 = fmul2(s01, k2);
+              s23 = fmul2(s23, k2);
+              if (large) {
+                s01 = make_float2(tanh_any(s01.x), tanh_any(s01.y));
+                s23 = make_float2(tanh_any(s23.x), tanh_any(s23.y));
+              } else {
+                s01 = tanh_small2(s01);
+                s23 = tanh_small2(s23);
+              }
+              slope01 = ffma2(make_float2(-s01.x, -s01.y), s01, one);
+              slope23 = ffma2(make_float2(-s23.x, -s23.y), s23, one);
+            }
+            float2 n01 = fmul2(make_float2(l4.x, l4.y), nlog2e);
+            float2 n23 = fmul2(make_float2(l4.z, l4.w), nlog2e);
+            if constexpr ((MODE & kBias) != 0) {
+              const float at = (float)(r - qbase - 4 * j4);  // key - query of column 4 j4
+              if (diag) {
+                n01.x = fmaf(-slope2, fabsf(at), n01.x);
+                n01.y = fmaf(-slope2, fabsf(at - 1.f), n01.y);
+                n23.x = fmaf(-slope2, fabsf(at - 2.f), n23.x);
+                n23.y = fmaf(-slope2, fabsf(at - 3.f), n23.y);
+              } else {  // no key past a query
+                const float2 sl = make_float2(slope2, slope2);
+                n01 = ffma2(sl, make_float2(at, at - 1.f), n01);
+                n23 = ffma2(sl, make_float2(at - 2.f, at - 3.f), n23);
+              }
+            }
+            const float2 x01 = ffma2(s01, c2, n01);
+            const float2 x23 = ffma2(s23, c2, n23);
             float pv[4] = {ex2(x01.x), ex2(x01.y), ex2(x23.x), ex2(x23.y)};
             // dP^T - delta as fma(delta, -1, dP^T): one rounding, as a subtraction
             const float2 g01 = ffma2(make_float2(d4.x, d4.y), m1,
@@ -1056,13 +1371,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                                                  __uint_as_float(draw[4 * j4 + 3])));
             float2 dv01 = fmul2(make_float2(pv[0], pv[1]), g01);
             float2 dv23 = fmul2(make_float2(pv[2], pv[3]), g23);
+            if constexpr ((MODE & kCap) != 0) {
+              dv01 = fmul2(dv01, slope01);
+              dv23 = fmul2(dv23, slope23);
+            }
             float dvs[4] = {dv01.x, dv01.y, dv23.x, dv23.y};
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
               const int j = 4 * j4 + u;
               bool off = false;
-              if (kMask) off = (diag && r > qbase + j) || j >= tail;
-              if (SEG && segmask && stat_seg[j] != sk) off = true;
+              if (kMask) off = (diag && !open && r > qbase + j) || j >= tail;
+              if (SEG && segmask &&
+                  (stat_seg[j] != sk || (GENERAL && stat_seg[j] < 0)))
+                off = true;
               if (off) pv[u] = dvs[u] = 0.f;
             }
             dv01 = make_float2(dvs[0], dvs[1]);
@@ -1117,7 +1438,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const BwdItem inf = items[slot];
       if (inf.nq < 0) break;  // no more items
       const int k0 = inf.kt * BT;
-      for (int j = 0; j < inf.nq / 2; ++j) {
+      int ql = 0, bhq = inf.bh;  // the pair's list entry and its row block of dq_acc
+      if constexpr (GENERAL) bhq = inf.bh / heads * p.H + inf.bh % heads * p.group;
+      for (int j = 0; j < inf.nq / 2; ++j, ql += 2) {
+        if (GENERAL && ql == inf.nq1) {
+          ql = 0;
+          ++bhq;
+        }
         const int J = (g >> 1) + j;  // running pair index
         if (!(ok = mbar_wait(&dq_full[J & 1], (J >> 1) & 1, abort_flag, err))) break;
         tc_fence_after();
@@ -1128,7 +1455,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&dq_free[J & 1]);
-        const int row0 = k0 + qtile(slot, 2 * j + (quad >> 1)) * BQ + (quad & 1) * 32;
+        const int row0 = (GENERAL ? inf.qb : k0) + qtile(slot, ql + (quad >> 1)) * BQ +
+                         (quad & 1) * 32;
         if (row0 < p.T) {  // warp-uniform
           if (lane == 0) bulk_wait_read();  // the previous reduce has read the staging boxes
           __syncwarp();
@@ -1142,8 +1470,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            tma_reduce_add_3d(&tmDQ, stage, 0, row0, inf.bh);
-            tma_reduce_add_3d(&tmDQ, stage + 4096, 32, row0, inf.bh);
+            tma_reduce_add_3d(&tmDQ, stage, 0, row0, bhq);
+            tma_reduce_add_3d(&tmDQ, stage + 4096, 32, row0, bhq);
             bulk_commit();
           }
         }
@@ -1157,7 +1485,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tc_fence_after();
       {
         const int key = k0 + quad * 32 + lane;
-        const int bi = inf.bh / p.H, hi = inf.bh - bi * p.H;
+        const int bi = inf.bh / heads, hi = inf.bh - bi * heads;
         if (lane == 0) bulk_wait_read();  // the last dQ reduce has read the staging area
         __syncwarp();
         float* park = reinterpret_cast<float*>(stage);  // [32 rows][64] fp32, 16-byte chunks xor-swizzled
@@ -1228,8 +1556,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 // delta[bh, t] = sum_e dO * O, and zero the dQ accumulator row. Eight lanes
 // per row (16-byte loads), four rows per warp.
 __global__ void attn_delta_kernel(const bf16* __restrict__ o, const bf16* __restrict__ dout,
-                                  int64_t osb, int64_t osh, int64_t ost, int B, int H, int T,
-                                  float* __restrict__ delta, float* __restrict__ dq_acc) {
+                                  int64_t osb, int64_t osh, int64_t ost, int64_t gsb, int64_t gsh,
+                                  int64_t gst, int B, int H, int T, float* __restrict__ delta,
+                                  float* __restrict__ dq_acc) {
   const int64_t rows = (int64_t)B * H * T;
   const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
   const int seg = threadIdx.x & 7;
@@ -1239,8 +1568,9 @@ __global__ void attn_delta_kernel(const bf16* __restrict__ o, const bf16* __rest
   const int t = (int)(rr - bh * T);
   const int b = (int)(bh / H), h = (int)(bh - (int64_t)b * H);
   const int64_t off = b * osb + h * osh + (int64_t)t * ost + seg * 8;
+  const int64_t goff = b * gsb + h * gsh + (int64_t)t * gst + seg * 8;
   const uint4 qo = *reinterpret_cast<const uint4*>(o + off);
-  const uint4 qg = *reinterpret_cast<const uint4*>(dout + off);
+  const uint4 qg = *reinterpret_cast<const uint4*>(dout + goff);
   const uint32_t* wo = &qo.x;
   const uint32_t* wg = &qg.x;
   float s = 0.f;
@@ -1347,9 +1677,18 @@ static bool make_map4(CUtensorMap* m, const void* base, int B, int H, int T, int
   cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
   cuuint32_t box[4] = {HD, (cuuint32_t)box_rows, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box,
-             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  auto encode = [&] {
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box,
+               estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+    // a thread that has not used the device yet (autograd's): bind its context
+    cudaFree(nullptr);
+    r = encode();
+  }
+  return r == CUDA_SUCCESS;
 }
 
 }  // namespace gptb200
@@ -1419,7 +1758,7 @@ extern "C" int gptb200_attention_fwd(const void* q, const void* k, const void* v
   int dev = 0;
   cudaGetDevice(&dev);
   const int seg = segment_ids != nullptr;
-  auto kern = seg ? attn_fwd_tc<true> : attn_fwd_tc<false>;
+  auto kern = seg ? attn_fwd_tc<true, kClassic> : attn_fwd_tc<false, kClassic>;
   const int smem = seg ? FwdSmem<true>::TOTAL : FwdSmem<false>::TOTAL;
   int sms = 148;
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -1476,7 +1815,7 @@ extern "C" int gptb200_attention_bwd(const void* q, const void* k, const void* v
                                            (rows * 4 + 255) / 256 * 256);
   attn_delta_kernel<<<(unsigned)((rows * 8 + 255) / 256), 256, 0, st>>>(
       reinterpret_cast<const bf16*>(o), reinterpret_cast<const bf16*>(dout), o_stride_b,
-      o_stride_h, o_stride_t, B, H, T, delta, dq_acc);
+      o_stride_h, o_stride_t, o_stride_b, o_stride_h, o_stride_t, B, H, T, delta, dq_acc);
   GPTB200_CHECK_LAUNCH();
   AttnParams p = {};
   p.B = B;
@@ -1501,8 +1840,9 @@ extern "C" int gptb200_attention_bwd(const void* q, const void* k, const void* v
   cudaGetDevice(&dev);
   const int seg = segment_ids != nullptr;
   const int groups = seq >= 2048 ? 2 : 1;
-  auto kern = seg ? (groups == 2 ? attn_bwd_tc<true, 2> : attn_bwd_tc<true, 1>)
-                  : (groups == 2 ? attn_bwd_tc<false, 2> : attn_bwd_tc<false, 1>);
+  auto kern = seg ? (groups == 2 ? attn_bwd_tc<true, 2, kClassic> : attn_bwd_tc<true, 1, kClassic>)
+                  : (groups == 2 ? attn_bwd_tc<false, 2, kClassic>
+                                 : attn_bwd_tc<false, 1, kClassic>);
   const int smem = seg ? BwdSmem<true>::TOTAL : BwdSmem<false>::TOTAL;
   int sms = 148;
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -1525,6 +1865,186 @@ extern "C" int gptb200_attention_bwd(const void* q, const void* k, const void* v
                                                stride_h, stride_t, B, H, T, softmax_scale,
                                                reinterpret_cast<const bf16*>(rope_cos),
                                                reinterpret_cast<const bf16*>(rope_sin));
+  GPTB200_CHECK_LAUNCH();
+  return 0;
+}
+
+// ------------------------------------------------------------------ score-modified attention
+namespace gptb200 {
+
+// Everything about a call that is checked or looked up before a launch.
+static int score_check(const gptb200_score_attention* a) {
+  if (!a || !a->q || !a->k || !a->v || !a->o || !a->lse) return GPTB200_EINVAL;
+  if (a->batch <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->seq <= 0) return GPTB200_EINVAL;
+  if (!(a->softmax_scale > 0.f) || !(a->softcap >= 0.f) || isinf(a->softcap) ||
+      isinf(a->softmax_scale))
+    return GPTB200_EINVAL;
+  if (a->head_dim != HD || a->heads % a->kv_heads) return GPTB200_EUNSUPPORTED;
+  if (a->batch * a->heads > 65535 || a->seq > (1 << 24)) return GPTB200_ESHAPE;
+  if (a->segment_ids && a->seq > (int64_t)kMaxSegChunks * kSegChunk) return GPTB200_EUNSUPPORTED;
+  int64_t strides = 0;
+  for (int i = 0; i < 3; ++i) strides |= a->q_stride[i] | a->kv_stride[i] | a->o_stride[i];
+  if (strides % 8) return GPTB200_ESHAPE;
+  if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) |
+       reinterpret_cast<uintptr_t>(a->v) | reinterpret_cast<uintptr_t>(a->o)) & 15)
+    return GPTB200_ESHAPE;
+  if ((reinterpret_cast<uintptr_t>(a->segment_ids) | reinterpret_cast<uintptr_t>(a->prefix_lens) |
+       reinterpret_cast<uintptr_t>(a->slopes) | reinterpret_cast<uintptr_t>(a->lse)) & 3)
+    return GPTB200_ESHAPE;
+  return 0;
+}
+
+static AttnParams score_params(const gptb200_score_attention* a) {
+  AttnParams p = {};
+  p.B = (int)a->batch;
+  p.H = (int)a->heads;
+  p.T = (int)a->seq;
+  p.KVH = (int)a->kv_heads;
+  p.group = p.H / p.KVH;
+  p.scale = a->softmax_scale;
+  p.cap = a->softcap;
+  p.slopes = a->slopes;
+  p.prefix = a->prefix_lens;
+  p.o = reinterpret_cast<bf16*>(a->o);
+  p.osb = a->o_stride[0];
+  p.osh = a->o_stride[1];
+  p.ost = a->o_stride[2];
+  p.lse = a->lse;
+  p.seg = a->segment_ids;
+  return p;
+}
+
+// One persistent launch: the shared-memory attribute (set once per kernel and
+// device) and one CTA per SM or item.
+template <typename K, typename... Args>
+static int launch_persistent(K kern, bool (&done)[64], int64_t items, int threads, int smem,
+                             cudaStream_t st, Args... args) {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (dev >= 64 || !done[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return -static_cast<int>(e);
+    if (dev < 64) done[dev] = true;
+  }
+  kern<<<(unsigned)std::min<int64_t>(items, sms), threads, smem, st>>>(args...);
+  GPTB200_CHECK_LAUNCH();
+  return 0;
+}
+
+struct ScoreMaps {
+  CUtensorMap q, k, v, g, dq;
+};
+
+template <bool SEG, int MODE>
+static int score_fwd_launch(const AttnParams& p, const ScoreMaps& m, cudaStream_t st) {
+  static bool done[64] = {};
+  const int64_t items = (int64_t)((p.T + 2 * FQ - 1) / (2 * FQ)) * p.B * p.H;
+  return launch_persistent(attn_fwd_tc<SEG, MODE>, done, items, kFwdThreads, FwdSmem<SEG>::TOTAL,
+                           st, m.q, m.k, m.v, p);
+}
+
+template <bool SEG, int GROUPS, int MODE>
+static int score_bwd_launch(const AttnParams& p, const ScoreMaps& m, cudaStream_t st) {
+  static bool done[64] = {};
+  const int64_t items = (int64_t)((p.T + BT - 1) / BT) * p.B * p.KVH;
+  return launch_persistent(attn_bwd_tc<SEG, GROUPS, MODE>, done, items, kBwdThreads,
+                           BwdSmem<SEG>::TOTAL, st, m.q, m.k, m.v, m.g, m.dq, p);
+}
+
+// f<MODE>() for the call's cap and bias.
+template <typename F>
+static int score_mode(const gptb200_score_attention* a, F&& f) {
+  if (a->softcap > 0.f)
+    return a->slopes ? f(std::integral_constant<int, kGeneral | kCap | kBias>())
+                     : f(std::integral_constant<int, kGeneral | kCap>());
+  return a->slopes ? f(std::integral_constant<int, kGeneral | kBias>())
+                   : f(std::integral_constant<int, kGeneral>());
+}
+
+}  // namespace gptb200
+
+extern "C" int gptb200_score_attention_fwd(const gptb200_score_attention* a, void* stream) {
+  const int s = score_check(a);
+  if (s) return s;
+  AttnParams p = score_params(a);
+  ScoreMaps m;
+  const int64_t *qs = a->q_stride, *ks = a->kv_stride;
+  if (!make_map4(&m.q, a->q, p.B, p.H, p.T, qs[0], qs[1], qs[2], FQ) ||
+      !make_map4(&m.k, a->k, p.B, p.KVH, p.T, ks[0], ks[1], ks[2], FK) ||
+      !make_map4(&m.v, a->v, p.B, p.KVH, p.T, ks[0], ks[1], ks[2], FK))
+    return GPTB200_ESHAPE;
+  p.sched = sched_slot(0);
+  if (!p.sched) return GPTB200_EUNSUPPORTED;
+  auto st = reinterpret_cast<cudaStream_t>(stream);
+  return score_mode(a, [&](auto mode) {
+    constexpr int MODE = decltype(mode)::value;
+    return p.seg ? score_fwd_launch<true, MODE>(p, m, st) : score_fwd_launch<false, MODE>(p, m, st);
+  });
+}
+
+extern "C" int gptb200_score_attention_bwd(const gptb200_score_attention* a, const void* dout,
+                                           const int64_t* dout_stride, void* dq, void* dk, void* dv,
+                                           const int64_t* dq_stride, const int64_t* dkv_stride,
+                                           const void* rope_cos, const void* rope_sin,
+                                           void* workspace, void* stream) {
+  const int s = score_check(a);
+  if (s) return s;
+  if (!dout || !dout_stride || !dq || !dk || !dv || !dq_stride || !dkv_stride || !workspace)
+    return GPTB200_EINVAL;
+  if ((rope_cos == nullptr) != (rope_sin == nullptr)) return GPTB200_EINVAL;
+  int64_t strides = 0;
+  for (int i = 0; i < 3; ++i) strides |= dout_stride[i] | dq_stride[i] | dkv_stride[i];
+  if (strides % 8) return GPTB200_ESHAPE;
+  if ((reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dq) |
+       reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) |
+       reinterpret_cast<uintptr_t>(workspace)) & 15)
+    return GPTB200_ESHAPE;
+  AttnParams p = score_params(a);
+  const int64_t rows = a->batch * a->heads * a->seq;
+  float* delta = reinterpret_cast<float*>(workspace);
+  float* dq_acc = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) +
+                                           (rows * 4 + 255) / 256 * 256);
+  ScoreMaps m;
+  const int64_t *qs = a->q_stride, *ks = a->kv_stride;
+  if (!make_map4(&m.q, a->q, p.B, p.H, p.T, qs[0], qs[1], qs[2], BQ) ||
+      !make_map4(&m.k, a->k, p.B, p.KVH, p.T, ks[0], ks[1], ks[2], BT) ||
+      !make_map4(&m.v, a->v, p.B, p.KVH, p.T, ks[0], ks[1], ks[2], BT) ||
+      !make_map4(&m.g, dout, p.B, p.H, p.T, dout_stride[0], dout_stride[1], dout_stride[2], BQ) ||
+      !make_dq_map(&m.dq, dq_acc, p.B * p.H, p.T))
+    return GPTB200_ESHAPE;
+  p.sched = sched_slot(1);
+  if (!p.sched) return GPTB200_EUNSUPPORTED;
+  auto st = reinterpret_cast<cudaStream_t>(stream);
+  attn_delta_kernel<<<(unsigned)((rows * 8 + 255) / 256), 256, 0, st>>>(
+      p.o, reinterpret_cast<const bf16*>(dout), p.osb, p.osh, p.ost, dout_stride[0], dout_stride[1],
+      dout_stride[2], p.B, p.H, p.T, delta, dq_acc);
+  GPTB200_CHECK_LAUNCH();
+  p.delta = delta;
+  p.dq_acc = dq_acc;
+  p.dk = reinterpret_cast<bf16*>(dk);
+  p.dv = reinterpret_cast<bf16*>(dv);
+  p.sb = dkv_stride[0];
+  p.sh = dkv_stride[1];
+  p.st = dkv_stride[2];
+  p.rcos = reinterpret_cast<const bf16*>(rope_cos);
+  p.rsin = reinterpret_cast<const bf16*>(rope_sin);
+  const bool two = p.T >= 2048;  // softmax groups, as in the plain backward
+  const int e = score_mode(a, [&](auto mode) {
+    constexpr int MODE = decltype(mode)::value;
+    if (p.seg)
+      return two ? score_bwd_launch<true, 2, MODE>(p, m, st) : score_bwd_launch<true, 1, MODE>(p, m, st);
+    return two ? score_bwd_launch<false, 2, MODE>(p, m, st) : score_bwd_launch<false, 1, MODE>(p, m, st);
+  });
+  if (e) return e;
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int64_t chunks = rows * (HD / 8);
+  const int blocks = (int)std::min<int64_t>((chunks + 255) / 256, (int64_t)sms * 8);
+  attn_dq_store_kernel<<<blocks, 256, 0, st>>>(dq_acc, reinterpret_cast<bf16*>(dq), dq_stride[0],
+                                               dq_stride[1], dq_stride[2], p.B, p.H, p.T, p.scale,
+                                               p.rcos, p.rsin);
   GPTB200_CHECK_LAUNCH();
   return 0;
 }

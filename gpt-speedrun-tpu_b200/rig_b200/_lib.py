@@ -70,6 +70,29 @@ class AdamWConfig(ctypes.Structure):
     ]
 
 
+class ScoreAttention(ctypes.Structure):
+    _fields_ = [
+        ("q", c_vp),
+        ("k", c_vp),
+        ("v", c_vp),
+        ("q_stride", c_i64 * 3),
+        ("kv_stride", c_i64 * 3),
+        ("o", c_vp),
+        ("o_stride", c_i64 * 3),
+        ("lse", c_vp),
+        ("batch", c_i64),
+        ("heads", c_i64),
+        ("kv_heads", c_i64),
+        ("seq", c_i64),
+        ("head_dim", c_i64),
+        ("softmax_scale", c_f32),
+        ("softcap", c_f32),
+        ("slopes", c_vp),
+        ("segment_ids", c_vp),
+        ("prefix_lens", c_vp),
+    ]
+
+
 class AdamW8State(ctypes.Structure):
     _fields_ = [("m", c_vp), ("m_exp", c_vp), ("v", c_vp), ("v_exp", c_vp)]
 
@@ -130,6 +153,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp,
          c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_f32, c_vp, c_vp, c_vp, c_vp, c_vp],
+    ),
+    "gptb200_score_attention_fwd": (c_int, [ctypes.POINTER(ScoreAttention), c_vp]),
+    "gptb200_score_attention_bwd": (
+        c_int,
+        [ctypes.POINTER(ScoreAttention), c_vp, ctypes.POINTER(c_i64), c_vp, c_vp, c_vp,
+         ctypes.POINTER(c_i64), ctypes.POINTER(c_i64), c_vp, c_vp, c_vp, c_vp],
     ),
     "gptb200_lce_fwd_workspace_size": (c_size, [c_i64, c_i64]),
     "gptb200_lce_fwd": (

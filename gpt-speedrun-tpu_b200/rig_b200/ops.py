@@ -400,6 +400,100 @@ def attention_bwd(q, k, v, o, do, lse, dq, dk, dv, *, scale: float, layout="bhsd
     return dq, dk, dv
 
 
+def _tma_strides(t: torch.Tensor, layout: str) -> tuple[int, int, int]:
+    """`_strides4` with the strides of length-1 dimensions, which nothing uses,
+    replaced by one that a tensor map accepts."""
+
+    sizes = t.shape[:3] if layout == "bhsd" else (t.shape[0], t.shape[2], t.shape[1])
+    return tuple(s if n > 1 else t.shape[3] for s, n in zip(_strides4(t, layout), sizes))
+
+
+def _score_call(q, k, v, o, lse, scale, layout, softcap, slopes, segment_ids, prefix_lens):
+    """Checks a score-modified attention call; returns (struct, b, h, kv heads, t)."""
+
+    _cuda(q, k, v, o, lse, slopes, segment_ids, prefix_lens)
+    if layout not in ("bhsd", "bthd"):
+        raise ValueError(f"unknown attention layout {layout!r}")
+    for name, t_ in (("q", q), ("k", k), ("v", v), ("o", o)):
+        if t_.dim() != 4 or t_.dtype != BF16:
+            raise ValueError(f"{name} must be a rank-4 bfloat16 view, got {t_.dtype} {tuple(t_.shape)}")
+    b, t, h, d = q.shape if layout == "bthd" else (q.shape[0], q.shape[2], q.shape[1], q.shape[3])
+    kv = k.shape[2 if layout == "bthd" else 1]
+    want = (b, t, kv, d) if layout == "bthd" else (b, kv, t, d)
+    if o.shape != q.shape or tuple(k.shape) != want or tuple(v.shape) != want:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} and o "
+                         f"{tuple(o.shape)} do not match")
+    if kv == 0 or h % kv:
+        raise ValueError(f"{h} query heads cannot share {kv} key/value heads")
+    kvs = _tma_strides(k, layout)
+    if _tma_strides(v, layout) != kvs:
+        raise ValueError("k and v must share strides")
+    if lse.dtype != F32 or lse.numel() != b * h * t or not lse.is_contiguous():
+        raise ValueError(f"lse must be contiguous float32 [{b}, {h}, {t}]")
+    if slopes is not None and (slopes.dtype != F32 or tuple(slopes.shape) != (h,)
+                               or not slopes.is_contiguous()):
+        raise ValueError(f"slopes must be contiguous float32 [{h}], got {slopes.dtype} "
+                         f"{tuple(slopes.shape)}")
+    if prefix_lens is not None and (prefix_lens.dtype != torch.int32
+                                    or tuple(prefix_lens.shape) != (b,)
+                                    or not prefix_lens.is_contiguous()):
+        raise ValueError(f"prefix_lens must be contiguous int32 [{b}], got {prefix_lens.dtype} "
+                         f"{tuple(prefix_lens.shape)}")
+    if segment_ids is not None and not segment_ids.is_contiguous():
+        raise ValueError("segment_ids must be contiguous")
+    _segments(segment_ids, b, t)
+    s3 = ctypes.c_int64 * 3
+    c = _lib.ScoreAttention(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), s3(*_tma_strides(q, layout)), s3(*kvs), o.data_ptr(),
+        s3(*_tma_strides(o, layout)), lse.data_ptr(), b, h, kv, t, d, float(scale), float(softcap),
+        _ptr(slopes), _ptr(segment_ids), _ptr(prefix_lens))
+    return c, b, h, kv, t
+
+
+def score_attention_fwd(q, k, v, o, lse, *, scale: float, layout: str = "bhsd",
+                        softcap: float = 0.0, slopes=None, segment_ids=None, prefix_lens=None):
+    """Causal attention over softcap * tanh(scale q.k / softcap) - slopes[h] |i - j|.
+
+    q and o have H heads, k and v H or a divisor of it (shared key/value heads);
+    rank-4 views in `layout`, used as given (apply RoPE before). softcap 0 and
+    slopes None leave their part out. segment_ids: int32 [B, T], attention stays
+    within an id and negative ids are padding; prefix_lens: int32 [B], keys below
+    it are seen by every query. A query that sees nothing gets o = 0, lse = -inf.
+    """
+
+    c, *_ = _score_call(q, k, v, o, lse, scale, layout, softcap, slopes, segment_ids, prefix_lens)
+    call("gptb200_score_attention_fwd", ctypes.byref(c), _stream())
+    return o, lse
+
+
+def score_attention_bwd(q, k, v, o, do, lse, dq, dk, dv, *, scale: float, layout: str = "bhsd",
+                        softcap: float = 0.0, slopes=None, segment_ids=None, prefix_lens=None,
+                        rope=None, workspace=None):
+    """Gradients of `score_attention_fwd` (its o and lse); dk and dv sum over the
+    query heads that share them. With `rope` dq and dk are rotated back."""
+
+    c, b, h, _, t = _score_call(q, k, v, o, lse, scale, layout, softcap, slopes, segment_ids,
+                                prefix_lens)
+    _cuda(do, dq, dk, dv, workspace)
+    for name, g, x in (("do", do, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+        if g.shape != x.shape or g.dtype != BF16:
+            raise ValueError(f"{name} must be bfloat16 {tuple(x.shape)}, got {g.dtype} {tuple(g.shape)}")
+    dkvs = _tma_strides(dk, layout)
+    if _tma_strides(dv, layout) != dkvs:
+        raise ValueError("dk and dv must share strides")
+    size = int(_lib.load().gptb200_attention_bwd_workspace_size(b, h, t))
+    if workspace is None:
+        workspace = _scratch(size, q.device)
+    elif workspace.numel() * workspace.element_size() < size:
+        raise ValueError(f"the workspace needs {size} bytes")
+    s3 = ctypes.c_int64 * 3
+    cos, sin = rope if rope is not None else (None, None)
+    call("gptb200_score_attention_bwd", ctypes.byref(c), do.data_ptr(), s3(*_tma_strides(do, layout)),
+         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), s3(*_tma_strides(dq, layout)), s3(*dkvs),
+         _ptr(cos), _ptr(sin), _ptr(workspace), _stream())
+    return dq, dk, dv
+
+
 # ----------------------------------------------------------------- cross entropy
 def lce_fwd_workspace(n: int, v: int, device) -> torch.Tensor:
     size = _lib.load().gptb200_lce_fwd_workspace_size(n, v)

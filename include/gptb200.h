@@ -241,6 +241,45 @@ int gptb200_attention_bwd(const void* q, const void* k, const void* v, int64_t s
                           const void* rope_cos, const void* rope_sin, const int32_t* segment_ids,
                           void* workspace, void* stream);
 
+/* ------------------------------------------------------------------ score-modified attention
+ * Causal attention whose scores are capped and biased before the softmax (no
+ * reference counterpart):
+ *   s'_ij = softcap * tanh(softmax_scale q_i.k_j / softcap) - slopes[h] |i - j|
+ * softcap 0: no cap; slopes NULL: no bias (finite fp32 [heads] otherwise; they
+ * are constants, no gradient). heads is a multiple of kv_heads: query head h
+ * reads key/value head h / (heads / kv_heads), whose dk and dv sum over its
+ * query heads. Query i sees key j if
+ *   (j <= i or j < prefix_lens[b]) and, with segment_ids,
+ *   segment_ids[b, i] == segment_ids[b, j] >= 0.
+ * A negative id marks padding. A query that sees nothing gets o = 0, lse =
+ * -inf and contributes no gradient. k, v, q and dout at places that the masks
+ * hide must be finite numbers (0 * NaN is NaN). prefix_lens (int32 [batch], or
+ * NULL) is clamped to [0, seq]. Strides {batch, head, time} in elements,
+ * multiples of 8, head dimension contiguous; k and v share theirs. head_dim 64,
+ * bf16; with segment ids seq <= 65536. lse: fp32 [batch, heads, seq]. */
+typedef struct gptb200_score_attention {
+  const void *q, *k, *v;
+  int64_t q_stride[3], kv_stride[3];
+  void* o;
+  int64_t o_stride[3];
+  float* lse;
+  int64_t batch, heads, kv_heads, seq, head_dim;
+  float softmax_scale, softcap;
+  const float* slopes;
+  const int32_t* segment_ids;
+  const int32_t* prefix_lens;
+} gptb200_score_attention;
+int gptb200_score_attention_fwd(const gptb200_score_attention* call, void* stream);
+/* Backward of the same call (o and lse as the forward wrote them). dq, dk, dv
+ * are written; dk and dv share dkv_stride. With rope tables dq and dk are
+ * rotated back as in gptb200_attention_bwd. workspace:
+ * gptb200_attention_bwd_workspace_size(batch, heads, seq) bytes. */
+int gptb200_score_attention_bwd(const gptb200_score_attention* call, const void* dout,
+                                const int64_t* dout_stride, void* dq, void* dk, void* dv,
+                                const int64_t* dq_stride, const int64_t* dkv_stride,
+                                const void* rope_cos, const void* rope_sin, void* workspace,
+                                void* stream);
+
 /* ------------------------------------------------------------------ routed MLP (MoE)
  * recipes/reference_moe/train.py:1230-1372 (routed_mlp_local, load_balance_loss)
  * as kernels around gptb200_gemm. Assignment a = token * top_k + choice; the
