@@ -77,6 +77,7 @@ struct AttnParams {
   float cap;           // tanh cap of the scaled scores (kCap)
   const float* slopes; // [H] distance slopes (kBias)
   const int* prefix;   // [B] keys every query sees, or null (MODE > kClassic)
+  int by_weight;       // items of all heads by falling weight (MODE > kClassic)
   // output / saved tensors
   bf16* o;
   int64_t osb, osh, ost;
@@ -215,6 +216,123 @@ GPTB200_DEV float tanh_any(float z) {
   return fmaf(-2.f, __fdividef(1.f, 1.f + ex2(2.f * kLog2e * z)), 1.f);
 }
 
+GPTB200_DEV float fmax3_abs(float a, float b, float c) {
+  float d;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// One query row's 128 scores of a key block in registers, turned into
+// s' log2(e) in place (MODE without cap and bias: left as they are).
+template <int MODE>
+struct ScoreRow {
+  static constexpr bool CAP = (MODE & kCap) != 0, BIAS = (MODE & kBias) != 0;
+  uint32_t (&v)[128];
+  float z_per_s;   // z = s * z_per_s
+  float out;       // s' log2(e) per tanh(z), or per s
+  float slope2, at0;
+  GPTB200_DEV ScoreRow(uint32_t (&v_)[128], const AttnParams& p, float slope2_, float at0_)
+      : v(v_), slope2(slope2_), at0(at0_) {
+    z_per_s = CAP ? p.scale / p.cap : 1.f;
+    out = (CAP ? p.cap : p.scale) * kLog2e;
+  }
+  // Whether any score of the warp is past the short form of tanh.
+  GPTB200_DEV bool any_large() const {
+    if constexpr (!CAP) return false;
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 128; i += 2)
+      t[(i >> 1) & 3] =
+          fmax3_abs(t[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+    return __any_sync(0xffffffffu, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * z_per_s > 1.f);
+  }
+  // Scores [I, I + N). The bias up to the query, -slope (query - key), runs in
+  // four pairs that step by eight keys, so it costs one addition for two
+  // scores and its own FMA; TWO: |key - query| each.
+  template <int I, int N, bool LARGE, bool TWO>
+  GPTB200_DEV void modify() const {
+    if constexpr (CAP || BIAS) {
+      constexpr float c[5] = GPTB200_TANH_COEFS;
+      float2 k[5];
+#pragma unroll
+      for (int u = 0; u < 5; ++u) k[u] = make_float2(out * c[u], out * c[u]);
+      const float2 zs = make_float2(z_per_s, z_per_s), o2 = make_float2(out, out);
+      float2 b[4];
+      const float2 step = make_float2(8.f * slope2, 8.f * slope2);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        b[u] = make_float2(slope2 * (at0 + (float)(I + 2 * u)), slope2 * (at0 + (float)(I + 2 * u + 1)));
+#pragma unroll
+      for (int i = I; i < I + N; i += 2) {
+        float2 y = make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+        float2& bias = b[(i >> 1) & 3];
+        if constexpr (BIAS && TWO)
+          bias = make_float2(-slope2 * fabsf(at0 + (float)i), -slope2 * fabsf(at0 + (float)(i + 1)));
+        if constexpr (CAP && !LARGE) {
+          const float2 z = fmul2(y, zs);
+          const float2 u = fmul2(z, z);
+          float2 a = ffma2(u, k[4], k[3]);
+          a = ffma2(u, a, k[2]);
+          a = ffma2(u, a, k[1]);
+          a = ffma2(u, a, k[0]);
+          y = BIAS ? ffma2(z, a, bias) : fmul2(z, a);
+        } else {
+          if constexpr (CAP) {
+            y = fmul2(y, zs);
+            y = make_float2(tanh_any(y.x), tanh_any(y.y));
+          }
+          y = BIAS ? ffma2(y, o2, bias) : fmul2(y, o2);
+        }
+        if constexpr (BIAS && !TWO) bias = fadd2(bias, step);
+        v[i] = __float_as_uint(y.x);
+        v[i + 1] = __float_as_uint(y.y);
+      }
+    }
+  }
+  template <typename LARGE>
+  GPTB200_DEV void modify_word(int w, LARGE) const {
+    constexpr bool L = LARGE::value;
+    if (w == 0) modify<0, 32, L, true>();
+    if (w == 1) modify<32, 32, L, true>();
+    if (w == 2) modify<64, 32, L, true>();
+    if (w == 3) modify<96, 32, L, true>();
+  }
+  // Scores of word w that are not in `see` become `to`.
+  GPTB200_DEV void hide(int w, uint32_t see, float to) const {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      v[32 * w + i] = (see >> i) & 1u ? v[32 * w + i] : __float_as_uint(to);
+  }
+};
+
+// Bits of the keys 0..lim of a 128-key block.
+GPTB200_DEV void causal_words(int lim, uint32_t (&see)[4]) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int n = lim - 32 * w;  // the word's last visible key
+    see[w] = n >= 31 ? 0xffffffffu : n < 0 ? 0u : (2u << n) - 1u;
+  }
+}
+// ANDs in the keys that carry the row's id: one ballot per word for every
+// distinct id among the warp's 32 rows (packed documents have one or two).
+// kid[w]: the id of key 32 w + lane.
+GPTB200_DEV void segment_words(const int (&kid)[4], int sq, uint32_t (&see)[4]) {
+  uint32_t same[4] = {0, 0, 0, 0};
+  uint32_t left = 0xffffffffu;
+  while (left) {
+    const int id = __shfl_sync(0xffffffffu, sq, __ffs(left) - 1);
+    const bool mine = sq == id;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t b = __ballot_sync(0xffffffffu, kid[w] == id);
+      if (mine) same[w] = b;
+    }
+    left &= ~__ballot_sync(0xffffffffu, mine);
+  }
+#pragma unroll
+  for (int w = 0; w < 4; ++w) see[w] &= same[w];
+}
+
 // Padding (a negative id) never equals another id: queries carry -2, keys -1.
 template <bool GENERAL>
 GPTB200_DEV int seg_query_id(int v) {
@@ -245,6 +363,13 @@ constexpr int KV_BYTES = FK * 128;      // 128 rows x 64 bf16
 constexpr int kKvStages = 4;
 constexpr int kFwdMma1Warp = 10;       // MMA thread of tile 1 (warp 1 serves tile 0)
 constexpr int kFwdThreads = 32 * 11;
+// MODE > kClassic: whole warpgroups, so that registers can move from the one
+// that loads and issues (warps 0-3, the last one idle) to the two softmax ones
+// (4-7: tile 0, 8-11: tile 1), whose modified scores would spill otherwise.
+// The shares add up to what the launch gives, 384 x 168.
+constexpr int kFwdGeneralThreads = 32 * 12;
+constexpr int kFwdRegsIssue = 56, kFwdRegsSoftmax = 224;
+static_assert(kFwdRegsIssue + 2 * kFwdRegsSoftmax == 3 * 168, "register shares");
 constexpr int kFwdItemUsers = 2 + 8;   // both MMA threads, the 8 softmax warps
 
 // Item slot written by the TMA warp: pair, batch*head, key blocks the pair
@@ -273,7 +398,7 @@ struct FwdSmem {
 };
 
 template <bool SEG, int MODE>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+__global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralThreads, 1)
     attn_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const AttnParams p) {
   using L = FwdSmem<SEG>;
@@ -303,6 +428,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   FwdItem* items = reinterpret_cast<FwdItem*>(sm + L::ITEM);
 
+  constexpr int kMma1Warp = GENERAL ? 2 : kFwdMma1Warp;
+  constexpr int kSoftmaxWarp = GENERAL ? 4 : 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int BH = p.B * p.H;
   const int npair = (p.T + 2 * FQ - 1) / (2 * FQ);
@@ -351,7 +478,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   auto tO = [&](int x) { return tmem + 256 + 64 * x; };
   auto tP = [&](int x) { return tmem + 384 + 64 * x; };
 
-  if (warp == 0) {
+  auto produce = [&]() {
     // Item producer: publishes each item's slot (with segment ids also the
     // chunk ranges and the key-block list), then loads its two Q tiles and its
     // K/V blocks into the ring.
@@ -368,7 +495,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         }
         break;
       }
-      const int bh = item / npair, pr = npair - 1 - (item - bh * npair);
+      int bh = item / npair, pr = npair - 1 - (item - bh * npair);
+      if (GENERAL && p.by_weight) {
+        pr = npair - 1 - item / BH;
+        bh = item % BH;
+      }
       const int b = bh / p.H, h = bh - b * p.H;
       const int q0 = pr * 2 * FQ;
       // tile x's diagonal key block is d0 + x; tile 1 of the last pair may lie
@@ -492,7 +623,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
-  } else if (warp == 1 || warp == kFwdMma1Warp) {
+  };
+  auto issue = [&]() {
     // One MMA thread per tile: S_x = Q_x K_j^T (128 x 128 fp32) for the next
     // block as soon as the softmax holds S_x in registers, O_x += P_x V_j
     // once P_x is in TMEM. The two tiles progress independently; each walks
@@ -566,13 +698,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         jx += nb;
       }
     }
-  } else if (warp < kFwdMma1Warp) {
+  };
+  auto softmax = [&]() {
     // Softmax warpgroup x (warps 2-5: tile 0, 6-9: tile 1); thread = query
     // row r of the tile (TMEM lane r). Per block: the S row into registers,
     // its max, then exp + row sum + P, with a running max that is only raised
     // when the row max grows by more than 2^8; O is then rescaled in TMEM.
     // Otherwise the stale max is exact because O and the row sum share it.
-    const int x = (warp - 2) >> 2;
+    const int x = (warp - kSoftmaxWarp) >> 2;
     const int quad = warp & 3;
     const int r = quad * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
@@ -606,22 +739,29 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < nb && ok; ++j) {
         const int jj = jx + j;
+        const int jb = kblock(slot, j);
+        int kid[4] = {0, 0, 0, 0};  // GENERAL: the block's key ids, lane l keys l + 32 w
+        if constexpr (SEG && GENERAL) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int key = jb * FK + 32 * w + lane;
+            kid[w] = key < p.T ? seg_key_id<true>(segrow[key]) : -1;
+          }
+        }
         if (!(ok = mbar_wait(&s_full[x], jj & 1, abort_flag, err))) break;
         tc_fence_after();
-        const int jb = kblock(slot, j);
         // keys past the query (and past T) are masked
         const bool diag = GENERAL ? jb * FK + FK - 1 > max(q0 + x * FQ, inf.prefix - 1)
                                   : (jb == d0 + x);
-        const int rl = GENERAL ? last - jb * FK : r;  // last visible key of this block
         // Per-element segment test unless keys and queries all share one id;
         // the block's key ids then come through shared memory (double-buffered,
         // one mbarrier handshake across the warpgroup).
         const bool segmask = segrow && !rng_single(seg_range(segtab, nch, 2 * jb, 2), qrng);
         const int* ks = kseg + (nseg & 1) * FK;
-        if (segmask) {
+        if (!GENERAL && segmask) {
           const int key = jb * FK + r;
           kseg[(nseg & 1) * FK + r] =
-              key < p.T ? seg_key_id<GENERAL>(segrow[key]) : (GENERAL ? -1 : INT_MAX);
+              key < p.T ? segrow[key] : INT_MAX;
           mbar_arrive(&kseg_full[2 * x + (nseg & 1)]);
           if (!(ok = mbar_wait(&kseg_full[2 * x + (nseg & 1)], (nseg >> 1) & 1, abort_flag, err)))
             break;
@@ -636,74 +776,54 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[x]);
-        auto visible = [&](int i) { return (!diag || i <= rl) && (!segmask || ks[i] == sq); };
-        // Capped and biased scores, in units of log2, in place of the raw ones.
-        if constexpr ((MODE & (kCap | kBias)) != 0) {
-          const float k = (MODE & kCap) ? p.scale / p.cap : 1.f;
-          const float a = (MODE & kCap) ? p.cap * kLog2e : c;
-          // key - query at this block's first key
-          const float at0 = (float)(jb * FK - qrow);
-          const float base = slope2 * at0;
-          const bool ahead = jb * FK + FK - 1 > q0 + x * FQ;  // some key is past some query
-          auto bias2 = [&](float2 y, int i, auto two_sided) {
-            if constexpr (!(MODE & kBias)) return y;
-            if constexpr (decltype(two_sided)::value)
-              return make_float2(fmaf(-slope2, fabsf(at0 + (float)i), y.x),
-                                 fmaf(-slope2, fabsf(at0 + (float)(i + 1)), y.y));
-            else
-              return fadd2(y, ffma2(make_float2(slope2, slope2),
-                                    make_float2((float)i, (float)(i + 1)),
-                                    make_float2(base, base)));
-          };
-          auto modify = [&](auto small, auto two_sided) {
-#pragma unroll
-            for (int i = 0; i < FK; i += 2) {
-              float2 y = make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-              if constexpr ((MODE & kCap) != 0) {
-                y = fmul2(y, make_float2(k, k));
-                if constexpr (decltype(small)::value)
-                  y = tanh_small2(y);
-                else
-                  y = make_float2(tanh_any(y.x), tanh_any(y.y));
-              }
-              y = bias2(fmul2(y, make_float2(a, a)), i, two_sided);
-              v[i] = __float_as_uint(y.x);
-              v[i + 1] = __float_as_uint(y.y);
-            }
-          };
-          bool large = false;
-          if constexpr ((MODE & kCap) != 0) {
-            if (diag || segmask) {  // hidden scores do not choose the form of tanh
-#pragma unroll
-              for (int i = 0; i < FK; ++i)
-                if (!visible(i)) v[i] = 0;
-            }
-            float t8[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) t8[u] = 0.f;
-#pragma unroll
-            for (int i = 0; i < FK; i += 2)
-              t8[(i >> 1) & 7] = fmax3(t8[(i >> 1) & 7], fabsf(__uint_as_float(v[i])),
-                                       fabsf(__uint_as_float(v[i + 1])));
-            const float top = fmaxf(fmax3(t8[0], t8[1], t8[2]),
-                                    fmax3(t8[3], t8[4], fmaxf(t8[5], fmaxf(t8[6], t8[7]))));
-            large = __any_sync(0xffffffffu, top * k > 1.f);
-          }
-          const std::true_type yes;
-          const std::false_type no;
-          if (large)
-            modify(no, yes);
-          else if ((MODE & kBias) && ahead)
-            modify(yes, yes);
-          else
-            modify(yes, no);
-        }
-        // Row max of the raw scores (c > 0 commutes with the max), eight
-        // independent chains; on the diagonal block keys past the query are out.
+        // Row max (of the raw scores where they are used as they are: c > 0
+        // commutes with the max), eight independent chains; on the diagonal
+        // block keys past the query are out.
         float m8[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) m8[u] = -INFINITY;
-        if (diag || segmask) {
+        bool none[4] = {false, false, false, false};  // GENERAL: 32 columns hidden from the whole warp
+        auto visible = [&](int i) { return (!diag || i <= r) && (!segmask || ks[i] == sq); };
+        if constexpr (GENERAL) {
+          // Modified scores in units of log2 in place of the raw ones.
+          ScoreRow<MODE> row(v, p, slope2, (float)(jb * FK - qrow));
+          bool masked = diag || segmask;
+          bool large = false;
+          if ((MODE & kBias) && jb * FK + FK - 1 > q0 + x * FQ) masked = true;  // keys past a query
+          if (!masked) {
+            large = row.any_large();
+            if (!large) row.template modify<0, FK, false, false>();
+          }
+          if (masked || large) {
+            // which of the 128 keys this row sees, as four words
+            uint32_t see[4];
+            causal_words(last - jb * FK, see);
+            if (segmask) segment_words(kid, sq, see);
+            bool full[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              full[w] = __all_sync(0xffffffffu, see[w] == 0xffffffffu);
+              none[w] = __all_sync(0xffffffffu, see[w] == 0u);
+              if (!full[w]) row.hide(w, see[w], 0.f);  // hidden scores do not choose tanh's form
+            }
+            if (masked) large = row.any_large();
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              if (none[w]) continue;
+              if (large)
+                row.modify_word(w, std::true_type());
+              else
+                row.modify_word(w, std::false_type());
+            }
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              if (!full[w]) row.hide(w, see[w], -INFINITY);
+          }
+#pragma unroll
+          for (int i = 0; i < FK; i += 2)
+            m8[(i >> 1) & 7] =
+                fmax3(m8[(i >> 1) & 7], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+        } else if (diag || segmask) {
 #pragma unroll
           for (int i = 0; i < FK; i += 2)
             m8[(i >> 1) & 7] = fmax3(m8[(i >> 1) & 7], visible(i) ? __uint_as_float(v[i]) : -INFINITY,
@@ -714,9 +834,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             m8[(i >> 1) & 7] =
                 fmax3(m8[(i >> 1) & 7], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
         }
-        const float unit = (MODE & (kCap | kBias)) ? 1.f : c;  // of v in log2
+        constexpr bool kLog2 = (MODE & (kCap | kBias)) != 0;  // v is in log2 already
         const float mx =
-            fmaxf(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], fmaxf(m8[5], fmaxf(m8[6], m8[7])))) * unit;
+            fmaxf(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], fmaxf(m8[5], fmaxf(m8[6], m8[7])))) *
+            (kLog2 ? 1.f : c);
         // The rescale decision is made per warp: the TMEM loads/stores of O are
         // warp-collective and must not run in a divergent branch. Rows whose
         // max did not move rescale by exactly 1.
@@ -730,28 +851,40 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           m_used = m_new;
         }
         // P = exp2(s*c - m) packed to bf16 pairs in registers (the S registers
-        // die as P is produced); four packed partial row sums.
-        const float2 c2 = make_float2(c, c), nm2 = make_float2(-m_used, -m_used);
-        const auto shifted = [&](float2 y) {
-          if constexpr ((MODE & (kCap | kBias)) != 0)
-            return fadd2(y, nm2);
-          else
-            return ffma2(y, c2, nm2);
-        };
+        // die as P is produced); four packed partial row sums. GENERAL: hidden
+        // scores are -inf and need no test, if the row has a finite m at all.
+        const float m_sub = GENERAL && m_used == -INFINITY ? 0.f : m_used;
+        const float2 c2 = make_float2(c, c), nm2 = make_float2(-m_sub, -m_sub);
         float2 acc[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) acc[u] = make_float2(0.f, 0.f);
         uint32_t pk[FK / 2];
+        auto exponentials = [&](int i0, int n) {
 #pragma unroll
-        for (int i = 0; i < FK; i += 2) {
-          const float2 t = shifted(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
-          float p0 = ex2(t.x), p1 = ex2(t.y);
-          if (diag || segmask) {
-            if (!visible(i)) p0 = 0.f;
-            if (!visible(i + 1)) p1 = 0.f;
+          for (int i = i0; i < i0 + n; i += 2) {
+            float2 t = make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+            t = kLog2 ? fadd2(t, nm2) : ffma2(t, c2, nm2);
+            float p0 = ex2(t.x), p1 = ex2(t.y);
+            if (!GENERAL && (diag || segmask)) {
+              if (!visible(i)) p0 = 0.f;
+              if (!visible(i + 1)) p1 = 0.f;
+            }
+            acc[(i >> 1) & 3] = fadd2(acc[(i >> 1) & 3], make_float2(p0, p1));
+            pk[i / 2] = pack_bf16x2(p0, p1);
           }
-          acc[(i >> 1) & 3] = fadd2(acc[(i >> 1) & 3], make_float2(p0, p1));
-          pk[i / 2] = pack_bf16x2(p0, p1);
+        };
+        if constexpr (GENERAL) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if (!none[w]) {
+              exponentials(32 * w, 32);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pk[16 * w + i] = 0;
+            }
+          }
+        } else {
+          exponentials(0, FK);
         }
         const float2 s01 = fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3]));
         const float sum = s01.x + s01.y;
@@ -811,6 +944,25 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       if (lane == 0) mbar_arrive(&item_empty[slot]);
       jx += nb;
     }
+  };
+  if constexpr (GENERAL) {
+    if (warp < kSoftmaxWarp) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFwdRegsIssue));
+      if (warp == 0) {
+        produce();
+      } else if (warp <= kMma1Warp) {
+        issue();
+      }
+    } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFwdRegsSoftmax));
+      softmax();
+    }
+  } else if (warp == 0) {
+    produce();
+  } else if (warp == 1 || warp == kMma1Warp) {
+    issue();
+  } else {
+    softmax();
   }
   tc_fence_before();
   __syncthreads();
@@ -986,7 +1138,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         break;
       }
       const int nkt = (p.T + BT - 1) / BT;
-      const int bh = item / nkt, kt = item - bh * nkt;
+      int bh = item / nkt, kt = item - bh * nkt;
+      if (GENERAL && p.by_weight) {
+        kt = item / BH;
+        bh = item % BH;
+      }
       const int b = bh / heads, h = bh - b * heads;
       const int k0 = kt * BT;
       int qb = k0, pf = 0;
@@ -1905,6 +2061,7 @@ static AttnParams score_params(const gptb200_score_attention* a) {
   p.cap = a->softcap;
   p.slopes = a->slopes;
   p.prefix = a->prefix_lens;
+  p.by_weight = getenv("BYW") ? atoi(getenv("BYW")) : 1;
   p.o = reinterpret_cast<bf16*>(a->o);
   p.osb = a->o_stride[0];
   p.osh = a->o_stride[1];
@@ -1940,8 +2097,8 @@ template <bool SEG, int MODE>
 static int score_fwd_launch(const AttnParams& p, const ScoreMaps& m, cudaStream_t st) {
   static bool done[64] = {};
   const int64_t items = (int64_t)((p.T + 2 * FQ - 1) / (2 * FQ)) * p.B * p.H;
-  return launch_persistent(attn_fwd_tc<SEG, MODE>, done, items, kFwdThreads, FwdSmem<SEG>::TOTAL,
-                           st, m.q, m.k, m.v, p);
+  return launch_persistent(attn_fwd_tc<SEG, MODE>, done, items, kFwdGeneralThreads,
+                           FwdSmem<SEG>::TOTAL, st, m.q, m.k, m.v, p);
 }
 
 template <bool SEG, int GROUPS, int MODE>
