@@ -222,90 +222,165 @@ GPTB200_DEV float fmax3_abs(float a, float b, float c) {
   return d;
 }
 
-// One query row's 128 scores of a key block in registers, turned into
-// s' log2(e) in place (MODE without cap and bias: left as they are).
+// A query row's raw scores, 32 columns (keys) at a time, and their way to the
+// probabilities exp2(s' log2(e) - m), packed as bf16 pairs. The callers loop over
+// the chunks of a block without unrolling: two warps of a scheduler at different
+// places of a block-long sequence of instructions fetch more than they compute.
 template <int MODE>
-struct ScoreRow {
+struct Score {
   static constexpr bool CAP = (MODE & kCap) != 0, BIAS = (MODE & kBias) != 0;
-  uint32_t (&v)[128];
-  float z_per_s;   // z = s * z_per_s
-  float out;       // s' log2(e) per tanh(z), or per s
-  float slope2, at0;
-  GPTB200_DEV ScoreRow(uint32_t (&v_)[128], const AttnParams& p, float slope2_, float at0_)
-      : v(v_), slope2(slope2_), at0(at0_) {
+  // A row keeps its maximum m until a score passes it by this many powers of
+  // two: bf16, the fp32 sums and O lose nothing below that, and exp2 is far
+  // from overflow.
+  static constexpr float kSlack = 40.f;
+  float z_per_s;  // tanh's argument per raw score
+  float out;      // s' log2(e) per tanh, or per raw score
+  float slope2;   // slope * log2(e)
+  GPTB200_DEV Score(const AttnParams& p, float slope2_) : slope2(slope2_) {
     z_per_s = CAP ? p.scale / p.cap : 1.f;
     out = (CAP ? p.cap : p.scale) * kLog2e;
   }
-  // Whether any score of the warp is past the short form of tanh.
-  GPTB200_DEV bool any_large() const {
-    if constexpr (!CAP) return false;
-    float t[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 128; i += 2)
-      t[(i >> 1) & 3] =
-          fmax3_abs(t[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-    return __any_sync(0xffffffffu, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * z_per_s > 1.f);
+  static GPTB200_DEV float2 both(float x) { return make_float2(x, x); }
+  static GPTB200_DEV float2 pair(const uint32_t (&v)[32], int i) {
+    return make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
   }
-  // Scores [I, I + N). The bias up to the query, -slope (query - key), runs in
-  // four pairs that step by eight keys, so it costs one addition for two
-  // scores and its own FMA; TWO: |key - query| each.
-  template <int I, int N, bool LARGE, bool TWO>
-  GPTB200_DEV void modify() const {
-    if constexpr (CAP || BIAS) {
-      constexpr float c[5] = GPTB200_TANH_COEFS;
-      float2 k[5];
+  // The polynomial's coefficients times `out`.
+  GPTB200_DEV void coefs(float2 (&k)[5]) const {
+    constexpr float c[5] = GPTB200_TANH_COEFS;
 #pragma unroll
-      for (int u = 0; u < 5; ++u) k[u] = make_float2(out * c[u], out * c[u]);
-      const float2 zs = make_float2(z_per_s, z_per_s), o2 = make_float2(out, out);
-      float2 b[4];
-      const float2 step = make_float2(8.f * slope2, 8.f * slope2);
+    for (int u = 0; u < 5; ++u) k[u] = both(out * c[u]);
+  }
+  // Four pairs at a time, so that their dependent steps interleave.
+  static GPTB200_DEV void poly4(const float2 (&k)[5], const float2 (&u)[4], float2 (&a)[4]) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        b[u] = make_float2(slope2 * (at0 + (float)(I + 2 * u)), slope2 * (at0 + (float)(I + 2 * u + 1)));
+    for (int q = 0; q < 4; ++q) a[q] = ffma2(u[q], k[4], k[3]);
 #pragma unroll
-      for (int i = I; i < I + N; i += 2) {
-        float2 y = make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-        float2& bias = b[(i >> 1) & 3];
-        if constexpr (BIAS && TWO)
-          bias = make_float2(-slope2 * fabsf(at0 + (float)i), -slope2 * fabsf(at0 + (float)(i + 1)));
-        if constexpr (CAP && !LARGE) {
-          const float2 z = fmul2(y, zs);
-          const float2 u = fmul2(z, z);
-          float2 a = ffma2(u, k[4], k[3]);
-          a = ffma2(u, a, k[2]);
-          a = ffma2(u, a, k[1]);
-          a = ffma2(u, a, k[0]);
-          y = BIAS ? ffma2(z, a, bias) : fmul2(z, a);
-        } else {
-          if constexpr (CAP) {
-            y = fmul2(y, zs);
-            y = make_float2(tanh_any(y.x), tanh_any(y.y));
-          }
-          y = BIAS ? ffma2(y, o2, bias) : fmul2(y, o2);
+    for (int e = 2; e >= 0; --e) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) a[q] = ffma2(u[q], a[q], k[e]);
+    }
+  }
+
+  // Without masks, keys before the query, against the maximum m: arithmetic (FMA
+  // pipe) and exponentials (MUFU) of different columns overlap, with nothing to
+  // wait for in between. top and far collect the largest exponent and tanh
+  // argument squared; the caller discards the block if they do not do. `at`:
+  // first key - query. The bias, slope (key - query), with -m folded in, runs
+  // in four pairs that step by eight keys: one addition for two scores.
+  GPTB200_DEV void stream(const uint32_t (&v)[32], float at, float m, uint32_t (&pk)[16],
+                          float2 (&acc)[2], float& top, float& far) const {
+    float2 k[5];
+    if constexpr (CAP) coefs(k);
+    float2 off[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      off[q] = BIAS ? make_float2(fmaf(slope2, at + (float)(2 * q), -m),
+                                  fmaf(slope2, at + (float)(2 * q + 1), -m))
+                    : both(-m);
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+      float2 y[4];
+      if constexpr (CAP) {
+        float2 z[4], u[4], a[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) z[q] = fmul2(pair(v, i + 2 * q), both(z_per_s));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) u[q] = fmul2(z[q], z[q]);
+        poly4(k, u, a);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          far = fmax3(far, u[q].x, u[q].y);
+          y[q] = ffma2(z[q], a[q], off[q]);
         }
-        if constexpr (BIAS && !TWO) bias = fadd2(bias, step);
-        v[i] = __float_as_uint(y.x);
-        v[i + 1] = __float_as_uint(y.y);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) y[q] = ffma2(pair(v, i + 2 * q), both(out), off[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (BIAS) off[q] = fadd2(off[q], both(8.f * slope2));
+        top = fmax3(top, y[q].x, y[q].y);
+        y[q] = make_float2(ex2(y[q].x), ex2(y[q].y));
+        acc[q & 1] = fadd2(acc[q & 1], y[q]);
+        pk[i / 2 + q] = pack_bf16x2(y[q].x, y[q].y);
       }
     }
   }
-  template <typename LARGE>
-  GPTB200_DEV void modify_word(int w, LARGE) const {
-    constexpr bool L = LARGE::value;
-    if (w == 0) modify<0, 32, L, true>();
-    if (w == 1) modify<32, 32, L, true>();
-    if (w == 2) modify<64, 32, L, true>();
-    if (w == 3) modify<96, 32, L, true>();
+  // Whether a block that went through stream() has to be done in steps.
+  static GPTB200_DEV bool discard(float top, float far) {
+    // (m = -inf lifts everything to +inf)
+    return __any_sync(0xffffffffu, !(top <= kSlack) || (CAP && far > 1.f));
   }
-  // Scores of word w that are not in `see` become `to`.
-  GPTB200_DEV void hide(int w, uint32_t see, float to) const {
+
+  // Modified scores in place of the raw ones, in log2, and their maximum; those
+  // not in `see` become -inf (and do not choose tanh's form).
+  GPTB200_DEV float modify(uint32_t (&v)[32], float at, uint32_t see, bool full) const {
+    bool large = false;
+    if constexpr (CAP) {
+      float far = 0.f;
+      if (!full) hide(v, see, 0.f);
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      v[32 * w + i] = (see >> i) & 1u ? v[32 * w + i] : __float_as_uint(to);
+      for (int i = 0; i < 32; i += 2) far = fmax3_abs(far, pair(v, i).x, pair(v, i).y);
+      large = __any_sync(0xffffffffu, far * z_per_s > 1.f);
+    }
+    if (large) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        v[i] = __float_as_uint(
+            biased(out * tanh_any(__uint_as_float(v[i]) * z_per_s), at + (float)i));
+    } else {
+      float2 k[5];
+      if constexpr (CAP) coefs(k);
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) {
+        float2 y[4];
+        if constexpr (CAP) {
+          float2 z[4], u[4], a[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) z[q] = fmul2(pair(v, i + 2 * q), both(z_per_s));
+#pragma unroll
+          for (int q = 0; q < 4; ++q) u[q] = fmul2(z[q], z[q]);
+          poly4(k, u, a);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) y[q] = fmul2(z[q], a[q]);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) y[q] = fmul2(pair(v, i + 2 * q), both(out));
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          v[i + 2 * q] = __float_as_uint(biased(y[q].x, at + (float)(i + 2 * q)));
+          v[i + 2 * q + 1] = __float_as_uint(biased(y[q].y, at + (float)(i + 2 * q + 1)));
+        }
+      }
+    }
+    if (!full) hide(v, see, -INFINITY);
+    float t[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) t[(i >> 1) & 1] = fmax3(t[(i >> 1) & 1], pair(v, i).x, pair(v, i).y);
+    return fmaxf(t[0], t[1]);
+  }
+  GPTB200_DEV float biased(float y, float distance) const {
+    return BIAS ? fmaf(-slope2, fabsf(distance), y) : y;
+  }
+  static GPTB200_DEV void hide(uint32_t (&v)[32], uint32_t see, float to) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = (see >> i) & 1u ? v[i] : __float_as_uint(to);
+  }
+  // Probabilities of modified scores.
+  static GPTB200_DEV void exponentials(const uint32_t (&v)[32], float m, uint32_t (&pk)[16],
+                                       float2 (&acc)[2]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float2 y = fadd2(pair(v, i), both(-m));
+      y = make_float2(ex2(y.x), ex2(y.y));
+      acc[(i >> 1) & 1] = fadd2(acc[(i >> 1) & 1], y);
+      pk[i / 2] = pack_bf16x2(y.x, y.y);
+    }
   }
 };
 
-// Bits of the keys 0..lim of a 128-key block.
+// Bits of the keys 0..lim of a key block.
 GPTB200_DEV void causal_words(int lim, uint32_t (&see)[4]) {
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -334,19 +409,12 @@ GPTB200_DEV void segment_words(const int (&kid)[4], int sq, uint32_t (&see)[4]) 
 }
 
 // Padding (a negative id) never equals another id: queries carry -2, keys -1.
-template <bool GENERAL>
-GPTB200_DEV int seg_query_id(int v) {
-  return GENERAL && v < 0 ? -2 : v;
-}
-template <bool GENERAL>
-GPTB200_DEV int seg_key_id(int v) {
-  return GENERAL && v < 0 ? -1 : v;
-}
+GPTB200_DEV int seg_query_id(int v) { return v < 0 ? -2 : v; }
+GPTB200_DEV int seg_key_id(int v) { return v < 0 ? -1 : v; }
 // Range of a chunk's ids: a chunk of padding alone meets nothing, and a chunk
 // with some padding keeps -1 in its range, so that it is never a single id.
-template <bool GENERAL>
 GPTB200_DEV int2 seg_chunk(int mn, int mx) {
-  if (GENERAL && mn < 0) return mx < 0 ? make_int2(INT_MAX, INT_MIN) : make_int2(-1, mx);
+  if (mn < 0) return mx < 0 ? make_int2(INT_MAX, INT_MIN) : make_int2(-1, mx);
   return make_int2(mn, mx);
 }
 
@@ -365,11 +433,11 @@ constexpr int kFwdMma1Warp = 10;       // MMA thread of tile 1 (warp 1 serves ti
 constexpr int kFwdThreads = 32 * 11;
 // MODE > kClassic: whole warpgroups, so that registers can move from the one
 // that loads and issues (warps 0-3, the last one idle) to the two softmax ones
-// (4-7: tile 0, 8-11: tile 1), whose modified scores would spill otherwise.
-// The shares add up to what the launch gives, 384 x 168.
+// (4-7: tile 0, 8-11: tile 1), which keep a block's raw scores beside its
+// probabilities. The shares add up to what the launch gives.
 constexpr int kFwdGeneralThreads = 32 * 12;
-constexpr int kFwdRegsIssue = 56, kFwdRegsSoftmax = 224;
-static_assert(kFwdRegsIssue + 2 * kFwdRegsSoftmax == 3 * 168, "register shares");
+constexpr int kFwdRegs = 168, kFwdRegsIssue = 56, kFwdRegsSoftmax = 224;
+static_assert(kFwdRegsIssue + 2 * kFwdRegsSoftmax == 3 * kFwdRegs, "register shares");
 constexpr int kFwdItemUsers = 2 + 8;   // both MMA threads, the 8 softmax warps
 
 // Item slot written by the TMA warp: pair, batch*head, key blocks the pair
@@ -438,8 +506,11 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
   auto segtab_of = [&](int slot) {
     return reinterpret_cast<int2*>(sm + L::SEGTAB) + slot * kMaxSegChunks;
   };
-  // key block of list entry j of the item in `slot`
-  auto kblock = [&](int slot, int j) -> int {
+  // Key block of list entry j of the item in `slot` (nkv entries). MODE >
+  // kClassic walks the list from its end: the diagonal comes first and sets the
+  // rows' maxima, which a bias that falls with the distance then never raises.
+  auto kblock = [&](int slot, int j, int nkv) -> int {
+    if constexpr (GENERAL) j = nkv - 1 - j;
     if constexpr (SEG)
       return reinterpret_cast<const int*>(sm + L::BLOCKS)[slot * (kMaxSegChunks / 2) + j];
     else
@@ -537,7 +608,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
           }
           mn = __reduce_min_sync(0xffffffffu, mn);
           mx = __reduce_max_sync(0xffffffffu, mx);
-          if (lane == 0) tab[c] = seg_chunk<true>(mn, mx);
+          if (lane == 0) tab[c] = seg_chunk(mn, mx);
         }
         __syncwarp();
         if (lane == 0) {
@@ -616,7 +687,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
           const int s = gk % kKvStages;
           if (!(ok = mbar_wait(&kv_empty[s], ((gk / kKvStages) & 1) ^ 1, abort_flag, err))) break;
           mbar_arrive_expect_tx(&kv_full[s], 2 * KV_BYTES);
-          const int key0 = kblock(slot, j) * FK;
+          const int key0 = kblock(slot, j, nkv) * FK;
           tma_load_4d(sm + L::K + s * KV_BYTES, &tmK, &kv_full[s], 0, key0, hk, b);
           tma_load_4d(sm + L::V + s * KV_BYTES, &tmV, &kv_full[s], 0, key0, hk, b);
         }
@@ -641,6 +712,8 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
         const FwdItem inf = items[slot];
         if (inf.nkv < 0) break;  // no more items
         const int nb = x == 0 ? inf.n0 : (inf.has1 ? inf.nkv : 0);
+        // the tile's blocks are list entries [j0, j0 + nb)
+        const int j0 = GENERAL && x == 0 ? inf.nkv - nb : 0;
         const uint32_t sQ = smem_u32(sm + L::Q + (slot * 2 + x) * Q_BYTES);
         auto issue_s = [&](int s) {
           const uint32_t sK = smem_u32(sm + L::K + s * KV_BYTES);
@@ -650,25 +723,34 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
                       umma_smem_desc(sK + k * 32, 16, 1024), idS, k > 0);
           umma_commit(&s_full[x]);
         };
+        // a block this tile skips: release it once it has arrived
+        auto skip = [&](int j) {
+          const int s = (gk + j) % kKvStages;
+          if (!mbar_wait(&kv_full[s], ((gk + j) / kKvStages) & 1, abort_flag, err)) return false;
+          mbar_arrive(&kv_empty[s]);
+          return true;
+        };
+        for (int j = 0; ok && j < j0; ++j) ok = skip(j);
+        if (!ok) break;
         if (nb > 0) {
           // S of the item's first block: Q loaded, the block loaded, and the
           // previous item's last S taken out of TMEM by the softmax
+          const int s0 = (gk + j0) % kKvStages;
           ok = mbar_wait(&q_full[slot], (ii >> 1) & 1, abort_flag, err) &&
-               mbar_wait(&kv_full[gk % kKvStages], (gk / kKvStages) & 1, abort_flag, err) &&
+               mbar_wait(&kv_full[s0], ((gk + j0) / kKvStages) & 1, abort_flag, err) &&
                (jx == 0 || mbar_wait(&s_free[x], (jx - 1) & 1, abort_flag, err));
           if (!ok) break;
           tc_fence_after();
-          issue_s(gk % kKvStages);
+          issue_s(s0);
         }
-        for (int j = 0; ok && j < inf.nkv; ++j) {
+        for (int j = j0; ok && j < inf.nkv; ++j) {
           const int s = (gk + j) % kKvStages;
-          if (j >= nb) {  // a block this tile skips: release it once it has arrived
-            if (!(ok = mbar_wait(&kv_full[s], ((gk + j) / kKvStages) & 1, abort_flag, err))) break;
-            mbar_arrive(&kv_empty[s]);
+          if (j >= j0 + nb) {
+            ok = skip(j);
             continue;
           }
-          const int jj = jx + j;  // running block index of this tile
-          if (j + 1 < nb) {
+          const int jj = jx + j - j0;  // running block index of this tile
+          if (j + 1 < j0 + nb) {
             const int s1 = (gk + j + 1) % kKvStages;
             if (!(ok = mbar_wait(&kv_full[s1], ((gk + j + 1) / kKvStages) & 1, abort_flag, err)) ||
                 !(ok = mbar_wait(&s_free[x], jj & 1, abort_flag, err)))
@@ -683,7 +765,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
 #pragma unroll
           for (int k = 0; k < FK / 16; ++k)
             umma_bf16_ts(tO(x), tP(x) + k * 8, umma_smem_desc(sV + k * 2048, KV_BYTES, 1024), idO,
-                         (j > 0 || k > 0));
+                         (j > j0 || k > 0));
           umma_commit(&pv_done[x]);
           umma_commit(&kv_empty[s]);
         }
@@ -699,13 +781,13 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
       }
     }
   };
-  auto softmax = [&]() {
+  [[maybe_unused]] auto softmax = [&]() {
     // Softmax warpgroup x (warps 2-5: tile 0, 6-9: tile 1); thread = query
     // row r of the tile (TMEM lane r). Per block: the S row into registers,
     // its max, then exp + row sum + P, with a running max that is only raised
     // when the row max grows by more than 2^8; O is then rescaled in TMEM.
     // Otherwise the stale max is exact because O and the row sum share it.
-    const int x = (warp - kSoftmaxWarp) >> 2;
+    const int x = (warp - 2) >> 2;
     const int quad = warp & 3;
     const int r = quad * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
@@ -726,42 +808,25 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
       const int qrow = q0 + x * FQ + r;
       const int* segrow = SEG ? p.seg + (int64_t)b * p.T : nullptr;
       const int2* segtab = SEG ? segtab_of(slot) : nullptr;
-      const int nch = GENERAL ? inf.nch
-                              : min((p.T + kSegChunk - 1) / kSegChunk, 2 * (d0 + inf.has1 + 1));
+      const int nch = min((p.T + kSegChunk - 1) / kSegChunk, 2 * (d0 + inf.has1 + 1));
       // this row's segment id (rows past T take an id no key has)
-      const int sq = segrow ? (qrow < p.T ? seg_query_id<GENERAL>(segrow[qrow])
-                                          : (GENERAL ? -2 : INT_MIN))
-                            : 0;
-      // the last key this row sees under the causal and the prefix mask
-      const int last = GENERAL ? max(qrow, inf.prefix - 1) : qrow;
-      const float slope2 = (MODE & kBias) ? p.slopes[h] * kLog2e : 0.f;
+      const int sq = segrow ? (qrow < p.T ? segrow[qrow] : INT_MIN) : 0;
       const int2 qrng = segrow ? seg_range(segtab, nch, 2 * (d0 + x), 2) : make_int2(0, 0);
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < nb && ok; ++j) {
         const int jj = jx + j;
-        const int jb = kblock(slot, j);
-        int kid[4] = {0, 0, 0, 0};  // GENERAL: the block's key ids, lane l keys l + 32 w
-        if constexpr (SEG && GENERAL) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int key = jb * FK + 32 * w + lane;
-            kid[w] = key < p.T ? seg_key_id<true>(segrow[key]) : -1;
-          }
-        }
         if (!(ok = mbar_wait(&s_full[x], jj & 1, abort_flag, err))) break;
         tc_fence_after();
-        // keys past the query (and past T) are masked
-        const bool diag = GENERAL ? jb * FK + FK - 1 > max(q0 + x * FQ, inf.prefix - 1)
-                                  : (jb == d0 + x);
+        const int jb = kblock(slot, j, inf.nkv);
+        const bool diag = (jb == d0 + x);  // keys past the query (and past T) are masked
         // Per-element segment test unless keys and queries all share one id;
         // the block's key ids then come through shared memory (double-buffered,
         // one mbarrier handshake across the warpgroup).
         const bool segmask = segrow && !rng_single(seg_range(segtab, nch, 2 * jb, 2), qrng);
         const int* ks = kseg + (nseg & 1) * FK;
-        if (!GENERAL && segmask) {
+        if (segmask) {
           const int key = jb * FK + r;
-          kseg[(nseg & 1) * FK + r] =
-              key < p.T ? segrow[key] : INT_MAX;
+          kseg[(nseg & 1) * FK + r] = key < p.T ? segrow[key] : INT_MAX;
           mbar_arrive(&kseg_full[2 * x + (nseg & 1)]);
           if (!(ok = mbar_wait(&kseg_full[2 * x + (nseg & 1)], (nseg >> 1) & 1, abort_flag, err)))
             break;
@@ -776,54 +841,13 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[x]);
-        // Row max (of the raw scores where they are used as they are: c > 0
-        // commutes with the max), eight independent chains; on the diagonal
-        // block keys past the query are out.
+        // Row max of the raw scores (c > 0 commutes with the max), eight
+        // independent chains; on the diagonal block keys past the query are out.
         float m8[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) m8[u] = -INFINITY;
-        bool none[4] = {false, false, false, false};  // GENERAL: 32 columns hidden from the whole warp
         auto visible = [&](int i) { return (!diag || i <= r) && (!segmask || ks[i] == sq); };
-        if constexpr (GENERAL) {
-          // Modified scores in units of log2 in place of the raw ones.
-          ScoreRow<MODE> row(v, p, slope2, (float)(jb * FK - qrow));
-          bool masked = diag || segmask;
-          bool large = false;
-          if ((MODE & kBias) && jb * FK + FK - 1 > q0 + x * FQ) masked = true;  // keys past a query
-          if (!masked) {
-            large = row.any_large();
-            if (!large) row.template modify<0, FK, false, false>();
-          }
-          if (masked || large) {
-            // which of the 128 keys this row sees, as four words
-            uint32_t see[4];
-            causal_words(last - jb * FK, see);
-            if (segmask) segment_words(kid, sq, see);
-            bool full[4];
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              full[w] = __all_sync(0xffffffffu, see[w] == 0xffffffffu);
-              none[w] = __all_sync(0xffffffffu, see[w] == 0u);
-              if (!full[w]) row.hide(w, see[w], 0.f);  // hidden scores do not choose tanh's form
-            }
-            if (masked) large = row.any_large();
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              if (none[w]) continue;
-              if (large)
-                row.modify_word(w, std::true_type());
-              else
-                row.modify_word(w, std::false_type());
-            }
-#pragma unroll
-            for (int w = 0; w < 4; ++w)
-              if (!full[w]) row.hide(w, see[w], -INFINITY);
-          }
-#pragma unroll
-          for (int i = 0; i < FK; i += 2)
-            m8[(i >> 1) & 7] =
-                fmax3(m8[(i >> 1) & 7], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-        } else if (diag || segmask) {
+        if (diag || segmask) {
 #pragma unroll
           for (int i = 0; i < FK; i += 2)
             m8[(i >> 1) & 7] = fmax3(m8[(i >> 1) & 7], visible(i) ? __uint_as_float(v[i]) : -INFINITY,
@@ -834,10 +858,8 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
             m8[(i >> 1) & 7] =
                 fmax3(m8[(i >> 1) & 7], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
         }
-        constexpr bool kLog2 = (MODE & (kCap | kBias)) != 0;  // v is in log2 already
         const float mx =
-            fmaxf(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], fmaxf(m8[5], fmaxf(m8[6], m8[7])))) *
-            (kLog2 ? 1.f : c);
+            fmaxf(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], fmaxf(m8[5], fmaxf(m8[6], m8[7])))) * c;
         // The rescale decision is made per warp: the TMEM loads/stores of O are
         // warp-collective and must not run in a divergent branch. Rows whose
         // max did not move rescale by exactly 1.
@@ -851,40 +873,22 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
           m_used = m_new;
         }
         // P = exp2(s*c - m) packed to bf16 pairs in registers (the S registers
-        // die as P is produced); four packed partial row sums. GENERAL: hidden
-        // scores are -inf and need no test, if the row has a finite m at all.
-        const float m_sub = GENERAL && m_used == -INFINITY ? 0.f : m_used;
-        const float2 c2 = make_float2(c, c), nm2 = make_float2(-m_sub, -m_sub);
+        // die as P is produced); four packed partial row sums.
+        const float2 c2 = make_float2(c, c), nm2 = make_float2(-m_used, -m_used);
         float2 acc[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) acc[u] = make_float2(0.f, 0.f);
         uint32_t pk[FK / 2];
-        auto exponentials = [&](int i0, int n) {
 #pragma unroll
-          for (int i = i0; i < i0 + n; i += 2) {
-            float2 t = make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-            t = kLog2 ? fadd2(t, nm2) : ffma2(t, c2, nm2);
-            float p0 = ex2(t.x), p1 = ex2(t.y);
-            if (!GENERAL && (diag || segmask)) {
-              if (!visible(i)) p0 = 0.f;
-              if (!visible(i + 1)) p1 = 0.f;
-            }
-            acc[(i >> 1) & 3] = fadd2(acc[(i >> 1) & 3], make_float2(p0, p1));
-            pk[i / 2] = pack_bf16x2(p0, p1);
+        for (int i = 0; i < FK; i += 2) {
+          const float2 t = ffma2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), c2, nm2);
+          float p0 = ex2(t.x), p1 = ex2(t.y);
+          if (diag || segmask) {
+            if (!visible(i)) p0 = 0.f;
+            if (!visible(i + 1)) p1 = 0.f;
           }
-        };
-        if constexpr (GENERAL) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            if (!none[w]) {
-              exponentials(32 * w, 32);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) pk[16 * w + i] = 0;
-            }
-          }
-        } else {
-          exponentials(0, FK);
+          acc[(i >> 1) & 3] = fadd2(acc[(i >> 1) & 3], make_float2(p0, p1));
+          pk[i / 2] = pack_bf16x2(p0, p1);
         }
         const float2 s01 = fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3]));
         const float sum = s01.x + s01.y;
@@ -915,8 +919,176 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
       if (ok && nb > 0) {
         if (!(ok = mbar_wait(&pv_done[x], (jx + nb - 1) & 1, abort_flag, err))) break;
         tc_fence_after();
-        // a row that sees no key: zeros, lse -inf
-        const float inv = GENERAL && l == 0.f ? 0.f : 1.f / l;
+        const float inv = 1.f / l;
+        float o[32];
+        bf16* orow = p.o + b * p.osb + h * p.osh + (int64_t)qrow * p.ost;
+#pragma unroll
+        for (int cc = 0; cc < HD / 32; ++cc) {
+          tmem_ld32(tO(x) + lane_off + cc * 32, o);
+          if (qrow < p.T) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              uint4 q;
+              q.x = pack_bf16x2(o[8 * g] * inv, o[8 * g + 1] * inv);
+              q.y = pack_bf16x2(o[8 * g + 2] * inv, o[8 * g + 3] * inv);
+              q.z = pack_bf16x2(o[8 * g + 4] * inv, o[8 * g + 5] * inv);
+              q.w = pack_bf16x2(o[8 * g + 6] * inv, o[8 * g + 7] * inv);
+              *reinterpret_cast<uint4*>(orow + cc * 32 + 8 * g) = q;
+            }
+          }
+        }
+        if (qrow < p.T) p.lse[(int64_t)bh * p.T + qrow] = (m_used + __log2f(l)) * kLn2;
+      }
+      if (!ok) break;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[slot]);
+      jx += nb;
+    }
+  };
+  // The same for modified scores: one streaming pass per block against the
+  // maximum that the rows have so far (Score::stream). Blocks with masked
+  // places, a row whose scores outgrow its maximum and scores past the short
+  // form of tanh take steps instead, from the raw scores still in TMEM.
+  [[maybe_unused]] auto softmax_general = [&]() {
+    const int x = (warp - kSoftmaxWarp) >> 2;
+    const int quad = warp & 3;
+    const int r = quad * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    bool ok = true;
+    int jx = 0, ii = 0;
+    for (; ok; ++ii) {
+      const int slot = ii & 1;
+      if (!(ok = mbar_wait(&item_full[slot], (ii >> 1) & 1, abort_flag, err))) break;
+      const FwdItem inf = items[slot];
+      if (inf.nkv < 0) break;  // no more items
+      const int nb = x == 0 ? inf.n0 : (inf.has1 ? inf.nkv : 0);
+      const int j0 = x == 0 ? inf.nkv - nb : 0;
+      const int bh = inf.bh, b = bh / p.H, h = bh - b * p.H;
+      const int q0 = inf.pr * 2 * FQ;
+      const int d0 = q0 / FK;
+      const int qrow = q0 + x * FQ + r;
+      const int* segrow = SEG ? p.seg + (int64_t)b * p.T : nullptr;
+      const int2* segtab = SEG ? segtab_of(slot) : nullptr;
+      // this row's segment id (rows past T take one no key has)
+      const int sq = SEG ? (qrow < p.T ? seg_query_id(segrow[qrow]) : -2) : 0;
+      const int2 qrng = SEG ? seg_range(segtab, inf.nch, 2 * (d0 + x), 2) : make_int2(0, 0);
+      // the last key this row sees under the causal and the prefix mask
+      const int last = max(qrow, inf.prefix - 1);
+      const Score<MODE> score(p, (MODE & kBias) ? p.slopes[h] * kLog2e : 0.f);
+      float m_used = -INFINITY, l = 0.f;
+      for (int j = 0; j < nb && ok; ++j) {
+        const int jj = jx + j;
+        const int jb = kblock(slot, j0 + j, inf.nkv);
+        int kid[4] = {0, 0, 0, 0};  // the block's key ids, lane l keys l + 32 w
+        if constexpr (SEG) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int key = jb * FK + 32 * w + lane;
+            kid[w] = key < p.T ? seg_key_id(segrow[key]) : -1;
+          }
+        }
+        // keys past a query (and past T) are masked, keys of another id too
+        const bool diag = jb * FK + FK - 1 > max(q0 + x * FQ, inf.prefix - 1);
+        const bool segmask = SEG && !rng_single(seg_range(segtab, inf.nch, 2 * jb, 2), qrng);
+        const bool ahead = (MODE & kBias) && jb * FK + FK - 1 > q0 + x * FQ;  // |i - j| either way
+        if (!(ok = mbar_wait(&s_full[x], jj & 1, abort_flag, err))) break;
+        tc_fence_after();
+        // P and O of the previous block must have been consumed by its P.V MMA
+        if (j > 0) {
+          if (!(ok = mbar_wait(&pv_done[x], (jj - 1) & 1, abort_flag, err))) break;
+          tc_fence_after();
+        }
+        const uint32_t aS = tS(x) + lane_off, aP = tP(x) + lane_off;
+        const float at0 = (float)(jb * FK - qrow);
+        uint32_t v[32], pk[16];
+        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        float alpha = 1.f;
+        bool rescale = false;
+        bool steps = diag || segmask || ahead;
+        if (!steps) {
+          float top = -INFINITY, far = 0.f;
+#pragma unroll 1
+          for (int w = 0; w < 4; ++w) {
+            tmem_ld32_nw(aS + 32 * w, v);
+            tmem_wait_ld();
+            score.stream(v, at0 + (float)(32 * w), m_used, pk, acc, top, far);
+            tmem_st8_nw(aP + 16 * w, pk);
+            tmem_st8_nw(aP + 16 * w + 8, pk + 8);
+          }
+          steps = Score<MODE>::discard(top, far);
+        }
+        if (steps) {
+          // Masks, a new maximum or tanh's long form: modified scores go back
+          // into S, then the maximum, then the probabilities. Words (32 keys)
+          // hidden from the whole warp cost nothing but their zeros.
+          uint32_t see[4];  // which keys this row sees
+          causal_words(last - jb * FK, see);
+          if (segmask) segment_words(kid, sq, see);
+          float top = -INFINITY;
+          unsigned hidden = 0;  // bit w: word w
+#pragma unroll 1
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t sees = w < 2 ? (w == 0 ? see[0] : see[1]) : (w == 2 ? see[2] : see[3]);
+            if (__all_sync(0xffffffffu, sees == 0u)) {
+              hidden |= 1u << w;
+              continue;
+            }
+            const bool full = __all_sync(0xffffffffu, sees == 0xffffffffu);
+            tmem_ld32_nw(aS + 32 * w, v);
+            tmem_wait_ld();
+            top = fmaxf(top, score.modify(v, at0 + (float)(32 * w), sees, full));
+            tmem_st32(aS + 32 * w, reinterpret_cast<const float*>(v));
+          }
+          // Decided per warp (the TMEM accesses of O are warp-collective); a row
+          // whose max stays rescales by 1, one that has seen no key yet too.
+          rescale = __any_sync(0xffffffffu, top > m_used + 8.0f);
+          if (rescale) {
+            const float m_new = fmaxf(m_used, top);
+            alpha = m_new == -INFINITY ? 1.f : ex2(m_used - m_new);
+            m_used = m_new;
+          }
+          const float sub = m_used == -INFINITY ? 0.f : m_used;  // exp2(-inf - sub) = 0
+          acc[0] = acc[1] = make_float2(0.f, 0.f);
+#pragma unroll 1
+          for (int w = 0; w < 4; ++w) {
+            if ((hidden >> w) & 1u) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pk[i] = 0;
+            } else {
+              tmem_ld32_nw(aS + 32 * w, v);
+              tmem_wait_ld();
+              Score<MODE>::exponentials(v, sub, pk, acc);
+            }
+            tmem_st8_nw(aP + 16 * w, pk);
+            tmem_st8_nw(aP + 16 * w + 8, pk + 8);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[x]);
+        const float2 s2 = fadd2(acc[0], acc[1]);
+        const float sum = s2.x + s2.y;
+        l = l * alpha + sum;
+        if (rescale && j > 0) {
+          float o[32];
+#pragma unroll
+          for (int cc = 0; cc < HD / 32; ++cc) {
+            tmem_ld32(tO(x) + lane_off + cc * 32, o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= alpha;
+            tmem_st32(tO(x) + lane_off + cc * 32, o);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x]);
+      }
+      if (ok && nb > 0) {
+        if (!(ok = mbar_wait(&pv_done[x], (jx + nb - 1) & 1, abort_flag, err))) break;
+        tc_fence_after();
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key: zeros
         float o[32];
         bf16* orow = p.o + b * p.osb + h * p.osh + (int64_t)qrow * p.ost;
 #pragma unroll
@@ -935,8 +1107,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
           }
         }
         if (qrow < p.T)
-          p.lse[(int64_t)bh * p.T + qrow] =
-              GENERAL && l == 0.f ? -INFINITY : (m_used + __log2f(l)) * kLn2;
+          p.lse[(int64_t)bh * p.T + qrow] = l == 0.f ? -INFINITY : (m_used + __log2f(l)) * kLn2;
       }
       if (!ok) break;
       tc_fence_before();
@@ -955,7 +1126,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
       }
     } else {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFwdRegsSoftmax));
-      softmax();
+      softmax_general();
     }
   } else if (warp == 0) {
     produce();
@@ -1173,7 +1344,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           }
           mn = __reduce_min_sync(0xffffffffu, mn);
           mx = __reduce_max_sync(0xffffffffu, mx);
-          if (lane == 0) tab[c] = seg_chunk<true>(mn, mx);
+          if (lane == 0) tab[c] = seg_chunk(mn, mx);
         }
         __syncwarp();
         if (lane == 0) {
@@ -1408,9 +1579,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const int nch = (p.T + kSegChunk - 1) / kSegChunk -
                       (GENERAL ? inf.qb / kSegChunk : 2 * inf.kt);
       // this key row's segment id (rows past T take an id no query has)
-      const int sk = segrow ? (key < p.T ? seg_key_id<GENERAL>(segrow[key])
-                                         : (GENERAL ? -1 : INT_MAX))
-                            : 0;
+      int sk = segrow ? (key < p.T ? segrow[key] : INT_MAX) : 0;
+      if (SEG && GENERAL) sk = key < p.T ? seg_key_id(sk) : -1;
       const int2 krng =
           segrow ? seg_range(segtab, nch, -qoff / kSegChunk, 2) : make_int2(0, 0);
       for (int it = wg; it < nq; it += kBwdSmGroups, ql += kBwdSmGroups) {
@@ -2061,7 +2231,6 @@ static AttnParams score_params(const gptb200_score_attention* a) {
   p.cap = a->softcap;
   p.slopes = a->slopes;
   p.prefix = a->prefix_lens;
-  p.by_weight = getenv("BYW") ? atoi(getenv("BYW")) : 1;
   p.o = reinterpret_cast<bf16*>(a->o);
   p.osb = a->o_stride[0];
   p.osh = a->o_stride[1];
@@ -2069,6 +2238,20 @@ static AttnParams score_params(const gptb200_score_attention* a) {
   p.lse = a->lse;
   p.seg = a->segment_ids;
   return p;
+}
+
+// Whether a launch walks the items of all heads by falling weight instead of
+// head by head. By weight the last items are light and every SM ends at about
+// the same time; head by head the tiles that the items of a head share stay in
+// L2. So: by weight while the shared tiles of all heads (`bytes`) fit, and
+// longer for capped scores, which compute more per byte. Measured at 12 heads,
+// capped and biased | without either (us, by weight / head by head):
+//   forward  1 x 8192: 299 / 370 | 170 / 215;   128 x 1024: 872 / 1142 | 486 / 463
+//   backward 1 x 8192: 537 / 655 | 343 / 391;   48 x 1024:  567 / 623  | 504 / 462
+//   backward 16 x 8192: 9660 / 9213 | 7502 / 5887
+static int by_weight(const gptb200_score_attention* a, int64_t bytes, int64_t plain_limit,
+                     int64_t cap_limit) {
+  return bytes <= (a->softcap > 0.f ? cap_limit : plain_limit) << 20;
 }
 
 // One persistent launch: the shared-memory attribute (set once per kernel and
@@ -2133,6 +2316,8 @@ extern "C" int gptb200_score_attention_fwd(const gptb200_score_attention* a, voi
     return GPTB200_ESHAPE;
   p.sched = sched_slot(0);
   if (!p.sched) return GPTB200_EUNSUPPORTED;
+  // K and V of every head
+  p.by_weight = by_weight(a, a->batch * a->kv_heads * a->seq * 2 * HD * 2, 160, 512);
   auto st = reinterpret_cast<cudaStream_t>(stream);
   return score_mode(a, [&](auto mode) {
     constexpr int MODE = decltype(mode)::value;
@@ -2186,6 +2371,8 @@ extern "C" int gptb200_score_attention_bwd(const gptb200_score_attention* a, con
   p.st = dkv_stride[2];
   p.rcos = reinterpret_cast<const bf16*>(rope_cos);
   p.rsin = reinterpret_cast<const bf16*>(rope_sin);
+  // Q and dO of every head
+  p.by_weight = by_weight(a, rows * 2 * HD * 2, 64, 256);
   const bool two = p.T >= 2048;  // softmax groups, as in the plain backward
   const int e = score_mode(a, [&](auto mode) {
     constexpr int MODE = decltype(mode)::value;

@@ -175,9 +175,10 @@ def test_slopes_of_either_sign_and_zero(cuda):
 
 
 @pytest.mark.gpu
-def test_plain_options_equal_causal_attention(cuda):
-    """Without cap, bias, prefix and padding: the plain kernels' outputs, bit for
-    bit (the same arithmetic in the same order; dq's parts arrive in any order)."""
+def test_plain_options_agree_with_causal_attention(cuda):
+    """Without cap, bias, prefix and padding this is the plain kernels' attention.
+    The two round P against different row maxima, so each is within the formula's
+    bounds and they are within twice those of each other."""
 
     for t, ids in ((300, False), (300, True), (2100, False)):
         q, k, v, do = (x.to(cuda) for x in _inputs(2, 2, 2, t, 5))
@@ -187,9 +188,10 @@ def test_plain_options_equal_causal_attention(cuda):
         ops.attention_fwd(q, k, v, o, plain, scale=0.125, segment_ids=seg)
         grads = [torch.empty_like(x) for x in (q, k, v)]
         ops.attention_bwd(q, k, v, o, do, plain, *grads, scale=0.125, segment_ids=seg)
-        assert torch.equal(got["o"], o) and torch.equal(lse, plain)
-        assert torch.equal(got["dk"], grads[1]) and torch.equal(got["dv"], grads[2])
-        assert (got["dq"].double() - grads[0].double()).norm() <= 1e-4 * grads[0].double().norm()
+        assert (lse - plain).abs().max() <= 32 * 2.0 ** -24 * (1 + plain.abs().max())
+        _, tol, _ = _formula(q, k, v, do, 0.125, 0.0, None, seg, None)
+        for n, want in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+            assert ((got[n].double() - want.double()).abs() <= 2 * tol[n]).all(), n
 
 
 @pytest.mark.gpu
