@@ -83,7 +83,8 @@ struct AttnParams {
   int64_t osb, osh, ost;
   float* lse;          // [B, H, T], natural log
   const bf16* dout;
-  const float* delta;  // [B, H, T]
+  const float* delta;  // [B, H, T] (MODE > kClassic: negated)
+  const float* neg_lse2;  // [B, H, T] -lse log2(e) (MODE > kClassic)
   float* dq_acc;       // [B, H, T, 64] fp32
   bf16* dk;
   bf16* dv;
@@ -367,6 +368,91 @@ struct Score {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = (see >> i) & 1u ? v[i] : __float_as_uint(to);
   }
+  // Backward, transposed: one key against 16 queries. stat: the queries' -lse
+  // log2(e) at [0, 16) and -delta at [64, 80). P = exp2(s' log2(e) - lse log2(e))
+  // and dS = P (dP - delta) ds'/ds, packed; zero at queries not in `see`.
+  // at: key - query of column 0. EDGE: with hidden queries or keys past a query;
+  // apart, because its tests would be issued (predicated off) in every chunk.
+  template <bool EDGE>
+  GPTB200_DEV void gradients(uint32_t (&s)[16], const uint32_t (&d)[16], const float* stat, float at,
+                             uint32_t see, uint32_t (&pk)[8], uint32_t (&dk)[8]) const {
+    bool large = false;
+    if constexpr (CAP) {
+      float far[2] = {0.f, 0.f};
+      if constexpr (EDGE) {  // hidden scores do not choose tanh's form
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = (see >> j) & 1u ? s[j] : 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < 16; j += 2)
+        far[(j >> 1) & 1] =
+            fmax3_abs(far[(j >> 1) & 1], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+      large = __any_sync(0xffffffffu, fmaxf(far[0], far[1]) * z_per_s > 1.f);
+    }
+    float2 k[5];
+    if constexpr (CAP) {
+      constexpr float c[5] = GPTB200_TANH_COEFS;
+#pragma unroll
+      for (int u = 0; u < 5; ++u) k[u] = both(c[u]);
+    }
+    float2 b = make_float2(slope2 * at, slope2 * (at - 1.f));  // the bias, key up to the query
+#pragma unroll
+    for (int j = 0; j < 16; j += 8) {
+      float2 t[4], w[4];  // tanh (without a cap: the raw score), ds' / ds
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        t[q] = make_float2(__uint_as_float(s[j + 2 * q]), __uint_as_float(s[j + 2 * q + 1]));
+      if constexpr (CAP) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) t[q] = fmul2(t[q], both(z_per_s));
+        if (large) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) t[q] = make_float2(tanh_any(t[q].x), tanh_any(t[q].y));
+        } else {
+          float2 u[4], a[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) u[q] = fmul2(t[q], t[q]);
+          poly4(k, u, a);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) t[q] = fmul2(t[q], a[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w[q] = ffma2(fmul2(t[q], t[q]), both(-1.f), both(1.f));
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int i = j + 2 * q;
+        const float4 n4 = *reinterpret_cast<const float4*>(stat + (i & ~3));
+        const float4 g4 = *reinterpret_cast<const float4*>(stat + 64 + (i & ~3));
+        float2 n = q & 1 ? make_float2(n4.z, n4.w) : make_float2(n4.x, n4.y);
+        const float2 g = q & 1 ? make_float2(g4.z, g4.w) : make_float2(g4.x, g4.y);
+        if constexpr (BIAS) {
+          if constexpr (EDGE) {
+            n.x = fmaf(-slope2, fabsf(at - (float)i), n.x);
+            n.y = fmaf(-slope2, fabsf(at - (float)(i + 1)), n.y);
+          } else {
+            n = fadd2(n, b);
+            b = fadd2(b, both(-2.f * slope2));
+          }
+        }
+        float2 x = ffma2(t[q], both(out), n);
+        x = make_float2(ex2(x.x), ex2(x.y));
+        float2 y = fmul2(x, fadd2(make_float2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), g));
+        if constexpr (CAP) y = fmul2(y, w[q]);
+        pk[i / 2] = pack_bf16x2(x.x, x.y);
+        dk[i / 2] = pack_bf16x2(y.x, y.y);
+      }
+    }
+    if constexpr (EDGE) {  // halves of the packed pairs
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t keep = ((see >> (2 * i)) & 1u ? 0x0000ffffu : 0u) |
+                              ((see >> (2 * i + 1)) & 1u ? 0xffff0000u : 0u);
+        pk[i] &= keep;
+        dk[i] &= keep;
+      }
+    }
+  }
   // Probabilities of modified scores.
   static GPTB200_DEV void exponentials(const uint32_t (&v)[32], float m, uint32_t (&pk)[16],
                                        float2 (&acc)[2]) {
@@ -406,6 +492,20 @@ GPTB200_DEV void segment_words(const int (&kid)[4], int sq, uint32_t (&see)[4]) 
   }
 #pragma unroll
   for (int w = 0; w < 4; ++w) see[w] &= same[w];
+}
+
+// Bits of the 16 queries that carry the key's id; id: of query `lane % 16`. One
+// ballot for every distinct id among the warp's 32 keys.
+GPTB200_DEV uint32_t segment_columns(int id, int key_id) {
+  uint32_t same = 0, left = 0xffffffffu;
+  while (left) {
+    const int one = __shfl_sync(0xffffffffu, key_id, __ffs(left) - 1);
+    const uint32_t b = __ballot_sync(0xffffffffu, id == one);
+    const bool mine = key_id == one;
+    if (mine) same = b & 0xffffu;
+    left &= ~__ballot_sync(0xffffffffu, mine);
+  }
+  return same;
 }
 
 // Padding (a negative id) never equals another id: queries carry -2, keys -1.
@@ -1202,8 +1302,18 @@ struct BwdSmem {
   static constexpr int TOTAL = BAR + 272;
 };
 
+// MODE > kClassic: the modified scores need more registers and more arithmetic
+// for each fetched statistic, so 8 softmax warps with wide register shares take
+// whole tiles in turn (two groups of four, 64 columns a warp) instead of 16
+// narrow ones. Warps 0-3 load and issue (TMA, gradient MMAs, score MMAs, idle),
+// 4-11 are the softmax, 12-15 read dQ out; shares per warpgroup as in the forward.
+constexpr int kBwdGeneralThreads = 32 * 24;
+constexpr int kBwdRegs = 80, kBwdRegsIssue = 48, kBwdRegsSoftmax = 80, kBwdRegsFlush = 112;
+static_assert(kBwdRegsIssue + 4 * kBwdRegsSoftmax + kBwdRegsFlush == 6 * kBwdRegs,
+              "register shares");
+
 template <bool SEG, int GROUPS, int MODE>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(MODE == kClassic ? kBwdThreads : kBwdGeneralThreads, 1)
     attn_bwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
                 const __grid_constant__ CUtensorMap tmDQ, const AttnParams p) {
@@ -1211,7 +1321,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   constexpr bool GENERAL = MODE != kClassic;
   constexpr int kQS = L::kQStages;
   constexpr int kBwdSmGroups = GROUPS;
-  constexpr int kBwdGroupWarps = kBwdSmWarps / kBwdSmGroups;
+  constexpr int kSmWarps = kBwdSmWarps;
+  constexpr int kSmWarp0 = GENERAL ? 4 : 2;  // first softmax warp
+  constexpr int kScoreWarp = GENERAL ? 2 : kBwdScoreWarp;
+  constexpr int kFlushWarp = GENERAL ? 20 : kBwdFlushWarp;
+  constexpr int kBwdGroupWarps = kSmWarps / kBwdSmGroups;
   constexpr int kBwdWarpCols = 64 / (kBwdGroupWarps / 4);
   extern __shared__ __align__(1024) uint8_t smem_bwd[];
   uint8_t* sm = smem_bwd;
@@ -1261,7 +1375,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&kv_full[s], 1);
       mbar_init(&kv_empty[s], 1);
       mbar_init(&item_full[s], 1);
-      mbar_init(&item_empty[s], kBwdItemUsers);
+      mbar_init(&item_empty[s], kBwdItemUsers - kBwdSmWarps + kSmWarps);
       mbar_init(&dq_full[s], 1);
       mbar_init(&dq_free[s], 4);
     }
@@ -1292,7 +1406,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const uint32_t tDV = tmem + 384, tDK = tmem + 448;
   auto tBuf = [&](int bb) { return tmem + 128 * bb; };
 
-  if (warp == 0) {
+  auto produce = [&]() {
     // Item producer: publishes each item's slot (and, with segment ids, its
     // chunk ranges and query-tile list), then loads its K/V and Q/dO tiles.
     bool ok = true;
@@ -1412,7 +1526,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       // query head: the key/value head's own, or the first of its group
       int hq = GENERAL ? h * p.group : h;
-      const float* Lg = p.lse + ((int64_t)b * p.H + hq) * p.T;
+      // (GENERAL: -lse log2(e) and -delta, as the arithmetic uses them)
+      const float* Lg = (GENERAL ? p.neg_lse2 : p.lse) + ((int64_t)b * p.H + hq) * p.T;
       const float* Dg = p.delta + ((int64_t)b * p.H + hq) * p.T;
       int ql = 0;  // entry of the head's list
       for (int it = 0; ok && it < nq; ++it, ++ql, ++g) {
@@ -1448,7 +1563,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         cp_async_mbar_arrive(&q_full[s]);
       }
     }
-  } else if (warp == 1) {
+  };
+  auto gradients = [&]() {
     // Gradient MMAs of tile g once its softmax is done. This thread and the
     // scores thread (warp 18) issue independently: a thread that stops at a
     // barrier leaves the tensor pipe to the other one.
@@ -1503,7 +1619,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         mbar_arrive(&item_empty[slot]);
       }
     }
-  } else if (warp == kBwdScoreWarp) {
+  };
+  auto scores = [&]() {
     // S^T = K Q^T and dP^T = V dO^T of each tile into TMEM buffer g % 3, as
     // far ahead as the buffers allow. The buffer last served tile g-3: read by
     // that tile's dV / dK MMAs and, when g-3 closed a query pair, holding that
@@ -1546,7 +1663,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         mbar_arrive(&item_empty[slot]);
       }
     }
-  } else if (warp < 2 + kBwdSmWarps) {
+  };
+  auto softmax = [&]() {
     // Softmax group wg takes the tiles it = wg, wg + kBwdSmGroups, ... of
     // each item. Warp w reads TMEM lanes of quadrant w % 4 (key rows) and
     // kBwdWarpCols query columns of the tile, in 16-column groups cg, and
@@ -1554,8 +1672,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     // warp overwrites scores another warp has yet to read. The tile's
     // statistics come from the shared memory of its Q/dO stage (cp.async).
     const int quad = warp & 3;
-    const int wg = (warp - 2) / kBwdGroupWarps;
-    const int cg0 = (((warp - 2) % kBwdGroupWarps) >> 2) * (kBwdWarpCols / 16);
+    const int wg = (warp - kSmWarp0) / kBwdGroupWarps;
+    const int cg0 = (((warp - kSmWarp0) % kBwdGroupWarps) >> 2) * (kBwdWarpCols / 16);
     const int r = quad * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const float c = p.scale * kLog2e;
@@ -1571,6 +1689,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const int k0 = inf.kt * BT;
       const int key = k0 + r;
       const int qoff = GENERAL ? inf.qb - k0 : 0;  // first query tile relative to the keys
+      [[maybe_unused]] Score<MODE> score(p, 0.f);
       // this key's row is seen by every query of its sequence
       const bool open = GENERAL && key < inf.prefix;
       int ql = wg, hq = GENERAL ? (inf.bh - b * heads) * p.group : 0;
@@ -1592,7 +1711,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const int bb = gt % 3;
         const uint32_t tb = tBuf(bb);
         const int qt = qtile(slot, GENERAL ? ql : it);  // query tile index (64 positions) past k0
-        const float slope2 = (MODE & kBias) ? p.slopes[hq] * kLog2e : 0.f;
+        if constexpr ((MODE & kBias) != 0) score.slope2 = p.slopes[hq] * kLog2e;
         if (!(ok = mbar_wait(&s_full[bb], (gt / 3) & 1, abort_flag, err))) break;
         if (!(ok = mbar_wait(&q_full[gt % kQS], (gt / kQS) & 1, abort_flag, err))) break;
         // The dS^T ring slot of this tile was last read by the dQ MMA of the
@@ -1601,6 +1720,63 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           break;
         tc_fence_after();
         uint8_t* sd = sm + L::DST + (gt & 3) * BT_BYTES;
+        if constexpr (GENERAL) {
+          const int q0 = qoff + qt * BQ;  // the tile's first query relative to the keys
+          // per-element segment test unless this key tile and query tile share one id
+          const bool segmask = SEG && !rng_single(seg_range(segtab, nch, qt, 1), krng);
+          const bool diag = q0 < BT;  // some key may be past some query
+          const float* stat =
+              reinterpret_cast<const float*>(sm + L::STAT + (gt % kQS) * L::kStatBytes);
+          const uint32_t ts = tb + lane_off;
+          auto fetch = [&](int cg, uint32_t (&sv)[16], uint32_t (&dp)[16]) {
+            tmem_ld16_nw(ts + cg * 16, sv);
+            tmem_ld16_nw(ts + 64 + cg * 16, dp);
+          };
+          auto put = [&](int cg, const uint32_t (&pk)[8], const uint32_t (&dk)[8]) {
+            tmem_st8_nw(ts + cg * 16, pk);
+            tmem_st8_nw(ts + cg * 16 + 8, dk);
+            *reinterpret_cast<uint4*>(sd + swz128(r, cg * 2)) = make_uint4(dk[0], dk[1], dk[2], dk[3]);
+            *reinterpret_cast<uint4*>(sd + swz128(r, cg * 2 + 1)) =
+                make_uint4(dk[4], dk[5], dk[6], dk[7]);
+          };
+          uint32_t pk[8], dk[8];
+          if (!diag && !segmask && k0 + q0 + BQ <= p.T) {
+            // every query sees every key
+#pragma unroll 1
+            for (int cg = cg0; cg < cg0 + kBwdWarpCols / 16; ++cg) {
+              uint32_t sv[16], dp[16];
+              fetch(cg, sv, dp);
+              tmem_wait_ld();
+              score.template gradients<false>(sv, dp, stat + cg * 16, (float)(r - q0 - cg * 16), 0,
+                                              pk, dk);
+              put(cg, pk, dk);
+            }
+          } else {
+#pragma unroll 1
+            for (int cg = cg0; cg < cg0 + kBwdWarpCols / 16; ++cg) {
+              uint32_t sv[16], dp[16];
+              fetch(cg, sv, dp);
+              const int rel = r - q0 - cg * 16;            // key - query of column 0
+              const int tail = p.T - k0 - q0 - cg * 16;    // columns from here lie past the end
+              // which of the 16 queries see this key
+              uint32_t see = 0xffffu;
+              if (diag && !open) see = rel <= 0 ? see : rel >= 16 ? 0u : see << rel & 0xffffu;
+              if (tail < 16) see &= tail <= 0 ? 0u : (1u << tail) - 1u;
+              if (segmask) {
+                const int id = reinterpret_cast<const int*>(stat)[128 + cg * 16 + (lane & 15)];
+                see &= segment_columns(seg_query_id(id), sk);
+              }
+              tmem_wait_ld();
+              if (__all_sync(0xffffffffu, see == 0u)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) pk[i] = dk[i] = 0;
+              } else {
+                score.template gradients<true>(sv, dp, stat + cg * 16, (float)rel, see, pk, dk);
+              }
+              put(cg, pk, dk);
+            }
+          }
+        } else {
 #pragma unroll
         for (int sub = 0; sub < kBwdWarpCols / 16; ++sub) {
         const int cg = cg0 + sub;
@@ -1613,9 +1789,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tmem_ld16_nw(tb + lane_off + cg * 16, sraw);
         tmem_ld16_nw(tb + 64 + lane_off + cg * 16, draw);
         tmem_wait_ld();
-        const int qbase = qoff + qt * BQ + cg * 16;  // query index relative to k0
-        // key r > query masks only near (with a prefix, before) the diagonal
-        const bool diag = GENERAL ? qoff + qt * BQ < BT : (qt < 2);
+        const int qbase = qt * BQ + cg * 16;  // query index relative to k0
+        const bool diag = (qt < 2);           // key r > query masks only near the diagonal
         const int tail = p.T - k0 - qbase;    // columns j >= tail lie past the sequence end
         const bool mask = diag || tail < 16;
         // per-element segment test unless this key tile and query tile share one id
@@ -1625,68 +1800,21 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         // tests run only on tiles that need them and the segment test only
         // when the tiles' ids differ.
         uint32_t pk[8], dk[8];
-        // tanh's short form needs |z| <= 1 of this warp's scores
-        const float kcap = (MODE & kCap) ? p.scale / p.cap : 0.f;
-        bool large = false;
-        if constexpr ((MODE & kCap) != 0) {
-          if (mask || segmask) {  // hidden scores do not choose the form
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if ((diag && !open && r > qbase + j) || j >= tail ||
-                  (SEG && segmask && (stat_seg[j] != sk || stat_seg[j] < 0)))
-                sraw[j] = 0;
-          }
-          float top = 0.f;
-#pragma unroll
-          for (int j = 0; j < 16; j += 2)
-            top = fmax3(top, fabsf(__uint_as_float(sraw[j])), fabsf(__uint_as_float(sraw[j + 1])));
-          large = __any_sync(0xffffffffu, top * kcap > 1.f);
-        }
         auto softmax_cols = [&](auto mask_tag) {
           constexpr bool kMask = decltype(mask_tag)::value;
-          const float2 c2 = (MODE & kCap) ? make_float2(p.cap * kLog2e, p.cap * kLog2e)
-                                          : make_float2(c, c);
+          const float2 c2 = make_float2(c, c);
           const float2 nlog2e = make_float2(-kLog2e, -kLog2e);
           const float2 m1 = make_float2(-1.f, -1.f);
 #pragma unroll
           for (int j4 = 0; j4 < 4; ++j4) {
             const float4 l4 = reinterpret_cast<const float4*>(stat)[j4];
             const float4 d4 = reinterpret_cast<const float4*>(stat + 64)[j4];
-            float2 s01 = make_float2(__uint_as_float(sraw[4 * j4]), __uint_as_float(sraw[4 * j4 + 1]));
-            float2 s23 = make_float2(__uint_as_float(sraw[4 * j4 + 2]),
-                                     __uint_as_float(sraw[4 * j4 + 3]));
-            [[maybe_unused]] float2 slope01, slope23;  // d s' / d (scaled score)
-            if constexpr ((MODE & kCap) != 0) {
-              const float2 k2 = make_float2(kcap, kcap), one = make_float2(1.f, 1.f);
-              s01 = fmul2(s01, k2);
-              s23 = fmul2(s23, k2);
-              if (large) {
-                s01 = make_float2(tanh_any(s01.x), tanh_any(s01.y));
-                s23 = make_float2(tanh_any(s23.x), tanh_any(s23.y));
-              } else {
-                s01 = tanh_small2(s01);
-                s23 = tanh_small2(s23);
-              }
-              slope01 = ffma2(make_float2(-s01.x, -s01.y), s01, one);
-              slope23 = ffma2(make_float2(-s23.x, -s23.y), s23, one);
-            }
-            float2 n01 = fmul2(make_float2(l4.x, l4.y), nlog2e);
-            float2 n23 = fmul2(make_float2(l4.z, l4.w), nlog2e);
-            if constexpr ((MODE & kBias) != 0) {
-              const float at = (float)(r - qbase - 4 * j4);  // key - query of column 4 j4
-              if (diag) {
-                n01.x = fmaf(-slope2, fabsf(at), n01.x);
-                n01.y = fmaf(-slope2, fabsf(at - 1.f), n01.y);
-                n23.x = fmaf(-slope2, fabsf(at - 2.f), n23.x);
-                n23.y = fmaf(-slope2, fabsf(at - 3.f), n23.y);
-              } else {  // no key past a query
-                const float2 sl = make_float2(slope2, slope2);
-                n01 = ffma2(sl, make_float2(at, at - 1.f), n01);
-                n23 = ffma2(sl, make_float2(at - 2.f, at - 3.f), n23);
-              }
-            }
-            const float2 x01 = ffma2(s01, c2, n01);
-            const float2 x23 = ffma2(s23, c2, n23);
+            const float2 x01 = ffma2(make_float2(__uint_as_float(sraw[4 * j4]),
+                                                 __uint_as_float(sraw[4 * j4 + 1])),
+                                     c2, fmul2(make_float2(l4.x, l4.y), nlog2e));
+            const float2 x23 = ffma2(make_float2(__uint_as_float(sraw[4 * j4 + 2]),
+                                                 __uint_as_float(sraw[4 * j4 + 3])),
+                                     c2, fmul2(make_float2(l4.z, l4.w), nlog2e));
             float pv[4] = {ex2(x01.x), ex2(x01.y), ex2(x23.x), ex2(x23.y)};
             // dP^T - delta as fma(delta, -1, dP^T): one rounding, as a subtraction
             const float2 g01 = ffma2(make_float2(d4.x, d4.y), m1,
@@ -1697,19 +1825,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                                                  __uint_as_float(draw[4 * j4 + 3])));
             float2 dv01 = fmul2(make_float2(pv[0], pv[1]), g01);
             float2 dv23 = fmul2(make_float2(pv[2], pv[3]), g23);
-            if constexpr ((MODE & kCap) != 0) {
-              dv01 = fmul2(dv01, slope01);
-              dv23 = fmul2(dv23, slope23);
-            }
             float dvs[4] = {dv01.x, dv01.y, dv23.x, dv23.y};
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
               const int j = 4 * j4 + u;
               bool off = false;
-              if (kMask) off = (diag && !open && r > qbase + j) || j >= tail;
-              if (SEG && segmask &&
-                  (stat_seg[j] != sk || (GENERAL && stat_seg[j] < 0)))
-                off = true;
+              if (kMask) off = (diag && r > qbase + j) || j >= tail;
+              if (SEG && segmask && stat_seg[j] != sk) off = true;
               if (off) pv[u] = dvs[u] = 0.f;
             }
             dv01 = make_float2(dvs[0], dvs[1]);
@@ -1731,6 +1853,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           *reinterpret_cast<uint4*>(sd + swz128(r, cg * 2 + q2)) =
               make_uint4(dk[4 * q2], dk[4 * q2 + 1], dk[4 * q2 + 2], dk[4 * q2 + 3]);
         }
+        }
         tmem_wait_st();
         fence_proxy_async_smem();
         tc_fence_before();
@@ -1742,9 +1865,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (lane == 0) mbar_arrive(&item_empty[slot]);
       g += nq;
     }
-  } else {
-    // dQ read-out: warp kBwdFlushWarp + i serves TMEM lane quadrant
-    // (kBwdFlushWarp + i) % 4. For each query pair (list entries 2j, 2j+1 of
+  };
+  auto flush = [&]() {
+    // dQ read-out: warp kFlushWarp + i serves TMEM lane quadrant
+    // (kFlushWarp + i) % 4. For each query pair (list entries 2j, 2j+1 of
     // an item; TMEM lane m is row m of the pair, quadrants 0-1 the first tile,
     // 2-3 the second) it loads its 32 rows x 64 fp32 columns as soon as the
     // pair's dQ MMA has completed, releases the TMEM buffer, stages the rows
@@ -1755,7 +1879,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     // this.
     const int quad = warp & 3;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-    uint8_t* stage = sm + L::DQS + (warp - kBwdFlushWarp) * 8192;
+    uint8_t* stage = sm + L::DQS + (warp - kFlushWarp) * 8192;
     bool ok = true;
     int g = 0, ii = 0;
     for (; ok; ++ii) {
@@ -1869,6 +1993,33 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       g += inf.nq;
     }
     if (lane == 0) bulk_wait_all();
+  };
+  if constexpr (GENERAL) {
+    if (warp < kSmWarp0) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBwdRegsIssue));
+      if (warp == 0) {
+        produce();
+      } else if (warp == 1) {
+        gradients();
+      } else if (warp == kScoreWarp) {
+        scores();
+      }
+    } else if (warp < kFlushWarp) {
+      softmax();
+    } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBwdRegsFlush));
+      flush();
+    }
+  } else if (warp == 0) {
+    produce();
+  } else if (warp == 1) {
+    gradients();
+  } else if (warp == kScoreWarp) {
+    scores();
+  } else if (warp < kSmWarp0 + kSmWarps) {
+    softmax();
+  } else {
+    flush();
   }
   tc_fence_before();
   __syncthreads();
@@ -1879,12 +2030,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   if (threadIdx.x == 0) sched_finish(p.sched);
 }
 
-// delta[bh, t] = sum_e dO * O, and zero the dQ accumulator row. Eight lanes
+// delta[bh, t] = sum_e dO * O, and zero the dQ accumulator row. With neg_lse2
+// the statistics as the score-modified backward takes them: -delta, -lse log2(e). Eight lanes
 // per row (16-byte loads), four rows per warp.
 __global__ void attn_delta_kernel(const bf16* __restrict__ o, const bf16* __restrict__ dout,
                                   int64_t osb, int64_t osh, int64_t ost, int64_t gsb, int64_t gsh,
                                   int64_t gst, int B, int H, int T, float* __restrict__ delta,
-                                  float* __restrict__ dq_acc) {
+                                  float* __restrict__ dq_acc, const float* __restrict__ lse,
+                                  float* __restrict__ neg_lse2) {
   const int64_t rows = (int64_t)B * H * T;
   const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
   const int seg = threadIdx.x & 7;
@@ -1911,7 +2064,10 @@ __global__ void attn_delta_kernel(const bf16* __restrict__ o, const bf16* __rest
   s += __shfl_xor_sync(0xffffffffu, s, 2);
   s += __shfl_xor_sync(0xffffffffu, s, 4);
   if (!valid) return;
-  if (seg == 0) delta[r] = s;
+  if (seg == 0) {
+    delta[r] = neg_lse2 ? -s : s;
+    if (neg_lse2) neg_lse2[r] = -kLog2e * lse[r];
+  }
   float4* z = reinterpret_cast<float4*>(dq_acc + r * HD + seg * 8);
   z[0] = make_float4(0.f, 0.f, 0.f, 0.f);
   z[1] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -2141,7 +2297,8 @@ extern "C" int gptb200_attention_bwd(const void* q, const void* k, const void* v
                                            (rows * 4 + 255) / 256 * 256);
   attn_delta_kernel<<<(unsigned)((rows * 8 + 255) / 256), 256, 0, st>>>(
       reinterpret_cast<const bf16*>(o), reinterpret_cast<const bf16*>(dout), o_stride_b,
-      o_stride_h, o_stride_t, o_stride_b, o_stride_h, o_stride_t, B, H, T, delta, dq_acc);
+      o_stride_h, o_stride_t, o_stride_b, o_stride_h, o_stride_t, B, H, T, delta, dq_acc, nullptr,
+      nullptr);
   GPTB200_CHECK_LAUNCH();
   AttnParams p = {};
   p.B = B;
@@ -2284,11 +2441,11 @@ static int score_fwd_launch(const AttnParams& p, const ScoreMaps& m, cudaStream_
                            FwdSmem<SEG>::TOTAL, st, m.q, m.k, m.v, p);
 }
 
-template <bool SEG, int GROUPS, int MODE>
+template <bool SEG, int MODE>
 static int score_bwd_launch(const AttnParams& p, const ScoreMaps& m, cudaStream_t st) {
   static bool done[64] = {};
   const int64_t items = (int64_t)((p.T + BT - 1) / BT) * p.B * p.KVH;
-  return launch_persistent(attn_bwd_tc<SEG, GROUPS, MODE>, done, items, kBwdThreads,
+  return launch_persistent(attn_bwd_tc<SEG, 2, MODE>, done, items, kBwdGeneralThreads,
                            BwdSmem<SEG>::TOTAL, st, m.q, m.k, m.v, m.g, m.dq, p);
 }
 
@@ -2325,6 +2482,13 @@ extern "C" int gptb200_score_attention_fwd(const gptb200_score_attention* a, voi
   });
 }
 
+extern "C" size_t gptb200_score_attention_bwd_workspace_size(int64_t batch, int64_t heads,
+                                                             int64_t seq) {
+  if (batch <= 0 || heads <= 0 || seq <= 0) return 0;
+  const int64_t rows = batch * heads * seq;
+  return (size_t)(2 * ((rows * 4 + 255) / 256 * 256) + rows * HD * 4);
+}
+
 extern "C" int gptb200_score_attention_bwd(const gptb200_score_attention* a, const void* dout,
                                            const int64_t* dout_stride, void* dq, void* dk, void* dv,
                                            const int64_t* dq_stride, const int64_t* dkv_stride,
@@ -2344,9 +2508,10 @@ extern "C" int gptb200_score_attention_bwd(const gptb200_score_attention* a, con
     return GPTB200_ESHAPE;
   AttnParams p = score_params(a);
   const int64_t rows = a->batch * a->heads * a->seq;
+  const int64_t stat_bytes = (rows * 4 + 255) / 256 * 256;
   float* delta = reinterpret_cast<float*>(workspace);
-  float* dq_acc = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) +
-                                           (rows * 4 + 255) / 256 * 256);
+  float* neg_lse2 = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + stat_bytes);
+  float* dq_acc = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + 2 * stat_bytes);
   ScoreMaps m;
   const int64_t *qs = a->q_stride, *ks = a->kv_stride;
   if (!make_map4(&m.q, a->q, p.B, p.H, p.T, qs[0], qs[1], qs[2], BQ) ||
@@ -2360,9 +2525,10 @@ extern "C" int gptb200_score_attention_bwd(const gptb200_score_attention* a, con
   auto st = reinterpret_cast<cudaStream_t>(stream);
   attn_delta_kernel<<<(unsigned)((rows * 8 + 255) / 256), 256, 0, st>>>(
       p.o, reinterpret_cast<const bf16*>(dout), p.osb, p.osh, p.ost, dout_stride[0], dout_stride[1],
-      dout_stride[2], p.B, p.H, p.T, delta, dq_acc);
+      dout_stride[2], p.B, p.H, p.T, delta, dq_acc, a->lse, neg_lse2);
   GPTB200_CHECK_LAUNCH();
   p.delta = delta;
+  p.neg_lse2 = neg_lse2;
   p.dq_acc = dq_acc;
   p.dk = reinterpret_cast<bf16*>(dk);
   p.dv = reinterpret_cast<bf16*>(dv);
@@ -2373,12 +2539,9 @@ extern "C" int gptb200_score_attention_bwd(const gptb200_score_attention* a, con
   p.rsin = reinterpret_cast<const bf16*>(rope_sin);
   // Q and dO of every head
   p.by_weight = by_weight(a, rows * 2 * HD * 2, 64, 256);
-  const bool two = p.T >= 2048;  // softmax groups, as in the plain backward
   const int e = score_mode(a, [&](auto mode) {
     constexpr int MODE = decltype(mode)::value;
-    if (p.seg)
-      return two ? score_bwd_launch<true, 2, MODE>(p, m, st) : score_bwd_launch<true, 1, MODE>(p, m, st);
-    return two ? score_bwd_launch<false, 2, MODE>(p, m, st) : score_bwd_launch<false, 1, MODE>(p, m, st);
+    return p.seg ? score_bwd_launch<true, MODE>(p, m, st) : score_bwd_launch<false, MODE>(p, m, st);
   });
   if (e) return e;
   int dev = 0, sms = 148;

@@ -155,6 +155,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_f32, c_vp, c_vp, c_vp, c_vp, c_vp],
     ),
     "gptb200_score_attention_fwd": (c_int, [ctypes.POINTER(ScoreAttention), c_vp]),
+    "gptb200_score_attention_bwd_workspace_size": (c_size, [c_i64, c_i64, c_i64]),
     "gptb200_score_attention_bwd": (
         c_int,
         [ctypes.POINTER(ScoreAttention), c_vp, ctypes.POINTER(c_i64), c_vp, c_vp, c_vp,

@@ -466,6 +466,10 @@ def score_attention_fwd(q, k, v, o, lse, *, scale: float, layout: str = "bhsd",
     return o, lse
 
 
+def score_attention_workspace_size(b: int, h: int, t: int) -> int:
+    return int(_lib.load().gptb200_score_attention_bwd_workspace_size(b, h, t))
+
+
 def score_attention_bwd(q, k, v, o, do, lse, dq, dk, dv, *, scale: float, layout: str = "bhsd",
                         softcap: float = 0.0, slopes=None, segment_ids=None, prefix_lens=None,
                         rope=None, workspace=None):
@@ -481,7 +485,7 @@ def score_attention_bwd(q, k, v, o, do, lse, dq, dk, dv, *, scale: float, layout
     dkvs = _tma_strides(dk, layout)
     if _tma_strides(dv, layout) != dkvs:
         raise ValueError("dk and dv must share strides")
-    size = int(_lib.load().gptb200_attention_bwd_workspace_size(b, h, t))
+    size = score_attention_workspace_size(b, h, t)
     if workspace is None:
         workspace = _scratch(size, q.device)
     elif workspace.numel() * workspace.element_size() < size:

@@ -273,7 +273,9 @@ int gptb200_score_attention_fwd(const gptb200_score_attention* call, void* strea
 /* Backward of the same call (o and lse as the forward wrote them). dq, dk, dv
  * are written; dk and dv share dkv_stride. With rope tables dq and dk are
  * rotated back as in gptb200_attention_bwd. workspace:
- * gptb200_attention_bwd_workspace_size(batch, heads, seq) bytes. */
+ * gptb200_score_attention_bwd_workspace_size(batch, heads, seq) bytes, 16-byte
+ * aligned. */
+size_t gptb200_score_attention_bwd_workspace_size(int64_t batch, int64_t heads, int64_t seq);
 int gptb200_score_attention_bwd(const gptb200_score_attention* call, const void* dout,
                                 const int64_t* dout_stride, void* dq, void* dk, void* dv,
                                 const int64_t* dq_stride, const int64_t* dkv_stride,
