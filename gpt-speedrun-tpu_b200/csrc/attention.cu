@@ -1302,11 +1302,13 @@ struct BwdSmem {
   static constexpr int TOTAL = BAR + 272;
 };
 
-// MODE > kClassic: the modified scores need more registers and more arithmetic
-// for each fetched statistic, so 8 softmax warps with wide register shares take
-// whole tiles in turn (two groups of four, 64 columns a warp) instead of 16
-// narrow ones. Warps 0-3 load and issue (TMA, gradient MMAs, score MMAs, idle),
-// 4-11 are the softmax, 12-15 read dQ out; shares per warpgroup as in the forward.
+// MODE > kClassic: whole warpgroups, so that registers can move from the one that
+// loads and issues (warps 0-3: TMA, gradient MMAs, score MMAs, idle) to the one
+// that reads dQ out (20-23); warps 4-19 are the softmax, in two groups on
+// alternate tiles. Measured (us, 1 x 12 x 8192 capped and biased | 8 x 12 x 1024):
+// 458 | 107 so, 494 | 116 with three groups of four warps, 513 | 116 with two
+// groups of four and twice the registers: fewer warps leave more of the TMEM
+// reads' latency in the open.
 constexpr int kBwdGeneralThreads = 32 * 24;
 constexpr int kBwdRegs = 80, kBwdRegsIssue = 48, kBwdRegsSoftmax = 80, kBwdRegsFlush = 112;
 static_assert(kBwdRegsIssue + 4 * kBwdRegsSoftmax + kBwdRegsFlush == 6 * kBwdRegs,
