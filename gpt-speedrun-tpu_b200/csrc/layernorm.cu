@@ -22,16 +22,20 @@
 namespace gptb200 {
 
 constexpr int kLnMaxWidth = 16384;
-// Rows a block of one-warp rows works on at a time.
-constexpr int kLnRows = 8;
+// Rows a block of one-warp rows works on at a time. The backward's lanes hold
+// three column sums, so its blocks are one to an SM and as wide as registers allow.
+constexpr int kLnRows = 8, kLnBwdRows = 8;
 
+// VEC elements as loaded. stay(): keeps a loop from holding the elements of a
+// loop-invariant vector unpacked, at twice the registers.
 template <typename T, int VEC>
-struct LnRaw;  // VEC elements as loaded
+struct LnRaw;
 template <>
 struct LnRaw<bf16, 8> {
   uint4 q;
   GPTB200_DEV void load(const bf16* p) { q = *reinterpret_cast<const uint4*>(p); }
   GPTB200_DEV void zero() { q = make_uint4(0, 0, 0, 0); }
+  GPTB200_DEV void stay() { asm volatile("" : "+r"(q.x), "+r"(q.y), "+r"(q.z), "+r"(q.w)); }
   GPTB200_DEV void get(float* v) const {
     unpack_bf16x2(q.x, v[0], v[1]);
     unpack_bf16x2(q.y, v[2], v[3]);
@@ -52,6 +56,7 @@ struct LnRaw<float, 8> {
     b = reinterpret_cast<const float4*>(p)[1];
   }
   GPTB200_DEV void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  GPTB200_DEV void stay() {}
   GPTB200_DEV void get(float* v) const {
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
     v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
@@ -66,6 +71,7 @@ struct LnRaw<bf16, 1> {
   bf16 q;
   GPTB200_DEV void load(const bf16* p) { q = *p; }
   GPTB200_DEV void zero() { q = __float2bfloat16(0.f); }
+  GPTB200_DEV void stay() {}
   GPTB200_DEV void get(float* v) const { v[0] = __bfloat162float(q); }
   static GPTB200_DEV void store(bf16* p, const float* v) { *p = __float2bfloat16(v[0]); }
 };
@@ -74,6 +80,7 @@ struct LnRaw<float, 1> {
   float q;
   GPTB200_DEV void load(const float* p) { q = *p; }
   GPTB200_DEV void zero() { q = 0.f; }
+  GPTB200_DEV void stay() {}
   GPTB200_DEV void get(float* v) const { v[0] = q; }
   static GPTB200_DEV void store(float* p, const float* v) { *p = v[0]; }
 };
@@ -111,23 +118,18 @@ struct LnParams {
   float eps;
 };
 
-template <int W>
-constexpr int ln_threads() {
-  return W == 1 ? 32 * kLnRows : 32 * W;
-}
-template <int W>
-constexpr int ln_rows_per_block() {
-  return W == 1 ? kLnRows : 1;
-}
+constexpr int ln_rows_per_block(int w, bool bwd) { return w > 1 ? 1 : bwd ? kLnBwdRows : kLnRows; }
+constexpr int ln_threads(int w, bool bwd) { return 32 * w * ln_rows_per_block(w, bwd); }
 
 template <typename T, int VEC, int W, int NV>
-__global__ void __launch_bounds__(ln_threads<W>()) ln_fwd_kernel(const LnParams p) {
+__global__ void __launch_bounds__(ln_threads(W, false)) ln_fwd_kernel(const LnParams p) {
+  constexpr bool AHEAD = true, BWD = false;
   using Raw = LnRaw<T, VEC>;
   __shared__ float2 red[2][W];
   int turn = 0;
   const int g = W == 1 ? threadIdx.x >> 5 : 0;
   const int t = W == 1 ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t step = (int64_t)gridDim.x * ln_rows_per_block<W>();
+  const int64_t step = (int64_t)gridDim.x * ln_rows_per_block(W, BWD);
   const T* x = reinterpret_cast<const T*>(p.x);
   T* y = reinterpret_cast<T*>(p.y);
   auto col = [&](int i) { return (i * 32 * W + t) * VEC; };
@@ -150,10 +152,17 @@ __global__ void __launch_bounds__(ln_threads<W>()) ln_fwd_kernel(const LnParams 
   }
   const float inv_d = 1.f / (float)p.d;
   Raw now[NV], next[NV];
-  int64_t r = (int64_t)blockIdx.x * ln_rows_per_block<W>() + g;
+  int64_t r = (int64_t)blockIdx.x * ln_rows_per_block(W, BWD) + g;
   if (r < p.rows) fetch(now, r);
   for (; r < p.rows; r += step) {
-    if (r + step < p.rows) fetch(next, r + step);
+    if constexpr (AHEAD) {
+      if (r + step < p.rows) fetch(next, r + step);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      w[i].stay();
+      c[i].stay();
+    }
     float sum = 0.f, none = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -192,23 +201,27 @@ __global__ void __launch_bounds__(ln_threads<W>()) ln_fwd_kernel(const LnParams 
         Raw::store(y + r * p.ldy + col(i), v);
       }
     }
+    if constexpr (AHEAD) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) now[i] = next[i];
+      for (int i = 0; i < NV; ++i) now[i] = next[i];
+    } else {
+      if (r + step < p.rows) fetch(now, r + step);
+    }
   }
 }
 
 // RES: dx_in is added. COL: the column sums of dx are wanted too.
 template <typename T, int VEC, int W, int NV, bool RES, bool COL>
-__global__ void __launch_bounds__(ln_threads<W>()) ln_bwd_kernel(const LnParams p) {
+__global__ void __launch_bounds__(ln_threads(W, true)) ln_bwd_kernel(const LnParams p) {
   using Raw = LnRaw<T, VEC>;
   // 32-bit rows have twice the bytes in flight already
-  constexpr bool AHEAD = sizeof(T) == 2;
+  constexpr bool AHEAD = sizeof(T) == 2, BWD = true;
   __shared__ float2 red[2][W];
   extern __shared__ float fold[];  // W == 1: one warp's columns for each row of the block
   int turn = 0;
   const int g = W == 1 ? threadIdx.x >> 5 : 0;
   const int t = W == 1 ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t step = (int64_t)gridDim.x * ln_rows_per_block<W>();
+  const int64_t step = (int64_t)gridDim.x * ln_rows_per_block(W, BWD);
   const T* x = reinterpret_cast<const T*>(p.x);
   const T* dy = reinterpret_cast<const T*>(p.dy);
   const T* res = reinterpret_cast<const T*>(p.dx_in);
@@ -247,12 +260,14 @@ __global__ void __launch_bounds__(ln_threads<W>()) ln_bwd_kernel(const LnParams 
   }
   const float inv_d = 1.f / (float)p.d;
   Row now, next;
-  int64_t r = (int64_t)blockIdx.x * ln_rows_per_block<W>() + g;
+  int64_t r = (int64_t)blockIdx.x * ln_rows_per_block(W, BWD) + g;
   if (r < p.rows) fetch(now, r);
   for (; r < p.rows; r += step) {
     if constexpr (AHEAD) {
       if (r + step < p.rows) fetch(next, r + step);
     }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) w[i].stay();
     const float mean = now.mean, rstd = now.rstd;
     const float shift = -mean * rstd;
     float s0 = 0.f, s1 = 0.f;
@@ -326,7 +341,7 @@ __global__ void __launch_bounds__(ln_threads<W>()) ln_bwd_kernel(const LnParams 
       for (int k = threadIdx.x; k < p.d; k += blockDim.x) {
         float s = 0.f;
 #pragma unroll
-        for (int u = 0; u < kLnRows; ++u) s += fold[u * p.d + k];
+        for (int u = 0; u < kLnBwdRows; ++u) s += fold[u * p.d + k];
         out[k] = s;
       }
     }
@@ -361,21 +376,29 @@ __global__ void __launch_bounds__(512) ln_sums_kernel(const float* __restrict__ 
   }
 }
 
-static int ln_sms() {
+static int ln_sms() {  // of the current device, asked once
+  static int known[64] = {};
   int dev = 0, n = 148;
   cudaGetDevice(&dev);
+  if (dev < 64 && known[dev]) return known[dev];
   cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (dev < 64) known[dev] = n;
   return n;
 }
 
-// Blocks of the backward: each leaves one row of partials, so the grid is
-// bounded by what can be resident (kLnBwdWarps warps on an SM).
-constexpr int kLnBwdWarps = 16;
-static int ln_warps(int64_t d) { return d <= 1024 ? 1 : d <= 4096 ? 4 : 16; }
-static int64_t ln_blocks(int64_t rows, int64_t d, int warps_per_sm) {
-  const int w = ln_warps(d);
-  const int64_t per = w == 1 ? kLnRows : 1;
-  const int64_t fit = (int64_t)ln_sms() * std::max(1, warps_per_sm / (w == 1 ? kLnRows : w));
+// Warps that share a row: as few as keep a lane's elements in registers, four
+// 8-element chunks at most, or for element accesses eight (up to 4096) or 32.
+static int ln_warps(int64_t d, bool vec) {
+  if (vec) return d <= 1024 ? 1 : d <= 8192 ? 8 : 16;
+  return d <= 256 ? 1 : d <= 1024 ? 4 : 16;
+}
+// A grid of what can be resident, or one pass over the rows. The backward's
+// blocks leave one row of partials each: `warps` on an SM.
+constexpr int kLnFwdWarps = 32, kLnBwdWarps = 16;
+static int64_t ln_blocks(int64_t rows, int w, bool bwd) {
+  const int64_t per = ln_rows_per_block(w, bwd);
+  const int block_warps = ln_threads(w, bwd) / 32;
+  const int64_t fit = (int64_t)ln_sms() * std::max(1, (bwd ? kLnBwdWarps : kLnFwdWarps) / block_warps);
   return std::min((rows + per - 1) / per, fit);
 }
 
@@ -383,30 +406,24 @@ static int64_t ln_blocks(int64_t rows, int64_t d, int warps_per_sm) {
 // allow 16-byte accesses, single elements otherwise.
 template <typename F>
 static int ln_dispatch(int64_t d, bool vec, F&& f) {
-  const int w = ln_warps(d);
+  const int w = ln_warps(d, vec);
+  const int n = (int)((d + 32 * w - 1) / (32 * w));  // elements of a lane
 #define GPTB200_LN(V, W, N) return f.template operator()<V, W, N>()
-  if (vec) {
-    const int n = (int)((d + 256 * w - 1) / (256 * w));
-    if (w == 1) {
-      if (n <= 1) GPTB200_LN(8, 1, 1);
-      if (n <= 2) GPTB200_LN(8, 1, 2);
-      if (n <= 3) GPTB200_LN(8, 1, 3);
-      GPTB200_LN(8, 1, 4);
-    }
-    if (w == 4) {
-      if (n <= 2) GPTB200_LN(8, 4, 2);
-      if (n <= 3) GPTB200_LN(8, 4, 3);
-      GPTB200_LN(8, 4, 4);
-    }
-    if (n <= 2) GPTB200_LN(8, 16, 2);
-    GPTB200_LN(8, 16, 4);
+  if (vec && w == 1) {
+    if (n <= 8) GPTB200_LN(8, 1, 1);
+    if (n <= 16) GPTB200_LN(8, 1, 2);
+    if (n <= 24) GPTB200_LN(8, 1, 3);
+    GPTB200_LN(8, 1, 4);
   }
-  const int n = (int)((d + 32 * w - 1) / (32 * w));
-  if (w == 1) {
-    if (n <= 8) GPTB200_LN(1, 1, 8);
-    GPTB200_LN(1, 1, 32);
+  if (vec && w == 8) {
+    if (n <= 8) GPTB200_LN(8, 8, 1);
+    if (n <= 16) GPTB200_LN(8, 8, 2);
+    GPTB200_LN(8, 8, 4);
   }
-  if (w == 4) GPTB200_LN(1, 4, 32);
+  if (vec) GPTB200_LN(8, 16, 4);
+  if (w == 1) GPTB200_LN(1, 1, 8);
+  if (w == 4) GPTB200_LN(1, 4, 8);
+  if (n <= 8) GPTB200_LN(1, 16, 8);
   GPTB200_LN(1, 16, 32);
 #undef GPTB200_LN
 }
@@ -417,8 +434,8 @@ struct LnForward {
   cudaStream_t st;
   template <int VEC, int W, int NV>
   int operator()() const {
-    const unsigned blocks = (unsigned)ln_blocks(p.rows, p.d, 48);
-    ln_fwd_kernel<T, VEC, W, NV><<<blocks, ln_threads<W>(), 0, st>>>(p);
+    const unsigned blocks = (unsigned)ln_blocks(p.rows, W, false);
+    ln_fwd_kernel<T, VEC, W, NV><<<blocks, ln_threads(W, false), 0, st>>>(p);
     GPTB200_CHECK_LAUNCH();
     return 0;
   }
@@ -436,9 +453,9 @@ struct LnBackward {
   }
   template <int VEC, int W, int NV, bool RES, bool COL>
   int launch() const {
-    const unsigned blocks = (unsigned)ln_blocks(p.rows, p.d, kLnBwdWarps);
-    const size_t smem = W == 1 ? sizeof(float) * kLnRows * (size_t)p.d : 0;  // <= 32 KB
-    ln_bwd_kernel<T, VEC, W, NV, RES, COL><<<blocks, ln_threads<W>(), smem, st>>>(p);
+    const unsigned blocks = (unsigned)ln_blocks(p.rows, W, true);
+    const size_t smem = W == 1 ? sizeof(float) * kLnBwdRows * (size_t)p.d : 0;  // <= 48 KB
+    ln_bwd_kernel<T, VEC, W, NV, RES, COL><<<blocks, ln_threads(W, true), smem, st>>>(p);
     GPTB200_CHECK_LAUNCH();
     return 0;
   }
@@ -492,7 +509,10 @@ extern "C" int gptb200_layer_norm_fwd(const void* x, const void* scale, const vo
 
 extern "C" size_t gptb200_layer_norm_bwd_workspace_size(int64_t rows, int64_t d) {
   if (rows <= 0 || d <= 0 || d > kLnMaxWidth) return 0;
-  return (size_t)ln_blocks(rows, d, kLnBwdWarps) * 3 * (size_t)d * sizeof(float);
+  // for either access, which the pointers decide
+  const int64_t blocks = std::max(ln_blocks(rows, ln_warps(d, true), true),
+                                  ln_blocks(rows, ln_warps(d, false), true));
+  return (size_t)blocks * 3 * (size_t)d * sizeof(float);
 }
 
 extern "C" int gptb200_layer_norm_bwd(const void* x, const void* scale, const float* mean,
@@ -529,7 +549,8 @@ extern "C" int gptb200_layer_norm_bwd(const void* x, const void* scale, const fl
   const LnSums to = {{dscale, dbias, dx_colsum}, {1.f, 1.f, colsum_alpha}};
   const dim3 grid((unsigned)((d + 31) / 32), col ? 3 : 2);
   ln_sums_kernel<<<grid, dim3(32, 16), 0, st>>>(p.part,
-                                                (int)ln_blocks(rows, d, kLnBwdWarps), (int)d, to);
+                                                (int)ln_blocks(rows, ln_warps(d, vec), true),
+                                                (int)d, to);
   GPTB200_CHECK_LAUNCH();
   return 0;
 }

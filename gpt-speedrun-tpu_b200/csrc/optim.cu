@@ -9,6 +9,7 @@
 // The step counter lives on the device, so a captured CUDA graph of the whole
 // step replays correctly.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -353,31 +354,51 @@ __device__ __forceinline__ uint32_t mix32(uint32_t h) {
   h = (h ^ (h >> 13)) * 0xC2B2AE35u;
   return h ^ (h >> 16);
 }
-__device__ __forceinline__ uint32_t dither_bits(int64_t e, uint32_t key) {
-  return mix32((uint32_t)e * 0x9E3779B1u + (uint32_t)(e >> 32) * 0x85EBCA77u + key);
-}
+// 32 random bits of element e: mix32(e * 0x9E3779B1 + (e >> 32) * 0x85EBCA77 + key).
 
-// Magnitude of a code with M mantissa bits under block exponent E.
+// Magnitude of a code with M mantissa bits under block exponent E < 255, given
+// `bits`, the code shifted to the mantissa's top.
 template <int M>
-__device__ __forceinline__ float q8_decode(int code, int E) {
-  const float x = __int_as_float((code << (23 - M)) + ((E - 15) << 23));
-  return E == 255 ? __int_as_float(0x7fffffff) : code == 0 ? 0.f : x;
+__device__ __forceinline__ float q8_decode(uint32_t bits, int E) {
+  return bits == 0 ? 0.f : __uint_as_float(bits + ((uint32_t)(E - 15) << 23));
 }
 // Block exponent for a largest magnitude with these bits: the one above if the
 // top code would not reach it. At least 16, so that the smallest code is a
 // normal number.
 template <int M>
-__device__ __forceinline__ int q8_exponent(int top_bits) {
-  const int e = (top_bits + ((1 << (23 - M)) - 1)) >> 23;
+__device__ __forceinline__ int q8_exponent(uint32_t top_bits) {
+  const int e = (int)((top_bits + ((1u << (23 - M)) - 1u)) >> 23);
   return e >= 255 ? 255 : max(e, 16);
 }
+// Code of a magnitude's bits; at least `low`. Below 16 << M without a test, as
+// q8_exponent leaves room for any dither below a unit (and where it could not,
+// in a block with E = 255, codes do not matter).
 template <int M>
-__device__ __forceinline__ int q8_encode(int bits, int dither, int E, int low) {
-  const int c = (bits + dither - ((E - 15) << 23)) >> (23 - M);
-  return min(max(c, low), (16 << M) - 1);
+__device__ __forceinline__ uint32_t q8_encode(uint32_t bits, uint32_t dither, int E, int low) {
+  return (uint32_t)max((int)(bits + dither - ((uint32_t)(E - 15) << 23)) >> (23 - M), low);
+}
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t bytes4(const uint32_t* c) {
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 }
 
-__global__ void __launch_bounds__(256) adamw8_kernel(
+// Eight lanes share a block, eight elements each: what a lane does once (group
+// lookup, addresses, exponents, shuffles) is spread over eight updates, since
+// the arithmetic, about 70 instructions an element, already fills two thirds of
+// the issue slots that the memory traffic leaves. The quotient m / r is the only
+// operation that is not rounded to nearest (its error, 2^-22 of the update, is
+// far below half a unit of the parameter).
+constexpr int kQLane = 8;
+
+// The group whose elements a lane's quad belongs to, and its multipliers.
+struct QuadGroup {
+  int64_t lo, hi;  // elements [lo, hi)
+  float lr, eps, wd;
+};
+
+// Four blocks of 256 threads on an SM (64 registers), measured against 3 and 5 at
+// 124.7 M parameters: 531, 545 and 566 us.
+__global__ void __launch_bounds__(256, 4) adamw8_kernel(
     float* __restrict__ p, uint8_t* __restrict__ mq, uint8_t* __restrict__ me,
     uint8_t* __restrict__ vq, uint8_t* __restrict__ ve, const float* __restrict__ g, int64_t begin,
     int64_t end, const gptb200_tensor_group* __restrict__ groups, int ngroups,
@@ -394,101 +415,161 @@ __global__ void __launch_bounds__(256) adamw8_kernel(
   const float inv1 = 1.0f / s.bc1, inv2 = 1.0f / sqrtf(s.bc2);
   double acc = 0.0;
   float accf = 0.f;
-  int cnt = 0, gi = 0;
-  // Sixteen lanes share a block, four elements each.
-  const int64_t stride = (int64_t)gridDim.x * blockDim.x * 4;
-  const int64_t stop = (end + kQBlock - 1) / kQBlock * kQBlock;  // whole blocks: shuffles below
-  for (int64_t e0 = begin + ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 4;
-       e0 - 4 * (threadIdx.x & 31) < stop; e0 += stride) {
-    const bool in = e0 < end;
-    gi = in ? find_group(sg, ngroups, gi, e0) : -1;
-    const bool live = gi >= 0;  // else padding between tensors, or past the end
-    const gptb200_tensor_group& G = sg[live ? gi : 0];
-    const int n = live ? (int)min((int64_t)4, min(end, G.offset + G.size) - e0) : 0;
-    float P[4] = {0.f, 0.f, 0.f, 0.f}, Gr[4] = {0.f, 0.f, 0.f, 0.f};
-    uint32_t mc = 0, vc = 0;
+  int cnt = 0;
+  QuadGroup q = {0, 0, 0.f, 0.f, 0.f};  // of the last element looked up
+  int gi = 0;
+  auto look_up = [&](int64_t e) {  // the elements of q from e on, at most 4
+    if (e < q.lo || e >= q.hi) {
+      gi = e < end ? find_group(sg, ngroups, gi, e) : -1;
+      if (gi < 0) {  // padding between tensors, or past the end
+        gi = 0;
+        return 0;
+      }
+      const gptb200_tensor_group& G = sg[gi];
+      q.lo = G.offset;
+      q.hi = min(end, G.offset + G.size);
+      q.lr = s.lr * G.lr_mult;
+      q.eps = cfg.eps * cfg.eps_horizon_scale * G.eps_mult;
+      q.wd = G.decay ? cfg.weight_decay * cfg.wd_horizon_scale * G.wd_mult : 0.f;
+    }
+    return (int)min((int64_t)4, q.hi - e);
+  };
+  // Elements e0..e0 + 7, of which n0 of the first four and n1 of the others are live.
+  auto update = [&](int64_t e0, int n0, int n1, const QuadGroup& ga, const QuadGroup& gb,
+                    auto whole) {
+    const bool all = decltype(whole)::value || n0 + n1 == 8;
+    const bool any = decltype(whole)::value || n0 + n1 > 0;
+    float P[8], Gr[8];
+    uint32_t mc[2] = {0, 0}, vc[2] = {0, 0};
     int em = 16, ev = 16;
-    if (n == 4) {
-      const float4 a = *reinterpret_cast<const float4*>(p + e0);
-      const float4 b = __ldcs(reinterpret_cast<const float4*>(g + e0));
-      P[0] = a.x, P[1] = a.y, P[2] = a.z, P[3] = a.w;
-      Gr[0] = b.x, Gr[1] = b.y, Gr[2] = b.z, Gr[3] = b.w;
+    if (all) {
+      const float4 a0 = *reinterpret_cast<const float4*>(p + e0);
+      const float4 a1 = *reinterpret_cast<const float4*>(p + e0 + 4);
+      const float4 g0 = *reinterpret_cast<const float4*>(g + e0);
+      const float4 g1 = *reinterpret_cast<const float4*>(g + e0 + 4);
+      P[0] = a0.x, P[1] = a0.y, P[2] = a0.z, P[3] = a0.w;
+      P[4] = a1.x, P[5] = a1.y, P[6] = a1.z, P[7] = a1.w;
+      Gr[0] = g0.x, Gr[1] = g0.y, Gr[2] = g0.z, Gr[3] = g0.w;
+      Gr[4] = g1.x, Gr[5] = g1.y, Gr[6] = g1.z, Gr[7] = g1.w;
     } else {
-      for (int j = 0; j < n; ++j) {
-        P[j] = p[e0 + j];
-        Gr[j] = g[e0 + j];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool in = (j & 3) < (j < 4 ? n0 : n1);
+        P[j] = in ? p[e0 + j] : 0.f;
+        Gr[j] = in ? g[e0 + j] : 0.f;
       }
     }
-    if (live) {
-      mc = *reinterpret_cast<const uint32_t*>(mq + e0);
-      vc = *reinterpret_cast<const uint32_t*>(vq + e0);
+    if (any) {
+      const uint2 a = *reinterpret_cast<const uint2*>(mq + e0);
+      const uint2 b = *reinterpret_cast<const uint2*>(vq + e0);
+      mc[0] = a.x, mc[1] = a.y, vc[0] = b.x, vc[1] = b.y;
       em = me[e0 / kQBlock];
       ev = ve[e0 / kQBlock];
     }
-    const float lr = s.lr * G.lr_mult;
-    const float eps = cfg.eps * cfg.eps_horizon_scale * G.eps_mult;
-    const float wd = G.decay ? cfg.weight_decay * cfg.wd_horizon_scale * G.wd_mult : 0.f;
-    float M[4], R[4];
-    int mtop = 0, vtop = 0;
+    // a block that held a NaN or an infinity stays NaN
+    const float b1n = em == 255 ? __int_as_float(0x7fffffff) : b1;
+    const float b2n = ev == 255 ? __int_as_float(0x7fffffff) : b2;
+    em = min(em, 254);
+    ev = min(ev, 254);
+    float M[8], R[8];
+    uint32_t mtop = 0, vtop = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 8; ++j) {
+      const int w = j >> 2, sh = 8 * (j & 3);
       accf += Gr[j] * Gr[j];
       const float gr = __fmul_rn(Gr[j], s.gscale);
-      const int c = (mc >> (8 * j)) & 255;
-      const float mag = q8_decode<3>(c & 127, em);
-      const float r = q8_decode<4>((vc >> (8 * j)) & 255, ev);
-      M[j] = __fadd_rn(__fmul_rn(b1, c & 128 ? -mag : mag), __fmul_rn(omb1, gr));
+      // code (and its sign) to the top of the mantissa
+      const uint32_t mb = sh < 20 ? mc[w] << (20 - sh) : mc[w] >> (sh - 20);
+      const uint32_t vb = sh < 19 ? vc[w] << (19 - sh) : vc[w] >> (sh - 19);
+      const float mag = q8_decode<3>(mb & 0x07f00000u, em);
+      const float r = q8_decode<4>(vb & 0x07f80000u, ev);
+      const float m0 = __uint_as_float(__float_as_uint(mag) ^ (mb << 4 & 0x80000000u));
+      M[j] = __fadd_rn(__fmul_rn(b1n, m0), __fmul_rn(omb1, gr));
       R[j] = __fsqrt_rn(
-          __fadd_rn(__fmul_rn(b2, __fmul_rn(r, r)), __fmul_rn(omb2, __fmul_rn(gr, gr))));
-      if (j >= n) M[j] = R[j] = 0.f;
-      mtop = max(mtop, __float_as_int(fabsf(M[j])));
-      vtop = max(vtop, __float_as_int(fabsf(R[j])));
-      const float adam = (M[j] * inv1) / (R[j] * inv2 + eps);
-      P[j] = P[j] - lr * (adam + wd * P[j]);
+          __fadd_rn(__fmul_rn(b2n, __fmul_rn(r, r)), __fmul_rn(omb2, __fmul_rn(gr, gr))));
+      if (!all && (j & 3) >= (j < 4 ? n0 : n1)) M[j] = R[j] = 0.f;
+      mtop = max(mtop, __float_as_uint(M[j]) & 0x7fffffffu);
+      vtop = max(vtop, __float_as_uint(R[j]));  // >= 0 or NaN
+      const QuadGroup& G = j < 4 ? ga : gb;
+      const float adam = __fdividef(M[j] * inv1, R[j] * inv2 + G.eps);
+      P[j] = P[j] - G.lr * (adam + G.wd * P[j]);
     }
-    if (n == 4) {
+    if (all) {
       *reinterpret_cast<float4*>(p + e0) = make_float4(P[0], P[1], P[2], P[3]);
-      if (pbf)
+      *reinterpret_cast<float4*>(p + e0 + 4) = make_float4(P[4], P[5], P[6], P[7]);
+      if (pbf) {
         *reinterpret_cast<uint2*>(pbf + e0) =
             make_uint2(pack_bf16x2(P[0], P[1]), pack_bf16x2(P[2], P[3]));
+        *reinterpret_cast<uint2*>(pbf + e0 + 4) =
+            make_uint2(pack_bf16x2(P[4], P[5]), pack_bf16x2(P[6], P[7]));
+      }
     } else {
-      for (int j = 0; j < n; ++j) {
-        p[e0 + j] = P[j];
-        if (pbf) pbf[e0 + j] = __float2bfloat16(P[j]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if ((j & 3) < (j < 4 ? n0 : n1)) {
+          p[e0 + j] = P[j];
+          if (pbf) pbf[e0 + j] = __float2bfloat16(P[j]);
+        }
       }
     }
-    // the block's exponents: the 16 lanes' largest magnitudes (as integers, so
+    // the block's exponents: the eight lanes' largest magnitudes (as integers, so
     // that a NaN or an infinity is larger than every number)
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
+    for (int o = 4; o > 0; o >>= 1) {
       mtop = max(mtop, __shfl_xor_sync(0xffffffffu, mtop, o));
       vtop = max(vtop, __shfl_xor_sync(0xffffffffu, vtop, o));
     }
     em = q8_exponent<3>(mtop);
     ev = q8_exponent<4>(vtop);
-    mc = vc = 0;
+    const uint32_t h0 =
+        (uint32_t)e0 * 0x9E3779B1u + (uint32_t)(e0 >> 32) * 0x85EBCA77u + key;  // e0 + j: no carry
+    uint32_t bm[8], bv[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t h = dither_bits(e0 + j, key);
-      const int mb = __float_as_int(M[j]), rb = __float_as_int(R[j]) & 0x7fffffff;
-      int cm = q8_encode<3>(mb & 0x7fffffff, (h >> 16) << 4, em, 0);
-      const int cv = q8_encode<4>(rb, (h & 0xffff) << 3, ev, rb != 0);
-      if (mb < 0 && cm) cm |= 128;
-      mc |= (uint32_t)cm << (8 * j);
-      vc |= (uint32_t)cv << (8 * j);
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t h = mix32(h0 + (uint32_t)j * 0x9E3779B1u);
+      const uint32_t mb = __float_as_uint(M[j]), rb = __float_as_uint(R[j]);
+      const uint32_t c = q8_encode<3>(mb & 0x7fffffffu, h >> 12 & 0xffff0u, em, 0);
+      bm[j] = c | ((c + 127u) & (mb >> 24) & 0x80u);  // the sign of a code that is not 0
+      bv[j] = q8_encode<4>(rb, h << 3 & 0x7fff8u, ev, (int)min(rb, 1u));
     }
-    if (live) {
-      *reinterpret_cast<uint32_t*>(mq + e0) = mc;
-      *reinterpret_cast<uint32_t*>(vq + e0) = vc;
+    const uint32_t cm[2] = {bytes4(bm), bytes4(bm + 4)}, cv[2] = {bytes4(bv), bytes4(bv + 4)};
+    // Codes are written wherever an element of the quad is live; dead quads of a
+    // live block belong to no tensor and stay as they are.
+    if (all) {
+      *reinterpret_cast<uint2*>(mq + e0) = make_uint2(cm[0], cm[1]);
+      *reinterpret_cast<uint2*>(vq + e0) = make_uint2(cv[0], cv[1]);
+    } else {
+      if (n0) {
+        *reinterpret_cast<uint32_t*>(mq + e0) = cm[0];
+        *reinterpret_cast<uint32_t*>(vq + e0) = cv[0];
+      }
+      if (n1) {
+        *reinterpret_cast<uint32_t*>(mq + e0 + 4) = cm[1];
+        *reinterpret_cast<uint32_t*>(vq + e0 + 4) = cv[1];
+      }
     }
     // one lane of each block writes its exponents: the first that holds a tensor's element
-    const unsigned any = __ballot_sync(0xffffffffu, live) >> (threadIdx.x & 16) & 0xffff;
-    if (live && (threadIdx.x & 15) == __ffs(any) - 1) {
+    const unsigned holds = __ballot_sync(0xffffffffu, any) >> (threadIdx.x & 24) & 0xff;
+    if (any && (threadIdx.x & 7) == __ffs(holds) - 1) {
       me[e0 / kQBlock] = (uint8_t)em;
       ve[e0 / kQBlock] = (uint8_t)ev;
     }
-    if (gi < 0) gi = 0;
-    if (++cnt == 16) {
+  };
+  const int64_t stride = (int64_t)gridDim.x * blockDim.x * kQLane;
+  const int64_t stop = (end + kQBlock - 1) / kQBlock * kQBlock;  // whole blocks: shuffles below
+  for (int64_t e0 = begin + ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * kQLane;
+       e0 - kQLane * (threadIdx.x & 31) < stop; e0 += stride) {
+    // One group holds all eight elements of every lane, mostly: then without the
+    // tests that a tensor's end needs (issued, predicated off, in every pass).
+    if (__all_sync(0xffffffffu, e0 >= q.lo && e0 + kQLane <= q.hi))
+      update(e0, 4, 4, q, q, std::true_type());
+    else {
+      const int n0 = look_up(e0);
+      const QuadGroup qa = q;
+      const int n1 = look_up(e0 + 4);
+      update(e0, n0, n1, qa, q, std::false_type());
+    }
+    if (++cnt == 8) {
       acc += accf;
       accf = 0.f;
       cnt = 0;
@@ -504,6 +585,7 @@ __global__ void __launch_bounds__(256) adamw8_kernel(
     double t = 0.0;
     for (int w = 0; w < 8; ++w) t += red[w];
     part[blockIdx.x] = t;
+    for (int b = blockIdx.x + gridDim.x; b < kRangeBlocks; b += gridDim.x) part[b] = 0.0;
   }
 }
 
@@ -517,13 +599,20 @@ __global__ void __launch_bounds__(256) adamw8_values_kernel(
     const uint2 mc = *reinterpret_cast<const uint2*>(mq + e);
     const uint2 vc = *reinterpret_cast<const uint2*>(vq + e);
     const int em = me[e / kQBlock], ev = ve[e / kQBlock];
+    // NaN blocks: one factor for the whole lane
+    const float fm = em == 255 ? __int_as_float(0x7fffffff) : 1.f;
+    const float fv = ev == 255 ? __int_as_float(0x7fffffff) : 1.f;
+    const int emc = min(em, 254), evc = min(ev, 254);
     float a[8], b[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int c = ((j < 4 ? mc.x : mc.y) >> (8 * (j & 3))) & 255;
-      const float mag = q8_decode<3>(c & 127, em);
-      a[j] = c & 128 ? -mag : mag;
-      b[j] = q8_decode<4>(((j < 4 ? vc.x : vc.y) >> (8 * (j & 3))) & 255, ev);
+      const int sh = 8 * (j & 3);
+      const uint32_t mw = j < 4 ? mc.x : mc.y, vw = j < 4 ? vc.x : vc.y;
+      const uint32_t mb = sh < 20 ? mw << (20 - sh) : mw >> (sh - 20);
+      const uint32_t vb = sh < 19 ? vw << (19 - sh) : vw >> (sh - 19);
+      const float mag = q8_decode<3>(mb & 0x07f00000u, emc);
+      a[j] = fm * __uint_as_float(__float_as_uint(mag) ^ (mb << 4 & 0x80000000u));
+      b[j] = fv * q8_decode<4>(vb & 0x07f80000u, evc);
     }
     *reinterpret_cast<uint4*>(m + e) = make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]),
                                                   pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
@@ -678,7 +767,9 @@ static int adamw8_launch(float* params, const gptb200_adamw8_state& q, const flo
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return -static_cast<int>(e);
   }
-  adamw8_kernel<<<kRangeBlocks, 256, smem, st>>>(
+  const int64_t wanted = (end - begin + 256 * kQLane - 1) / (256 * kQLane);
+  const int blocks = (int)std::min<int64_t>(wanted, kRangeBlocks);
+  adamw8_kernel<<<blocks, 256, smem, st>>>(
       params, q.m, q.m_exp, q.v, q.v_exp, grads, begin, end, groups, n_groups, cfg, sc, seed,
       reinterpret_cast<bf16*>(params_bf16), part);
   GPTB200_CHECK_LAUNCH();

@@ -269,6 +269,7 @@ def check(status: int, what: str) -> None:
 def call(name: str, *args) -> int:
     """Calls an entry point and raises GptB200Error on a non-zero status."""
 
-    status = getattr(load(), name)(*args)
-    check(status, name)
+    status = getattr(_lib or load(), name)(*args)
+    if status:
+        check(status, name)
     return status

@@ -23,8 +23,12 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # (device index) -> cudaStream_t, without a Stream object
+_device = torch._C._cuda_getDevice
+
+
 def _stream() -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return ctypes.c_void_p(_raw_stream(_device()))
 
 
 def _cuda(*ts: torch.Tensor | None) -> None:
@@ -211,31 +215,39 @@ def rms_norm_bwd(x, scale, rstd, dy, dx_in, dx_out, dscale, dx_colsum=None, cols
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
 
 
-def _norm_args(x, vectors: dict, rows: dict, stats: dict) -> int:
-    """Checks layer norm's tensors against x [rows, d]; returns x's dtype code."""
+def _bad(name: str, t: torch.Tensor, dtype, shape) -> None:
+    raise ValueError(f"{name} must be a CUDA tensor of {dtype} {tuple(shape)} with unit inner stride, got "
+                     f"{t.device} {t.dtype} {tuple(t.shape)} {tuple(t.stride())}")
 
-    if x.dtype not in _DTYPES:
+
+def _rows(name: str, t: torch.Tensor, shape, dtype) -> int:
+    """Checks a [rows, d] argument; returns its row stride in elements (a single
+    row may carry any)."""
+
+    s0, s1 = t.stride() if t.dim() == 2 else (0, 0)
+    n, d = shape
+    if not t.is_cuda or t.dtype is not dtype or t.shape != shape or (s1 != 1 and d > 1):
+        _bad(name, t, dtype, shape)
+    return s0 if n > 1 else d
+
+
+def _vector(name: str, t: torch.Tensor, size: int, dtype) -> int:
+    """Checks a contiguous vector argument; returns its address."""
+
+    if not t.is_cuda or t.dtype is not dtype or t.shape != (size,) or (size > 1 and t.stride(0) != 1):
+        _bad(name, t, dtype, (size,))
+    return t.data_ptr()
+
+
+def _norm_rows(x: torch.Tensor):
+    """(dtype code, shape, row stride) of layer norm's input."""
+
+    code = _DTYPES.get(x.dtype)
+    if code is None:
         raise TypeError(f"layer norm takes bfloat16 or float32 rows, got {x.dtype}")
     if x.dim() != 2:
         raise ValueError(f"layer norm takes 2-D rows, got {tuple(x.shape)}")
-    n, d = x.shape
-    wanted = [(vectors, (d,), x.dtype), (rows, (n, d), x.dtype), (stats, None, F32)]
-    for tensors, shape, dtype in wanted:
-        for name, t in tensors.items():
-            if t is None:
-                continue
-            want = shape if shape is not None else ((n,) if name in ("mean", "rstd") else (d,))
-            if tuple(t.shape) != want or t.dtype != dtype:
-                raise ValueError(f"{name} must be {dtype} {want}, got {t.dtype} {tuple(t.shape)}")
-            if (t.dim() == 1 and not t.is_contiguous()) or (t.dim() == 2 and t.stride(1) != 1 and d > 1):
-                raise ValueError(f"{name} must have unit inner stride, got {tuple(t.stride())}")
-    return _DTYPES[x.dtype]
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    """Row stride in elements (a single row may carry any stride)."""
-
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+    return code, x.shape, _rows("x", x, x.shape, x.dtype)
 
 
 def layer_norm_fwd(x, scale, bias, y, mean, rstd, eps: float = 1e-5):
@@ -243,11 +255,13 @@ def layer_norm_fwd(x, scale, bias, y, mean, rstd, eps: float = 1e-5):
     any row stride); mean and rstd (fp32 [rows]) are written for the backward.
     bias may be None. y may be x."""
 
-    _cuda(x, scale, bias, y, mean, rstd)
-    code = _norm_args(x, dict(scale=scale, bias=bias), dict(x=x, y=y), dict(mean=mean, rstd=rstd))
-    call("gptb200_layer_norm_fwd", x.data_ptr(), scale.data_ptr(), _ptr(bias), y.data_ptr(),
-         mean.data_ptr(), rstd.data_ptr(), x.shape[0], x.shape[1], _row_stride(x), _row_stride(y),
-         float(eps), code, _stream())
+    code, shape, ldx = _norm_rows(x)
+    n, d = shape
+    ldy = _rows("y", y, shape, x.dtype)
+    call("gptb200_layer_norm_fwd", x.data_ptr(), _vector("scale", scale, d, x.dtype),
+         None if bias is None else _vector("bias", bias, d, x.dtype), y.data_ptr(),
+         _vector("mean", mean, n, F32), _vector("rstd", rstd, n, F32), n, d, ldx, ldy, eps, code,
+         _stream())
     return y, mean, rstd
 
 
@@ -260,21 +274,23 @@ def layer_norm_bwd(x, scale, mean, rstd, dy, dx_in, dx_out, dscale, dbias=None, 
     """dx_out = dx_in + d(layer_norm)/dx . dy; dscale +=; dbias +=; dx_colsum +=
     alpha * colsum(dx_out). dx_in, dbias and dx_colsum may be None."""
 
-    _cuda(x, scale, mean, rstd, dy, dx_in, dx_out, dscale, dbias, dx_colsum, workspace)
-    code = _norm_args(x, dict(scale=scale), dict(x=x, dy=dy, dx_in=dx_in, dx_out=dx_out),
-                      dict(mean=mean, rstd=rstd, dscale=dscale, dbias=dbias, dx_colsum=dx_colsum))
-    rows, d = x.shape
-    if dx_in is not None and _row_stride(dx_in) != _row_stride(dx_out):
+    code, shape, ldx = _norm_rows(x)
+    n, d = shape
+    ldy = _rows("dy", dy, shape, x.dtype)
+    ldd = _rows("dx_out", dx_out, shape, x.dtype)
+    if dx_in is not None and _rows("dx_in", dx_in, shape, x.dtype) != ldd:
         raise ValueError("dx_in and dx_out must share strides")
-    size = layer_norm_bwd_workspace_size(rows, d)
+    size = layer_norm_bwd_workspace_size(n, d)
     if workspace is None:
         workspace = _scratch(size, x.device)
-    elif workspace.numel() * workspace.element_size() < size:
-        raise ValueError(f"the workspace needs {size} bytes")
-    call("gptb200_layer_norm_bwd", x.data_ptr(), scale.data_ptr(), mean.data_ptr(),
-         rstd.data_ptr(), dy.data_ptr(), _ptr(dx_in), dx_out.data_ptr(), dscale.data_ptr(),
-         _ptr(dbias), _ptr(dx_colsum), float(colsum_alpha), rows, d, _row_stride(x),
-         _row_stride(dy), _row_stride(dx_out), code, _ptr(workspace), _stream())
+    elif not workspace.is_cuda or workspace.numel() * workspace.element_size() < size:
+        raise ValueError(f"the workspace needs {size} bytes on the device")
+    call("gptb200_layer_norm_bwd", x.data_ptr(), _vector("scale", scale, d, x.dtype),
+         _vector("mean", mean, n, F32), _vector("rstd", rstd, n, F32), dy.data_ptr(), _ptr(dx_in),
+         dx_out.data_ptr(), _vector("dscale", dscale, d, F32),
+         None if dbias is None else _vector("dbias", dbias, d, F32),
+         None if dx_colsum is None else _vector("dx_colsum", dx_colsum, d, F32), colsum_alpha, n, d,
+         ldx, ldy, ldd, code, _ptr(workspace), _stream())
     return dx_out
 
 
@@ -400,54 +416,67 @@ def attention_bwd(q, k, v, o, do, lse, dq, dk, dv, *, scale: float, layout="bhsd
     return dq, dk, dv
 
 
-def _tma_strides(t: torch.Tensor, layout: str) -> tuple[int, int, int]:
-    """`_strides4` with the strides of length-1 dimensions, which nothing uses,
-    replaced by one that a tensor map accepts."""
+_I3 = ctypes.c_int64 * 3
 
-    sizes = t.shape[:3] if layout == "bhsd" else (t.shape[0], t.shape[2], t.shape[1])
-    return tuple(s if n > 1 else t.shape[3] for s, n in zip(_strides4(t, layout), sizes))
+
+def _view4(name: str, t: torch.Tensor, b: int, h: int, n: int, d: int, bthd: bool) -> _I3:
+    """Checks a bf16 attention argument of b batches, h heads, n positions; returns
+    its element strides (batch, head, time). The stride of a length-1 dimension,
+    which nothing uses, becomes one that a tensor map accepts."""
+
+    shape = (b, n, h, d) if bthd else (b, h, n, d)
+    if t.shape != shape or t.dtype is not BF16 or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA bfloat16 tensor {shape}, got {t.device} {t.dtype} "
+                         f"{tuple(t.shape)}")
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1:
+        raise ValueError("attention tensors need a contiguous head dimension")
+    if bthd:
+        s1, s2 = s2, s1
+    return _I3(s0 if b > 1 else d, s1 if h > 1 else d, s2 if n > 1 else d)
+
+
+def _same(x: _I3, y: _I3, what: str) -> _I3:
+    if x[0] != y[0] or x[1] != y[1] or x[2] != y[2]:
+        raise ValueError(f"{what} must share strides")
+    return x
+
+
+def _flat(name: str, t: torch.Tensor | None, shape, dtype) -> int | None:
+    """Checks an optional contiguous argument; returns its address."""
+
+    if t is None:
+        return None
+    if not t.is_cuda or t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous CUDA tensor of {dtype} {tuple(shape)}, got "
+                         f"{t.device} {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
 
 
 def _score_call(q, k, v, o, lse, scale, layout, softcap, slopes, segment_ids, prefix_lens):
-    """Checks a score-modified attention call; returns (struct, b, h, kv heads, t)."""
+    """Checks a score-modified attention call; returns (struct, b, h, kv heads, t, d)."""
 
-    _cuda(q, k, v, o, lse, slopes, segment_ids, prefix_lens)
-    if layout not in ("bhsd", "bthd"):
+    bthd = layout == "bthd"
+    if not bthd and layout != "bhsd":
         raise ValueError(f"unknown attention layout {layout!r}")
-    for name, t_ in (("q", q), ("k", k), ("v", v), ("o", o)):
-        if t_.dim() != 4 or t_.dtype != BF16:
-            raise ValueError(f"{name} must be a rank-4 bfloat16 view, got {t_.dtype} {tuple(t_.shape)}")
-    b, t, h, d = q.shape if layout == "bthd" else (q.shape[0], q.shape[2], q.shape[1], q.shape[3])
-    kv = k.shape[2 if layout == "bthd" else 1]
-    want = (b, t, kv, d) if layout == "bthd" else (b, kv, t, d)
-    if o.shape != q.shape or tuple(k.shape) != want or tuple(v.shape) != want:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} and o "
-                         f"{tuple(o.shape)} do not match")
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError(f"q and k must be rank-4 views, got {tuple(q.shape)}, {tuple(k.shape)}")
+    if bthd:
+        b, t, h, d = q.shape
+        kv = k.shape[2]
+    else:
+        b, h, t, d = q.shape
+        kv = k.shape[1]
     if kv == 0 or h % kv:
         raise ValueError(f"{h} query heads cannot share {kv} key/value heads")
-    kvs = _tma_strides(k, layout)
-    if _tma_strides(v, layout) != kvs:
-        raise ValueError("k and v must share strides")
-    if lse.dtype != F32 or lse.numel() != b * h * t or not lse.is_contiguous():
-        raise ValueError(f"lse must be contiguous float32 [{b}, {h}, {t}]")
-    if slopes is not None and (slopes.dtype != F32 or tuple(slopes.shape) != (h,)
-                               or not slopes.is_contiguous()):
-        raise ValueError(f"slopes must be contiguous float32 [{h}], got {slopes.dtype} "
-                         f"{tuple(slopes.shape)}")
-    if prefix_lens is not None and (prefix_lens.dtype != torch.int32
-                                    or tuple(prefix_lens.shape) != (b,)
-                                    or not prefix_lens.is_contiguous()):
-        raise ValueError(f"prefix_lens must be contiguous int32 [{b}], got {prefix_lens.dtype} "
-                         f"{tuple(prefix_lens.shape)}")
-    if segment_ids is not None and not segment_ids.is_contiguous():
-        raise ValueError("segment_ids must be contiguous")
-    _segments(segment_ids, b, t)
-    s3 = ctypes.c_int64 * 3
+    kvs = _same(_view4("k", k, b, kv, t, d, bthd), _view4("v", v, b, kv, t, d, bthd), "k and v")
     c = _lib.ScoreAttention(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), s3(*_tma_strides(q, layout)), s3(*kvs), o.data_ptr(),
-        s3(*_tma_strides(o, layout)), lse.data_ptr(), b, h, kv, t, d, float(scale), float(softcap),
-        _ptr(slopes), _ptr(segment_ids), _ptr(prefix_lens))
-    return c, b, h, kv, t
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _view4("q", q, b, h, t, d, bthd), kvs, o.data_ptr(),
+        _view4("o", o, b, h, t, d, bthd), _flat("lse", lse, (b, h, t), F32), b, h, kv, t, d, scale,
+        softcap, _flat("slopes", slopes, (h,), F32),
+        _flat("segment_ids", segment_ids, (b, t), torch.int32),
+        _flat("prefix_lens", prefix_lens, (b,), torch.int32))
+    return c, b, h, kv, t, d
 
 
 def score_attention_fwd(q, k, v, o, lse, *, scale: float, layout: str = "bhsd",
@@ -462,7 +491,7 @@ def score_attention_fwd(q, k, v, o, lse, *, scale: float, layout: str = "bhsd",
     """
 
     c, *_ = _score_call(q, k, v, o, lse, scale, layout, softcap, slopes, segment_ids, prefix_lens)
-    call("gptb200_score_attention_fwd", ctypes.byref(c), _stream())
+    call("gptb200_score_attention_fwd", c, _stream())
     return o, lse
 
 
@@ -476,24 +505,18 @@ def score_attention_bwd(q, k, v, o, do, lse, dq, dk, dv, *, scale: float, layout
     """Gradients of `score_attention_fwd` (its o and lse); dk and dv sum over the
     query heads that share them. With `rope` dq and dk are rotated back."""
 
-    c, b, h, _, t = _score_call(q, k, v, o, lse, scale, layout, softcap, slopes, segment_ids,
-                                prefix_lens)
-    _cuda(do, dq, dk, dv, workspace)
-    for name, g, x in (("do", do, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-        if g.shape != x.shape or g.dtype != BF16:
-            raise ValueError(f"{name} must be bfloat16 {tuple(x.shape)}, got {g.dtype} {tuple(g.shape)}")
-    dkvs = _tma_strides(dk, layout)
-    if _tma_strides(dv, layout) != dkvs:
-        raise ValueError("dk and dv must share strides")
+    c, b, h, kv, t, d = _score_call(q, k, v, o, lse, scale, layout, softcap, slopes, segment_ids,
+                                    prefix_lens)
+    bthd = layout == "bthd"
+    dkvs = _same(_view4("dk", dk, b, kv, t, d, bthd), _view4("dv", dv, b, kv, t, d, bthd), "dk and dv")
     size = score_attention_workspace_size(b, h, t)
     if workspace is None:
         workspace = _scratch(size, q.device)
-    elif workspace.numel() * workspace.element_size() < size:
-        raise ValueError(f"the workspace needs {size} bytes")
-    s3 = ctypes.c_int64 * 3
+    elif not workspace.is_cuda or workspace.numel() * workspace.element_size() < size:
+        raise ValueError(f"the workspace needs {size} bytes on the device")
     cos, sin = rope if rope is not None else (None, None)
-    call("gptb200_score_attention_bwd", ctypes.byref(c), do.data_ptr(), s3(*_tma_strides(do, layout)),
-         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), s3(*_tma_strides(dq, layout)), s3(*dkvs),
+    call("gptb200_score_attention_bwd", c, do.data_ptr(), _view4("do", do, b, h, t, d, bthd),
+         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _view4("dq", dq, b, h, t, d, bthd), dkvs,
          _ptr(cos), _ptr(sin), _ptr(workspace), _stream())
     return dq, dk, dv
 
@@ -615,19 +638,25 @@ def adamw8_state(n: int, device) -> tuple[torch.Tensor, torch.Tensor, torch.Tens
                  for k in (blocks * ADAMW8_BLOCK, blocks) * 2)
 
 
-def _adamw8(state, n: int, floats: dict) -> _lib.AdamW8State:
-    """Checks a state and the flat buffers that go with it."""
+def _adamw8(state, n: int) -> _lib.AdamW8State:
+    """Checks a state of n elements."""
 
-    _cuda(*state, *(t for t, _ in floats.values()))
+    m, me, v, ve = state
     blocks = (n + ADAMW8_BLOCK - 1) // ADAMW8_BLOCK
-    for t, size in zip(state, (blocks * ADAMW8_BLOCK, blocks) * 2, strict=True):
-        if t.dtype != torch.uint8 or t.numel() < size or not t.is_contiguous():
-            raise ValueError(f"an 8-bit state of {n} elements is contiguous uint8 arrays of "
+    for t, size in ((m, blocks * ADAMW8_BLOCK), (me, blocks), (v, blocks * ADAMW8_BLOCK), (ve, blocks)):
+        if not t.is_cuda or t.dtype is not torch.uint8 or t.numel() < size or not t.is_contiguous():
+            raise ValueError(f"an 8-bit state of {n} elements is contiguous uint8 CUDA arrays of "
                              f"{blocks * ADAMW8_BLOCK} codes and {blocks} exponents")
-    for name, (t, dtype) in floats.items():
-        if t is not None and (t.dtype != dtype or t.numel() != n or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous {dtype} of {n} elements")
-    return _lib.AdamW8State(*(t.data_ptr() for t in state))
+    return _lib.AdamW8State(m.data_ptr(), me.data_ptr(), v.data_ptr(), ve.data_ptr())
+
+
+def _adamw8_flat(name: str, t: torch.Tensor | None, n: int, dtype) -> int | None:
+    if t is None:
+        return None
+    if not t.is_cuda or t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous CUDA tensor of {n} {dtype} elements, got "
+                         f"{t.device} {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
 
 
 def adamw8_step(params, state, grads, groups_dev, n_groups, cfg, step, loss, history, params_bf16,
@@ -638,12 +667,12 @@ def adamw8_step(params, state, grads, groups_dev, n_groups, cfg, step, loss, his
     inputs give the same codes. workspace: `adamw_workspace`."""
 
     _cuda(groups_dev, step, loss, history, workspace)
-    q = _adamw8(state, params.numel(), dict(params=(params, F32), grads=(grads, F32),
-                                            params_bf16=(params_bf16, BF16)))
-    call("gptb200_adamw8_step", params.data_ptr(), ctypes.byref(q), grads.data_ptr(),
-         params.numel(), groups_dev.data_ptr(), n_groups, ctypes.byref(cfg), step.data_ptr(),
-         _ptr(loss), _ptr(history), _ptr(params_bf16), int(seed) & 0xFFFFFFFF,
-         workspace.data_ptr(), _stream())
+    n = params.numel()
+    q = _adamw8(state, n)
+    call("gptb200_adamw8_step", _adamw8_flat("params", params, n, F32), q,
+         _adamw8_flat("grads", grads, n, F32), n, groups_dev.data_ptr(), n_groups, cfg,
+         step.data_ptr(), _ptr(loss), _ptr(history), _adamw8_flat("params_bf16", params_bf16, n, BF16),
+         seed & 0xFFFFFFFF, workspace.data_ptr(), _stream())
 
 
 def adamw8_update_range(params, state, grads, begin, end, groups_dev, n_groups, cfg, slot,
@@ -651,23 +680,24 @@ def adamw8_update_range(params, state, grads, begin, end, groups_dev, n_groups, 
     """`adamw_update_range` with 8-bit moments; begin and end are multiples of 64."""
 
     _cuda(groups_dev, workspace)
-    q = _adamw8(state, params.numel(), dict(params=(params, F32), grads=(grads, F32),
-                                            params_bf16=(params_bf16, BF16)))
+    n = params.numel()
+    q = _adamw8(state, n)
     if not 0 <= begin < end <= state[0].numel():
         raise ValueError(f"[{begin}, {end}) is outside the {state[0].numel()} elements")
-    call("gptb200_adamw8_update_range", params.data_ptr(), ctypes.byref(q), grads.data_ptr(),
-         int(begin), int(end), groups_dev.data_ptr(), n_groups, ctypes.byref(cfg), int(slot),
-         _ptr(params_bf16), int(seed) & 0xFFFFFFFF, workspace.data_ptr(), _stream())
+    call("gptb200_adamw8_update_range", _adamw8_flat("params", params, n, F32), q,
+         _adamw8_flat("grads", grads, n, F32), int(begin), int(end), groups_dev.data_ptr(), n_groups,
+         cfg, int(slot), _adamw8_flat("params_bf16", params_bf16, n, BF16), seed & 0xFFFFFFFF,
+         workspace.data_ptr(), _stream())
 
 
 def adamw8_values(state) -> tuple[torch.Tensor, torch.Tensor]:
     """(m, sqrt(v)) that a state's codes stand for, as bf16 (exact)."""
 
     n = state[0].numel()
-    q = _adamw8(state, n, {})
+    q = _adamw8(state, n)
     m = torch.empty(n, dtype=BF16, device=state[0].device)
     root = torch.empty_like(m)
-    call("gptb200_adamw8_values", ctypes.byref(q), n, m.data_ptr(), root.data_ptr(), _stream())
+    call("gptb200_adamw8_values", q, n, m.data_ptr(), root.data_ptr(), _stream())
     return m, root
 
 
