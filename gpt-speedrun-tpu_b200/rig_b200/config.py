@@ -57,6 +57,12 @@ class Config:
     mlp_activation: str = "gelu"
     document_masking: bool = False        # the context preset's document-attention policy
     document_boundary_token: int = 50256  # recipes/reference/train.py:234-235
+    # variants the reference lacks: `normalization` may be "layer_norm" (scale and
+    # bias); a tanh cap of the attention scores (0: none); "distance": the scores
+    # fall with slope_h |i - j| (kernels.distance_slopes); bits of an Adam moment
+    attention_softcap: float = 0.0
+    attention_bias: str = "none"
+    optimizer_state_bits: int = 32
     # routed MLP (recipes/reference_moe/train.py:242-245); experts = 0: dense MLP
     experts: int = 0
     expert_top_k: int = 2
@@ -108,11 +114,21 @@ class Config:
         raise ValueError(f"unsupported attention scale {self.attention_scale!r}")
 
     @property
+    def score_attention(self) -> bool:
+        """Whether the attention scores are capped or biased."""
+
+        return self.attention_softcap > 0.0 or self.attention_bias != "none"
+
+    @property
     def tied(self) -> bool:
         return self.embeddings == "tied"
 
     def replace(self, **kw: Any) -> "Config":
         return dataclasses.replace(self, **kw)
+
+
+NORMALIZATIONS = ("rms_norm", "layer_norm")  # the reference's (train.py:323), and a variant
+ATTENTION_BIASES = ("none", "distance")
 
 
 def _require(mapping: Mapping[str, Any], key: str, where: str) -> Any:
@@ -126,7 +142,8 @@ def tpp_parameters(model: Mapping[str, Any]) -> int:
     vocabulary tables, per block 12 d^2 + 11 d, and the final norm."""
 
     d, layers, vocab = int(model["d_model"]), int(model["layers"]), int(model["vocab_size"])
-    return 2 * vocab * d + layers * (12 * d * d + 11 * d) + d
+    norm_biases = (2 * layers + 1) * d if model.get("normalization") == "layer_norm" else 0
+    return 2 * vocab * d + layers * (12 * d * d + 11 * d) + d + norm_biases
 
 
 def resolve_config(
@@ -163,8 +180,18 @@ def resolve_config(
     training = run["training"]
     optimizer = run["optimizer"]
     kernels = run["kernels"]
-    if model.get("normalization", "rms_norm") != "rms_norm":
-        raise ValueError("only rms_norm is supported (train.py:323)")
+    normalization = model.get("normalization", "rms_norm")
+    if normalization not in NORMALIZATIONS:
+        raise ValueError(f"normalization must be one of {NORMALIZATIONS}, got {normalization!r}")
+    softcap = float(model.get("attention_softcap", 0.0))
+    if not 0.0 <= softcap < math.inf:
+        raise ValueError(f"attention_softcap must be zero (no cap) or positive, got {softcap}")
+    bias = model.get("attention_bias", "none")
+    if bias not in ATTENTION_BIASES:
+        raise ValueError(f"attention_bias must be one of {ATTENTION_BIASES}, got {bias!r}")
+    state_bits = int(optimizer.get("state_bits", 32))
+    if state_bits not in (8, 32):
+        raise ValueError(f"optimizer.state_bits must be 8 or 32, got {state_bits}")
     _check_routing(model, tier_name)
 
     batch = int(batch_size or ctx["reference_batch_size"])
@@ -222,6 +249,10 @@ def resolve_config(
         dtype_name=str(training["dtype"]),
         sampling=str(training.get("sampling", "shuffled_epochs")),
         tier=tier_name,
+        normalization=normalization,
+        attention_softcap=softcap,
+        attention_bias=bias,
+        optimizer_state_bits=state_bits,
         document_masking=bool(ctx.get("document_masking", False)),
         experts=int(model.get("experts", 0)),
         expert_top_k=int(model.get("expert_top_k", 2)),
@@ -290,7 +321,7 @@ def tensor_multipliers(name: str, in_block: bool, config: Config) -> tuple[float
         return lr, eps, wd
     if name == "token_embedding":
         return 1.0, width ** -1, 1.0
-    if name == "final_ln_scale":
+    if name in ("final_ln_scale", "final_ln_bias"):
         return 1.0, 1.0, 1.0
     if name == "output_embedding":
         return width ** -1, 1.0, width

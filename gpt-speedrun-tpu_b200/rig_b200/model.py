@@ -23,6 +23,9 @@ Backward mirrors it with dgrad GEMMs (dGELU fused), weight-gradient GEMMs that
 accumulate into the fp32 gradient buffer with split-K atomics, bias-gradient
 column sums, RMSNorm backward fused with the residual-gradient add, and the
 attention backward writing dq/dk/dv straight into the packed qkv gradient.
+Variants of the same schedule (config.normalization "layer_norm", a capped or
+distance-biased attention, optimizer_state_bits 8) exchange the norm, the
+attention and the update kernels and nothing else.
 With data parallelism each block's gradient slice is all-reduced on NCCL as
 soon as its backward has been enqueued, overlapping the remaining backward.
 """
@@ -37,6 +40,7 @@ import numpy as np
 import torch
 
 from . import _lib, ops
+from .kernels.score_attention import distance_slopes
 from .config import (
     Config,
     decay_for_name,
@@ -58,7 +62,11 @@ ALIGN = 64
 
 
 def block_fields(config: Config) -> tuple[str, ...]:
-    return MOE_BLOCK_FIELDS if config.experts else BLOCK_FIELDS
+    fields = MOE_BLOCK_FIELDS if config.experts else BLOCK_FIELDS
+    if config.normalization == "layer_norm":  # a bias beside each norm's scale
+        fields = tuple(f for name in fields for f in
+                       ((name, name[:3] + "_bias") if name in ("ln1_scale", "ln2_scale") else (name,)))
+    return fields
 
 
 def block_shapes(config: Config) -> dict[str, tuple[int, ...]]:
@@ -66,11 +74,13 @@ def block_shapes(config: Config) -> dict[str, tuple[int, ...]]:
     E, eh = config.experts, config.expert_mult * config.d_model
     return {
         "ln1_scale": (d,),
+        "ln1_bias": (d,),
         "qkv_w": (d, 3 * d),
         "qkv_b": (3 * d,),
         "attn_w": (d, d),
         "attn_b": (d,),
         "ln2_scale": (d,),
+        "ln2_bias": (d,),
         "mlp_up_w": (d, h),
         "mlp_up_b": (h,),
         "mlp_down_w": (h, d),
@@ -97,7 +107,8 @@ class Slot:
 
 
 class ParamLayout:
-    """Flat layout: blocks 0..L-1, then final_ln_scale, token/output embedding."""
+    """Flat layout: blocks 0..L-1, then final_ln_scale (and final_ln_bias with layer
+    norm), token/output embedding."""
 
     def __init__(self, config: Config):
         self.config = config
@@ -119,6 +130,8 @@ class ParamLayout:
             self.block_ranges.append((start, off))
         tail = off
         add("final_ln_scale", "final_ln_scale", -1, (config.d_model,))
+        if config.normalization == "layer_norm":
+            add("final_ln_bias", "final_ln_bias", -1, (config.d_model,))
         add("token_embedding", "token_embedding", -1, (config.vocab_size, config.d_model))
         if not config.tied:
             add("output_embedding", "output_embedding", -1, (config.vocab_size, config.d_model))
@@ -157,13 +170,15 @@ def init_params(config: Config, seed: int) -> dict[str, np.ndarray]:
             shape = shapes[leaf]
             if leaf.endswith("_scale"):
                 value = np.ones(shape, dtype=np.float32)
-            elif leaf.endswith("_b"):
+            elif leaf.endswith(("_b", "_bias")):
                 value = np.zeros(shape, dtype=np.float32)
             else:
                 value = normal(shape, hidden_scale)
             out[f"blocks/{b}/{leaf}"] = value
     out["token_embedding"] = normal((config.vocab_size, config.d_model), config.init_std)
     out["final_ln_scale"] = np.ones((config.d_model,), dtype=np.float32)
+    if config.normalization == "layer_norm":
+        out["final_ln_bias"] = np.zeros((config.d_model,), dtype=np.float32)
     if not config.tied:
         out["output_embedding"] = normal(
             (config.vocab_size, config.d_model), config.init_std / config.width_multiplier
@@ -250,8 +265,13 @@ class GPTTrainer:
         n = self.layout.numel
         self.params = torch.zeros(n, dtype=torch.float32, device=dev)
         self.grads = torch.zeros(n, dtype=torch.float32, device=dev)
-        self.m = torch.zeros(n, dtype=torch.float32, device=dev)
-        self.v = torch.zeros(n, dtype=torch.float32, device=dev)
+        # Adam's moments: two fp32 buffers, or the codes and exponents of 8-bit ones
+        self.m = self.v = self.state8 = None
+        if config.optimizer_state_bits == 8:
+            self.state8 = ops.adamw8_state(n, dev)
+        else:
+            self.m = torch.zeros(n, dtype=torch.float32, device=dev)
+            self.v = torch.zeros(n, dtype=torch.float32, device=dev)
         self.params_bf16 = torch.zeros(n, dtype=torch.bfloat16, device=dev)
         self.step_dev = torch.zeros(1, dtype=torch.int32, device=dev)
         self.history = torch.zeros(max(1, history_steps or config.steps), 3,
@@ -259,6 +279,11 @@ class GPTTrainer:
         self.blocks = [_Block(self, b) for b in range(config.layers)]
         self.final_scale = self.param_view("final_ln_scale", bf16=True)
         self.g_final_scale = self.grad_view("final_ln_scale")
+        self.layer_norm = config.normalization == "layer_norm"
+        if self.layer_norm:
+            self.final_bias = self.param_view("final_ln_bias", bf16=True)
+            self.g_final_bias = self.grad_view("final_ln_bias")
+        self.slopes = distance_slopes(config.heads, dev) if config.attention_bias == "distance" else None
         self.tok_emb = self.param_view("token_embedding", bf16=True)
         self.g_tok_emb = self.grad_view("token_embedding")
         if config.tied:
@@ -287,8 +312,8 @@ class GPTTrainer:
             self.params[s.offset : s.offset + s.size].copy_(
                 torch.from_numpy(np.ascontiguousarray(arr)).reshape(-1))
         ops.cast_bf16(self.params, self.params_bf16)
-        self.m.zero_()
-        self.v.zero_()
+        for state in (self.m, self.v) if self.state8 is None else self.state8:
+            state.zero_()
         self.step_dev.zero_()
 
     def export(self, buf: torch.Tensor | None = None) -> dict[str, np.ndarray]:
@@ -306,6 +331,8 @@ class GPTTrainer:
         self.x = [torch.empty(N, d, **bf) for _ in range(L + 1)]
         self.ln1 = [torch.empty(N, d, **bf) for _ in range(L)]
         self.rstd1 = [torch.empty(N, **f32) for _ in range(L)]
+        means = 2 * L + 1 if c.normalization == "layer_norm" else 0  # per block two, and the final norm's
+        self.means = [torch.empty(N, **f32) for _ in range(means)]
         self.qkv = [torch.empty(N, 3 * d, **bf) for _ in range(L)]
         self.att = [torch.empty(N, d, **bf) for _ in range(L)]
         self.lse = [torch.empty(self.B, c.heads, self.T, **f32) for _ in range(L)]
@@ -331,7 +358,10 @@ class GPTTrainer:
         self.du = None if c.experts else torch.empty(N, h, **bf)
         self.datt = torch.empty(N, d, **bf)
         self.dqkv = torch.empty(N, 3 * d, **bf)
-        self.attn_ws = ops.attention_workspace(self.B, c.heads, self.T, dev)
+        self.attn_ws = (
+            torch.empty(ops.score_attention_workspace_size(self.B, c.heads, self.T),
+                        dtype=torch.uint8, device=dev)
+            if c.score_attention else ops.attention_workspace(self.B, c.heads, self.T, dev))
         self.lce_fwd_ws = ops.lce_fwd_workspace(N, c.vocab_size, dev)
         self.lce_bwd_ws = ops.lce_bwd_workspace(N, c.vocab_size, dev)
         self.tokens = torch.empty(self.B, self.T, dtype=torch.int32, device=dev)
@@ -339,7 +369,9 @@ class GPTTrainer:
         # One scratch buffer shared by the backward's ordered reductions (they
         # run one after another on the step's stream).
         wgrad_shapes = [(d, 3 * d), (d, d)] + ([] if c.experts else [(d, h), (h, d)])
-        need = [ops.rms_norm_bwd_workspace_size(N, d),
+        norm_bytes = (ops.layer_norm_bwd_workspace_size if c.normalization == "layer_norm"
+                      else ops.rms_norm_bwd_workspace_size)
+        need = [norm_bytes(N, d),
                 ops.embedding_bwd_workspace_size(N, d, c.vocab_size)]
         need += [ops.colsum_workspace_size(N, w) for w in (3 * d, h)]
         self.scratch = torch.empty(max(need), dtype=torch.uint8, device=dev)
@@ -480,6 +512,55 @@ class GPTTrainer:
         c = self.config
         return buf.view(self.B, self.T, c.heads, c.head_dim)
 
+    # ------------------------------------------------------------ norm, attention
+    def _norm_params(self, l: int, which: int):
+        """(scale, bias, their gradients) of norm `which` (1, 2) of block l, or of the
+        final norm for l = layers; the biases are None with RMSNorm."""
+
+        if l == self.config.layers:
+            owner, name = self, "final_"
+        else:
+            owner, name = self.blocks[l], f"ln{which}_"
+        bias = (getattr(owner, name + "bias"), getattr(owner, f"g_{name}bias")) if self.layer_norm else (None, None)
+        return getattr(owner, name + "scale"), bias[0], getattr(owner, f"g_{name}scale"), bias[1]
+
+    def _norm_fwd(self, x, l: int, which: int, y, rstd) -> None:
+        scale, bias, _, _ = self._norm_params(l, which)
+        if self.layer_norm:
+            ops.layer_norm_fwd(x, scale, bias, y, self.means[2 * l + which - 1], rstd)
+        else:
+            ops.rms_norm_fwd(x, scale, y, rstd)
+
+    def _norm_bwd(self, x, l: int, which: int, rstd, dy, dx_in, dx_out, colsum, alpha) -> None:
+        scale, _, g_scale, g_bias = self._norm_params(l, which)
+        if self.layer_norm:
+            ops.layer_norm_bwd(x, scale, self.means[2 * l + which - 1], rstd, dy, dx_in, dx_out,
+                               g_scale, g_bias, colsum, alpha, workspace=self.scratch)
+        else:
+            ops.rms_norm_bwd(x, scale, rstd, dy, dx_in, dx_out, g_scale, colsum, alpha,
+                             workspace=self.scratch)
+
+    def _attention_fwd(self, q, k, v, o, lse) -> None:
+        c = self.config
+        if c.score_attention:
+            ops.score_attention_fwd(q, k, v, o, lse, scale=c.softmax_scale, layout="bthd",
+                                    softcap=c.attention_softcap, slopes=self.slopes,
+                                    segment_ids=self.segments)
+        else:
+            ops.attention_fwd(q, k, v, o, lse, scale=c.softmax_scale, layout="bthd",
+                              segment_ids=self.segments)
+
+    def _attention_bwd(self, q, k, v, o, do, lse, dq, dk, dv) -> None:
+        c = self.config
+        if c.score_attention:
+            ops.score_attention_bwd(q, k, v, o, do, lse, dq, dk, dv, scale=c.softmax_scale,
+                                    layout="bthd", softcap=c.attention_softcap, slopes=self.slopes,
+                                    segment_ids=self.segments, rope=self.rope,
+                                    workspace=self.attn_ws)
+        else:
+            ops.attention_bwd(q, k, v, o, do, lse, dq, dk, dv, scale=c.softmax_scale, layout="bthd",
+                              rope=self.rope, workspace=self.attn_ws, segment_ids=self.segments)
+
     # ------------------------------------------------------------ step
     def set_batch(self, x: torch.Tensor, y: torch.Tensor) -> None:
         """Copies a [B, T] int32 batch (host pinned or device) into the step's buffers."""
@@ -498,16 +579,15 @@ class GPTTrainer:
             ops.document_segments(self.tokens.view(self.B, self.T), c.document_boundary_token,
                                   self.segments)
         for l, blk in enumerate(self.blocks):
-            ops.rms_norm_fwd(self.x[l], blk.ln1_scale, self.ln1[l], self.rstd1[l])
+            self._norm_fwd(self.x[l], l, 1, self.ln1[l], self.rstd1[l])
             # QKV projection with bias and RoPE on the q/k columns in the epilogue
             ops.matmul(self.ln1[l], blk.qkv_w, bias=blk.qkv_b, out=self.qkv[l],
                        kind=_lib.EPI_BIAS_ROPE, rope=self.rope, rope_cols=2 * d)
             q, k, v = self._qkv_views(self.qkv[l])
-            ops.attention_fwd(q, k, v, self._bthd(self.att[l]), self.lse[l], scale=c.softmax_scale,
-                              layout="bthd", segment_ids=self.segments)
+            self._attention_fwd(q, k, v, self._bthd(self.att[l]), self.lse[l])
             ops.matmul(self.att[l], blk.attn_w, bias=blk.attn_b, alpha=a, residual=self.x[l],
                        out=self.xm[l])
-            ops.rms_norm_fwd(self.xm[l], blk.ln2_scale, self.ln2[l], self.rstd2[l])
+            self._norm_fwd(self.xm[l], l, 2, self.ln2[l], self.rstd2[l])
             if c.experts:
                 self._moe_forward(l, blk)
                 continue
@@ -515,7 +595,7 @@ class GPTTrainer:
                        aux=self.gelu_grad[l], out=self.g[l])
             ops.matmul(self.g[l], blk.mlp_down_w, bias=blk.mlp_down_b, alpha=a,
                        residual=self.xm[l], out=self.x[l + 1])
-        ops.rms_norm_fwd(self.x[c.layers], self.final_scale, self.lnf, self.rstdf)
+        self._norm_fwd(self.x[c.layers], c.layers, 1, self.lnf, self.rstdf)
         ops.lce_fwd(self.lnf, self.out_emb, self.targets.view(-1), c.semantic_vocab_size,
                     self.losses, self.lse_ce, self.loss, workspace=self.lce_fwd_ws)
         if c.experts:
@@ -545,8 +625,8 @@ class GPTTrainer:
         # gradient of the bias of the branch below it; its column sums are fused.
         # (a routed MLP's biases are per expert: their sums come from moe_segment_colsum)
         mlp_bias = (lambda l: None) if c.experts else (lambda l: self.blocks[l].g_mlp_down_b)
-        ops.rms_norm_bwd(self.x[c.layers], self.final_scale, self.rstdf, self.dln, None, self.dx,
-                         self.g_final_scale, mlp_bias(c.layers - 1), a, workspace=self.scratch)
+        self._norm_bwd(self.x[c.layers], c.layers, 1, self.rstdf, self.dln, None, self.dx,
+                       mlp_bias(c.layers - 1), a)
         dx = self.dx
         for l in reversed(range(c.layers)):
             blk = self.blocks[l]
@@ -560,22 +640,19 @@ class GPTTrainer:
                 self._wgrad(self.ln2[l], self.du, blk.g_mlp_up_w, 1.0)
                 ops.colsum(self.du, blk.g_mlp_up_b, 1.0, workspace=self.scratch)
                 self._dgrad(self.du, blk.mlp_up_w, self.dln)
-            ops.rms_norm_bwd(self.xm[l], blk.ln2_scale, self.rstd2[l], self.dln, dx, dx,
-                             blk.g_ln2_scale, blk.g_attn_b, a, workspace=self.scratch)
+            self._norm_bwd(self.xm[l], l, 2, self.rstd2[l], self.dln, dx, dx, blk.g_attn_b, a)
             # attention: xm = x + a * (att Wo + bo)
             self._dgrad(dx, blk.attn_w, self.datt, alpha=a)
             self._wgrad(self.att[l], dx, blk.g_attn_w, a)
             q, k, v = self._qkv_views(self.qkv[l])
             dq, dk, dv = self._qkv_views(self.dqkv)
-            ops.attention_bwd(q, k, v, self._bthd(self.att[l]), self._bthd(self.datt), self.lse[l],
-                              dq, dk, dv, scale=c.softmax_scale, layout="bthd", rope=self.rope,
-                              workspace=self.attn_ws, segment_ids=self.segments)
+            self._attention_bwd(q, k, v, self._bthd(self.att[l]), self._bthd(self.datt), self.lse[l],
+                                dq, dk, dv)
             self._wgrad(self.ln1[l], self.dqkv, blk.g_qkv_w, 1.0)
             ops.colsum(self.dqkv, blk.g_qkv_b, 1.0, workspace=self.scratch)
             self._dgrad(self.dqkv, blk.qkv_w, self.dln)
             below = mlp_bias(l - 1) if l > 0 else None
-            ops.rms_norm_bwd(self.x[l], blk.ln1_scale, self.rstd1[l], self.dln, dx, dx,
-                             blk.g_ln1_scale, below, a, workspace=self.scratch)
+            self._norm_bwd(self.x[l], l, 1, self.rstd1[l], self.dln, dx, dx, below, a)
             if reduce_hook is not None:
                 reduce_hook(*self.layout.block_ranges[l])
         ops.embedding_bwd(self.tokens.view(-1), dx, self.g_tok_emb, workspace=self.scratch)
@@ -587,7 +664,15 @@ class GPTTrainer:
             for part in tail_parts(*self.layout.tail_range):
                 reduce_hook(*part)
 
+    # seed of the 8-bit moments' rounding (the same on every data-parallel rank)
+    state_seed: int = 0
+
     def optimizer_step(self) -> None:
+        if self.state8 is not None:
+            ops.adamw8_step(self.params, self.state8, self.grads, self.groups_dev, self.n_groups,
+                            self.adam_cfg, self.step_dev, self.loss, self.history,
+                            self.params_bf16, self.state_seed, self.adam_ws)
+            return
         ops.adamw_step(self.params, self.m, self.v, self.grads, self.groups_dev, self.n_groups,
                        self.adam_cfg, self.step_dev, self.loss, self.history, self.params_bf16,
                        self.adam_ws)
@@ -737,9 +822,15 @@ class GPTTrainer:
             with torch.cuda.stream(opt):
                 if work is not None:
                     work.wait()
-                ops.adamw_update_range(self.params, self.m, self.v, self.grads, start, end,
-                                       self.groups_dev, self.n_groups, self.adam_cfg, len(slots),
-                                       self.params_bf16, self.adam_ws)
+                if self.state8 is not None:
+                    ops.adamw8_update_range(self.params, self.state8, self.grads, start, end,
+                                            self.groups_dev, self.n_groups, self.adam_cfg,
+                                            len(slots), self.params_bf16, self.state_seed,
+                                            self.adam_ws)
+                else:
+                    ops.adamw_update_range(self.params, self.m, self.v, self.grads, start, end,
+                                           self.groups_dev, self.n_groups, self.adam_cfg,
+                                           len(slots), self.params_bf16, self.adam_ws)
             slots.append((start, end))
 
         if self.world_size > 1:

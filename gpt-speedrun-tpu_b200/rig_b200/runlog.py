@@ -162,6 +162,10 @@ def checkpoint_metadata(config: Any, seed: int) -> dict[str, Any]:
     """The model description that travels in checkpoint.npz, with the key
     structure of recipes/reference/train.py:1042-1076."""
 
+    variant = {}  # what the reference's models lack, where a model has it
+    if config.score_attention:
+        variant = {"attention_softcap": config.attention_softcap,
+                   "attention_bias": config.attention_bias}
     return {
         "schema_version": 6,
         "seed": int(seed),
@@ -191,5 +195,6 @@ def checkpoint_metadata(config: Any, seed: int) -> dict[str, Any]:
             "tied_embeddings": bool(config.tied),
             "tier": config.tier,
             "parameterization": config.parameterization,
+            **variant,
         },
     }
