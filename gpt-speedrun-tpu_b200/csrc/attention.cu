@@ -511,12 +511,11 @@ GPTB200_DEV uint32_t segment_columns(int id, int key_id) {
 // Padding (a negative id) never equals another id: queries carry -2, keys -1.
 GPTB200_DEV int seg_query_id(int v) { return v < 0 ? -2 : v; }
 GPTB200_DEV int seg_key_id(int v) { return v < 0 ? -1 : v; }
-// Range of a chunk's ids: a chunk of padding alone meets nothing, and a chunk
-// with some padding keeps -1 in its range, so that it is never a single id.
-GPTB200_DEV int2 seg_chunk(int mn, int mx) {
-  if (mn < 0) return mx < 0 ? make_int2(INT_MAX, INT_MIN) : make_int2(-1, mx);
-  return make_int2(mn, mx);
-}
+// Ranges of ids with padding as -1: it is part of its chunk's (and so of its
+// tile's) range, but what meets, or is one id without a test, is an id >= 0.
+GPTB200_DEV int2 seg_chunk(int mn, int mx) { return make_int2(max(mn, -1), max(mx, -1)); }
+GPTB200_DEV bool seg_meet(int2 a, int2 b) { return rng_meet(a, b) && min(a.y, b.y) >= 0; }
+GPTB200_DEV bool seg_single(int2 a, int2 b) { return rng_single(a, b) && a.x >= 0; }
 
 // ------------------------------------------------------------------ forward
 // Persistent: one CTA per SM walks work items (pair of 128-query tiles pr,
@@ -718,8 +717,8 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
           int n = 0, n_le0 = 0;
           for (int j = 0; j < nkv; ++j) {
             const int2 kr = seg_range(tab, nch, 2 * j, 2);
-            if (j == d0 || j == dmax || (j < n0 && rng_meet(kr, qr0)) ||
-                (has1 && rng_meet(kr, qr1))) {
+            if (j == d0 || j == dmax || (j < n0 && seg_meet(kr, qr0)) ||
+                (has1 && seg_meet(kr, qr1))) {
               bl[n++] = j;
               if (j < n0) ++n_le0;
             }
@@ -1090,7 +1089,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
         }
         // keys past a query (and past T) are masked, keys of another id too
         const bool diag = jb * FK + FK - 1 > max(q0 + x * FQ, inf.prefix - 1);
-        const bool segmask = SEG && !rng_single(seg_range(segtab, inf.nch, 2 * jb, 2), qrng);
+        const bool segmask = SEG && !seg_single(seg_range(segtab, inf.nch, 2 * jb, 2), qrng);
         const bool ahead = (MODE & kBias) && jb * FK + FK - 1 > q0 + x * FQ;  // |i - j| either way
         if (!(ok = mbar_wait(&s_full[x], jj & 1, abort_flag, err))) break;
         tc_fence_after();
@@ -1468,7 +1467,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kBwdThreads : kBwdGeneralTh
           const int2 kr = seg_range(tab, nch, (k0 - qb) / kSegChunk, 2);
           int n = 0;
           for (int it = 0; it < nq_all; ++it)
-            if (rng_meet(seg_range(tab, nch, it, 1), kr)) ql[n++] = it;
+            if (seg_meet(seg_range(tab, nch, it, 1), kr)) ql[n++] = it;
           while ((n & 1) || n == 0) ql[n++] = nq_all;
           nq = n;
         }
@@ -1725,7 +1724,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kBwdThreads : kBwdGeneralTh
         if constexpr (GENERAL) {
           const int q0 = qoff + qt * BQ;  // the tile's first query relative to the keys
           // per-element segment test unless this key tile and query tile share one id
-          const bool segmask = SEG && !rng_single(seg_range(segtab, nch, qt, 1), krng);
+          const bool segmask = SEG && !seg_single(seg_range(segtab, nch, qt, 1), krng);
           const bool diag = q0 < BT;  // some key may be past some query
           const float* stat =
               reinterpret_cast<const float*>(sm + L::STAT + (gt % kQS) * L::kStatBytes);

@@ -152,6 +152,28 @@ def test_formula(cuda, b, h, kv, t, mask, cap, bias):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("edges", [(64,), (192,), (256,), (320,), (64, 128), (128, 192, 320)])
+def test_padding_from_chunk_and_tile_boundaries(cuda, edges):
+    """Padding that starts or ends where the kernels' 64- and 128-position tiles do,
+    with whole tiles of it between tokens of one id; prefixes over both."""
+
+    t = 400
+    seg = torch.zeros(2, t, dtype=torch.int32)
+    for i in range(t):  # tokens and padding in turn, from edge to edge
+        seg[:, i] = 0 if sum(i >= e for e in edges) % 2 == 0 else -1
+    seg[1] = torch.where(seg[1] < 0, 2, -1)
+    seg = seg.to(cuda)
+    for cap, bias, prefix in ((30.0, True, None), (0.0, False, [t, 100])):
+        q, k, v, do = (x.to(cuda) for x in _inputs(2, 2, 1, t, 12))
+        how = dict(softcap=cap, slopes=kernels.distance_slopes(2, cuda) if bias else None,
+                   segment_ids=seg,
+                   prefix_lens=None if prefix is None else torch.tensor(prefix, dtype=torch.int32, device=cuda))
+        want, tol, want_lse = _formula(q, k, v, do, 0.125, cap, how["slopes"], seg, how["prefix_lens"])
+        got, lse = _run(q, k, v, do, scale=0.125, **how)
+        _check(got, lse, want, tol, want_lse)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("cap,spread", [(1.5, 12.0), (30.0, 40.0), (4.0, 3.0), (1e4, 3.0)])
 def test_cap_from_linear_to_saturated(cuda, cap, spread):
     """Both forms of tanh, and scores around the limit between them."""
