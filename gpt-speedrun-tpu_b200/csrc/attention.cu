@@ -81,6 +81,7 @@ struct AttnParams {
   // output / saved tensors
   bf16* o;
   int64_t osb, osh, ost;
+  float* o32;          // [B, H, T, 64] fp32 instead of o and lse, or null (MODE > kClassic)
   float* lse;          // [B, H, T], natural log
   const bf16* dout;
   const float* delta;  // [B, H, T] (MODE > kClassic: negated)
@@ -1193,7 +1194,13 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
 #pragma unroll
         for (int cc = 0; cc < HD / 32; ++cc) {
           tmem_ld32(tO(x) + lane_off + cc * 32, o);
-          if (qrow < p.T) {
+          if (qrow < p.T && p.o32) {
+            float* row = p.o32 + ((int64_t)bh * p.T + qrow) * HD + cc * 32;
+#pragma unroll
+            for (int g = 0; g < 8; ++g)
+              reinterpret_cast<float4*>(row)[g] = make_float4(
+                  o[4 * g] * inv, o[4 * g + 1] * inv, o[4 * g + 2] * inv, o[4 * g + 3] * inv);
+          } else if (qrow < p.T) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
               uint4 q;
@@ -1205,7 +1212,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
             }
           }
         }
-        if (qrow < p.T)
+        if (qrow < p.T && !p.o32)
           p.lse[(int64_t)bh * p.T + qrow] = l == 0.f ? -INFINITY : (m_used + __log2f(l)) * kLn2;
       }
       if (!ok) break;
@@ -2038,7 +2045,7 @@ __global__ void attn_delta_kernel(const bf16* __restrict__ o, const bf16* __rest
                                   int64_t osb, int64_t osh, int64_t ost, int64_t gsb, int64_t gsh,
                                   int64_t gst, int B, int H, int T, float* __restrict__ delta,
                                   float* __restrict__ dq_acc, const float* __restrict__ lse,
-                                  float* __restrict__ neg_lse2) {
+                                  float* __restrict__ neg_lse2, bool o_in_acc) {
   const int64_t rows = (int64_t)B * H * T;
   const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
   const int seg = threadIdx.x & 7;
@@ -2049,17 +2056,29 @@ __global__ void attn_delta_kernel(const bf16* __restrict__ o, const bf16* __rest
   const int b = (int)(bh / H), h = (int)(bh - (int64_t)b * H);
   const int64_t off = b * osb + h * osh + (int64_t)t * ost + seg * 8;
   const int64_t goff = b * gsb + h * gsh + (int64_t)t * gst + seg * 8;
-  const uint4 qo = *reinterpret_cast<const uint4*>(o + off);
   const uint4 qg = *reinterpret_cast<const uint4*>(dout + goff);
-  const uint32_t* wo = &qo.x;
   const uint32_t* wg = &qg.x;
   float s = 0.f;
+  if (o_in_acc) {  // fp32 rows in the accumulator's place; this thread clears what it reads
+    const float4* src = reinterpret_cast<const float4*>(dq_acc + rr * HD + seg * 8);
+    const float4 a = src[0], c = src[1];
+    const float ov[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float o0, o1, g0, g1;
-    unpack_bf16x2(wo[j], o0, o1);
-    unpack_bf16x2(wg[j], g0, g1);
-    s += o0 * g0 + o1 * g1;
+    for (int j = 0; j < 4; ++j) {
+      float g0, g1;
+      unpack_bf16x2(wg[j], g0, g1);
+      s += ov[2 * j] * g0 + ov[2 * j + 1] * g1;
+    }
+  } else {
+    const uint4 qo = *reinterpret_cast<const uint4*>(o + off);
+    const uint32_t* wo = &qo.x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float o0, o1, g0, g1;
+      unpack_bf16x2(wo[j], o0, o1);
+      unpack_bf16x2(wg[j], g0, g1);
+      s += o0 * g0 + o1 * g1;
+    }
   }
   s += __shfl_xor_sync(0xffffffffu, s, 1);
   s += __shfl_xor_sync(0xffffffffu, s, 2);
@@ -2299,7 +2318,7 @@ extern "C" int gptb200_attention_bwd(const void* q, const void* k, const void* v
   attn_delta_kernel<<<(unsigned)((rows * 8 + 255) / 256), 256, 0, st>>>(
       reinterpret_cast<const bf16*>(o), reinterpret_cast<const bf16*>(dout), o_stride_b,
       o_stride_h, o_stride_t, o_stride_b, o_stride_h, o_stride_t, B, H, T, delta, dq_acc, nullptr,
-      nullptr);
+      nullptr, false);
   GPTB200_CHECK_LAUNCH();
   AttnParams p = {};
   p.B = B;
@@ -2460,12 +2479,10 @@ static int score_mode(const gptb200_score_attention* a, F&& f) {
                    : f(std::integral_constant<int, kGeneral>());
 }
 
-}  // namespace gptb200
-
-extern "C" int gptb200_score_attention_fwd(const gptb200_score_attention* a, void* stream) {
-  const int s = score_check(a);
-  if (s) return s;
+// The forward of a checked call, with fp32 rows for o and no lse if o32.
+static int score_forward(const gptb200_score_attention* a, float* o32, cudaStream_t st) {
   AttnParams p = score_params(a);
+  p.o32 = o32;
   ScoreMaps m;
   const int64_t *qs = a->q_stride, *ks = a->kv_stride;
   if (!make_map4(&m.q, a->q, p.B, p.H, p.T, qs[0], qs[1], qs[2], FQ) ||
@@ -2476,11 +2493,17 @@ extern "C" int gptb200_score_attention_fwd(const gptb200_score_attention* a, voi
   if (!p.sched) return GPTB200_EUNSUPPORTED;
   // K and V of every head
   p.by_weight = by_weight(a, a->batch * a->kv_heads * a->seq * 2 * HD * 2, 160, 512);
-  auto st = reinterpret_cast<cudaStream_t>(stream);
   return score_mode(a, [&](auto mode) {
     constexpr int MODE = decltype(mode)::value;
     return p.seg ? score_fwd_launch<true, MODE>(p, m, st) : score_fwd_launch<false, MODE>(p, m, st);
   });
+}
+
+}  // namespace gptb200
+
+extern "C" int gptb200_score_attention_fwd(const gptb200_score_attention* a, void* stream) {
+  const int s = score_check(a);
+  return s ? s : score_forward(a, nullptr, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t gptb200_score_attention_bwd_workspace_size(int64_t batch, int64_t heads,
@@ -2524,9 +2547,21 @@ extern "C" int gptb200_score_attention_bwd(const gptb200_score_attention* a, con
   p.sched = sched_slot(1);
   if (!p.sched) return GPTB200_EUNSUPPORTED;
   auto st = reinterpret_cast<cudaStream_t>(stream);
+  // delta = sum dO O from the stored O carries its rounding to bf16 (2^-9 |dO| |O|)
+  // into dS = P (dP - delta) of the whole row. Where a row has few keys, one of
+  // them tends to hold most of P, dP - delta is small for it and the rounding
+  // weighs more: dq and dk are 0.0046 off at 33 keys, 0.0037 at 64 to 256 and
+  // 0.0030 at 1,024 (relative; 0.0024 with an exact delta). So sequences of one
+  // key tile compute O again, in fp32 and into the accumulator that delta's
+  // kernel clears: one more launch for a forward of one block a tile.
+  const bool short_rows = p.T <= FK;
+  if (short_rows) {
+    const int f = score_forward(a, dq_acc, st);
+    if (f) return f;
+  }
   attn_delta_kernel<<<(unsigned)((rows * 8 + 255) / 256), 256, 0, st>>>(
       p.o, reinterpret_cast<const bf16*>(dout), p.osb, p.osh, p.ost, dout_stride[0], dout_stride[1],
-      dout_stride[2], p.B, p.H, p.T, delta, dq_acc, a->lse, neg_lse2);
+      dout_stride[2], p.B, p.H, p.T, delta, dq_acc, a->lse, neg_lse2, short_rows);
   GPTB200_CHECK_LAUNCH();
   p.delta = delta;
   p.neg_lse2 = neg_lse2;
