@@ -1094,11 +1094,15 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
         const bool ahead = (MODE & kBias) && jb * FK + FK - 1 > q0 + x * FQ;  // |i - j| either way
         if (!(ok = mbar_wait(&s_full[x], jj & 1, abort_flag, err))) break;
         tc_fence_after();
-        // P and O of the previous block must have been consumed by its P.V MMA
-        if (j > 0) {
-          if (!(ok = mbar_wait(&pv_done[x], (jj - 1) & 1, abort_flag, err))) break;
-          tc_fence_after();
-        }
+        // P and O of the previous block must have been consumed by its P.V MMA,
+        // which may still run while this block's first scores are computed.
+        auto previous_done = [&]() {
+          if (j > 0) {
+            ok = mbar_wait(&pv_done[x], (jj - 1) & 1, abort_flag, err);
+            tc_fence_after();
+          }
+          return ok;
+        };
         const uint32_t aS = tS(x) + lane_off, aP = tP(x) + lane_off;
         const float at0 = (float)(jb * FK - qrow);
         uint32_t v[32], pk[16];
@@ -1113,9 +1117,11 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
             tmem_ld32_nw(aS + 32 * w, v);
             tmem_wait_ld();
             score.stream(v, at0 + (float)(32 * w), m_used, pk, acc, top, far);
+            if (w == 0 && !previous_done()) break;
             tmem_st8_nw(aP + 16 * w, pk);
             tmem_st8_nw(aP + 16 * w + 8, pk + 8);
           }
+          if (!ok) break;
           steps = Score<MODE>::discard(top, far);
         }
         if (steps) {
@@ -1148,6 +1154,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
             alpha = m_new == -INFINITY ? 1.f : ex2(m_used - m_new);
             m_used = m_new;
           }
+          if (!previous_done()) break;
           const float sub = m_used == -INFINITY ? 0.f : m_used;  // exp2(-inf - sub) = 0
           acc[0] = acc[1] = make_float2(0.f, 0.f);
 #pragma unroll 1
@@ -2574,7 +2581,7 @@ extern "C" int gptb200_score_attention_bwd(const gptb200_score_attention* a, con
   p.rcos = reinterpret_cast<const bf16*>(rope_cos);
   p.rsin = reinterpret_cast<const bf16*>(rope_sin);
   // Q and dO of every head
-  p.by_weight = by_weight(a, rows * 2 * HD * 2, 64, 256);
+  p.by_weight = by_weight(a, rows * 2 * HD * 2, 64, 512);
   const int e = score_mode(a, [&](auto mode) {
     constexpr int MODE = decltype(mode)::value;
     return p.seg ? score_bwd_launch<true, MODE>(p, m, st) : score_bwd_launch<false, MODE>(p, m, st);
