@@ -238,9 +238,12 @@ struct Score {
   float z_per_s;  // tanh's argument per raw score
   float out;      // s' log2(e) per tanh, or per raw score
   float slope2;   // slope * log2(e)
+  float far_max;  // the largest raw score squared with |z| <= 1
   GPTB200_DEV Score(const AttnParams& p, float slope2_) : slope2(slope2_) {
     z_per_s = CAP ? p.scale / p.cap : 1.f;
     out = (CAP ? p.cap : p.scale) * kLog2e;
+    // below 2^-13 the ninth power in stream_coefs may underflow: never stream
+    far_max = z_per_s < 0x1p-13f ? -1.f : 1.f / (z_per_s * z_per_s);
   }
   static GPTB200_DEV float2 both(float x) { return make_float2(x, x); }
   static GPTB200_DEV float2 pair(const uint32_t (&v)[32], int i) {
@@ -265,38 +268,49 @@ struct Score {
 
   // Without masks, keys before the query, against the maximum m: arithmetic (FMA
   // pipe) and exponentials (MUFU) of different columns overlap, with nothing to
-  // wait for in between. top and far collect the largest exponent and tanh
-  // argument squared; the caller discards the block if they do not do. `at`:
-  // first key - query. The bias, slope (key - query), with -m folded in, runs
-  // in four pairs that step by eight keys: one addition for two scores.
-  GPTB200_DEV void stream(const uint32_t (&v)[32], float at, float m, uint32_t (&pk)[16],
-                          float2 (&acc)[2], float& top, float& far) const {
-    float2 k[5];
-    if constexpr (CAP) coefs(k);
-    float2 off[4];
+  // wait for in between. 16 columns at a time; the callers have the next ones on
+  // their way from TMEM meanwhile. top and far collect the largest exponent and
+  // raw score squared; the caller discards the block if they do not do. The tanh's
+  // argument is not formed: its factor is in the coefficients (stream_coefs). The
+  // bias, slope (key - query), with -m folded in, runs in four pairs that step by
+  // eight keys: one addition for two scores. `at`: first key - query.
+  GPTB200_DEV void stream_coefs(float2 (&k)[5]) const {
+    constexpr float c[5] = GPTB200_TANH_COEFS;
+    float f = out * z_per_s;
+#pragma unroll
+    for (int u = 0; u < 5; ++u) {
+      k[u] = both(f * c[u]);
+      f *= z_per_s * z_per_s;
+    }
+  }
+  GPTB200_DEV void stream_bias(float at, float m, float2 (&off)[4]) const {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       off[q] = BIAS ? make_float2(fmaf(slope2, at + (float)(2 * q), -m),
                                   fmaf(slope2, at + (float)(2 * q + 1), -m))
                     : both(-m);
+  }
+  GPTB200_DEV void stream(const uint32_t (&v)[16], const float2 (&k)[5], float2 (&off)[4],
+                          uint32_t* pk, float2 (&acc)[2], float& top, float& far) const {
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      float2 y[4];
+    for (int i = 0; i < 16; i += 8) {
+      float2 s[4], y[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        s[q] = make_float2(__uint_as_float(v[i + 2 * q]), __uint_as_float(v[i + 2 * q + 1]));
       if constexpr (CAP) {
-        float2 z[4], u[4], a[4];
+        float2 u[4], a[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) z[q] = fmul2(pair(v, i + 2 * q), both(z_per_s));
-#pragma unroll
-        for (int q = 0; q < 4; ++q) u[q] = fmul2(z[q], z[q]);
+        for (int q = 0; q < 4; ++q) u[q] = fmul2(s[q], s[q]);
         poly4(k, u, a);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           far = fmax3(far, u[q].x, u[q].y);
-          y[q] = ffma2(z[q], a[q], off[q]);
+          y[q] = ffma2(s[q], a[q], off[q]);
         }
       } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) y[q] = ffma2(pair(v, i + 2 * q), both(out), off[q]);
+        for (int q = 0; q < 4; ++q) y[q] = ffma2(s[q], both(out), off[q]);
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -309,9 +323,9 @@ struct Score {
     }
   }
   // Whether a block that went through stream() has to be done in steps.
-  static GPTB200_DEV bool discard(float top, float far) {
+  GPTB200_DEV bool discard(float top, float far) const {
     // (m = -inf lifts everything to +inf)
-    return __any_sync(0xffffffffu, !(top <= kSlack) || (CAP && far > 1.f));
+    return __any_sync(0xffffffffu, !(top <= kSlack) || (CAP && !(far <= far_max)));
   }
 
   // Modified scores in place of the raw ones, in log2, and their maximum; those
@@ -1112,17 +1126,25 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
         bool steps = diag || segmask || ahead;
         if (!steps) {
           float top = -INFINITY, far = 0.f;
+          float2 k[5], off[4];
+          if constexpr ((MODE & kCap) != 0) score.stream_coefs(k);
+          uint32_t va[16], vb[16];
+          tmem_ld16_nw(aS, va);
 #pragma unroll 1
           for (int w = 0; w < 4; ++w) {
-            tmem_ld32_nw(aS + 32 * w, v);
+            score.stream_bias(at0 + (float)(32 * w), m_used, off);
             tmem_wait_ld();
-            score.stream(v, at0 + (float)(32 * w), m_used, pk, acc, top, far);
+            tmem_ld16_nw(aS + 32 * w + 16, vb);
+            score.stream(va, k, off, pk, acc, top, far);
+            tmem_wait_ld();
+            if (w < 3) tmem_ld16_nw(aS + 32 * w + 32, va);
+            score.stream(vb, k, off, pk + 8, acc, top, far);
             if (w == 0 && !previous_done()) break;
             tmem_st8_nw(aP + 16 * w, pk);
             tmem_st8_nw(aP + 16 * w + 8, pk + 8);
           }
           if (!ok) break;
-          steps = Score<MODE>::discard(top, far);
+          steps = score.discard(top, far);
         }
         if (steps) {
           // Masks, a new maximum or tanh's long form: modified scores go back
