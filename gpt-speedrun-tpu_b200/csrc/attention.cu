@@ -40,17 +40,35 @@
 // prefix whose keys every query sees, and segment ids whose negative values
 // mark padding (a row that sees nothing gets o = 0, lse = -inf and no
 // gradients). What they add to the softmax warps:
-//  * tanh. The exponentials already fill the MUFU pipe (one per score, 16 per
-//    clock and SM, against 512 clocks of MMA per 128 x 128 scores), so tanh
-//    runs on the FMA pipe: z P(z^2) with five terms, relative error 7e-6, where
-//    a warp's scores have |z| <= 1; only a warp that holds a larger one takes
-//    1 - 2 / (1 + e^(2z)), two more MUFU operations per score.
+//  * tanh. The exponentials hold the MUFU pipe for 8 clocks a score (of a warp's
+//    32 rows), so tanh runs on the FMA pipe beside it, 8 clocks for a score too:
+//    z P(z^2) with five terms, relative error 7e-6, where a warp's scores have
+//    |z| <= 1; only a warp that holds a larger one takes 1 - 2 / (1 + e^(2z)),
+//    two more MUFU operations per score.
 //  * the bias. Linear in the key up to the query, so it is one packed FMA for
 //    two scores; |i - j| itself only near the diagonal and in the prefix.
-// The mask tests, the block lists and the loads stay as in kClassic. In the
-// backward an item is a key tile of a key/value head: it walks the query tiles
-// of every query head that shares it, so dK and dV of the group add up in TMEM,
-// in a fixed order.
+// Masks are words of 32 keys, made once per block and warp; blocks that no mask
+// reaches run code without them (tests that are predicated off still take issue
+// slots). The forward's rows go through one streaming pass against the maximum
+// they have so far, the diagonal block first (softmax_general). In the backward an
+// item is a key tile of a key/value head: it walks the query tiles of every query
+// head that shares it, so dK and dV of the group add up in TMEM, in a fixed order.
+// Roundings: P to bf16 before P.V and P^T dO, dS to bf16 before dK and dQ, delta
+// from O as stored (exact for one key tile); sums, maxima, lse, dQ's accumulator
+// and everything between are fp32.
+// What bounds them, 1 x 12 x 8192 (us, forward | backward):
+//    plain causal kernels 230 | 395; MODE without cap and bias 185 | 343; bias
+//    200 | 358; cap 258 | 428; both 259 | 453 (398 and 569 TFLOP/s).
+//  Forward: the latency of two softmax warps a scheduler. Without any arithmetic
+//  (raw scores packed as P) it takes 123 us; with it a warp spends 4,100 of 5,080
+//  clocks a block on its 64 pairs of scores a row, where the FMA pipe needs 1,024
+//  and two warps share a scheduler, and 830 waiting for the next block's scores,
+//  which are issued when it has finished with this block's. Splitting blocks in
+//  halves to issue them earlier halves that wait, but MMAs of 64 columns and twice
+//  the handshakes cost more (293 us against 279).
+//  Backward: shared memory. Without any arithmetic it takes 309 us, 1,510 clocks a
+//  tile of 128 x 64; the MMAs' operands (88 KB), dS^T, the Q and dO tiles and dQ's
+//  way out are 152 KB a tile, 1,190 clocks at 128 bytes a clock.
 #include <algorithm>
 #include <atomic>
 #include <mutex>
@@ -204,15 +222,6 @@ __device__ __forceinline__ void sched_finish(unsigned* sched) {
   {0.999993085861206f, -0.3329806327819824f, 0.13036808371543884f, -0.04481752589344978f, \
    0.009036410599946976f}
 
-GPTB200_DEV float2 tanh_small2(float2 z) {
-  constexpr float c[5] = GPTB200_TANH_COEFS;
-  const float2 u = fmul2(z, z);
-  float2 a = ffma2(u, make_float2(c[4], c[4]), make_float2(c[3], c[3]));
-  a = ffma2(u, a, make_float2(c[2], c[2]));
-  a = ffma2(u, a, make_float2(c[1], c[1]));
-  a = ffma2(u, a, make_float2(c[0], c[0]));
-  return fmul2(z, a);
-}
 // Any z: 1 - 2 / (1 + e^(2z)), an absolute error of a few 2^-24.
 GPTB200_DEV float tanh_any(float z) {
   return fmaf(-2.f, __fdividef(1.f, 1.f + ex2(2.f * kLog2e * z)), 1.f);
@@ -1063,7 +1072,10 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
   // The same for modified scores: one streaming pass per block against the
   // maximum that the rows have so far (Score::stream). Blocks with masked
   // places, a row whose scores outgrow its maximum and scores past the short
-  // form of tanh take steps instead, from the raw scores still in TMEM.
+  // form of tanh take steps instead, from the raw scores still in TMEM. The pass
+  // is a loop over 32 keys and no longer code: all 128 keys unrolled (15 KB) or 64
+  // take 268 to 283 us at 1 x 12 x 8192, this 259 (279 with TMEM loads that nothing
+  // covers).
   [[maybe_unused]] auto softmax_general = [&]() {
     const int x = (warp - kSoftmaxWarp) >> 2;
     const int quad = warp & 3;
@@ -2449,16 +2461,17 @@ static AttnParams score_params(const gptb200_score_attention* a) {
 // Whether a launch walks the items of all heads by falling weight instead of
 // head by head. By weight the last items are light and every SM ends at about
 // the same time; head by head the tiles that the items of a head share stay in
-// L2. So: by weight while the shared tiles of all heads (`bytes`) fit, and
-// longer for capped scores, which compute more per byte. Measured at 12 heads,
-// capped and biased | without either (us, by weight / head by head):
-//   forward  1 x 8192: 299 / 370 | 170 / 215;   128 x 1024: 872 / 1142 | 486 / 463
-//   backward 1 x 8192: 537 / 655 | 343 / 391;   48 x 1024:  567 / 623  | 504 / 462
-//   backward 16 x 8192: 9660 / 9213 | 7502 / 5887
-static int by_weight(const gptb200_score_attention* a, int64_t bytes, int64_t plain_limit,
-                     int64_t cap_limit) {
-  return bytes <= (a->softcap > 0.f ? cap_limit : plain_limit) << 20;
-}
+// L2. So: by weight while the shared tiles of all heads (`bytes`) fit, and in the
+// backward longer for capped scores, which compute more per byte. Measured at 12
+// heads (us, by weight / head by head; MB of shared tiles), capped and biased |
+// without either:
+//   forward  25 MB (1 x 8192): 260 / 331 | 185 / 235;  101 MB (4 x 8192): 945 / 1011
+//            | 690 / 718;  151 MB (48 x 1024): 257 / 259 | 206 / 192;  403 MB (128 x
+//            1024): 707 / 662 | 559 / 477
+//   backward 25 MB: 457 / 525 | 343 / 397;  101 MB: 1830 / 1834 | 1442 / 1390;
+//            151 MB: 553 / 619 | 517 / 476;  403 MB: 1477 / 1596 | 1374 / 1238 at
+//            128 x 1024, 8836 / 7381 | 7831 / 6131 at 16 x 8192
+static int by_weight(int64_t bytes, int64_t limit) { return bytes <= limit << 20; }
 
 // One persistent launch: the shared-memory attribute (set once per kernel and
 // device) and one CTA per SM or item.
@@ -2521,7 +2534,7 @@ static int score_forward(const gptb200_score_attention* a, float* o32, cudaStrea
   p.sched = sched_slot(0);
   if (!p.sched) return GPTB200_EUNSUPPORTED;
   // K and V of every head
-  p.by_weight = by_weight(a, a->batch * a->kv_heads * a->seq * 2 * HD * 2, 160, 512);
+  p.by_weight = by_weight(a->batch * a->kv_heads * a->seq * 2 * HD * 2, 128);
   return score_mode(a, [&](auto mode) {
     constexpr int MODE = decltype(mode)::value;
     return p.seg ? score_fwd_launch<true, MODE>(p, m, st) : score_fwd_launch<false, MODE>(p, m, st);
@@ -2603,7 +2616,7 @@ extern "C" int gptb200_score_attention_bwd(const gptb200_score_attention* a, con
   p.rcos = reinterpret_cast<const bf16*>(rope_cos);
   p.rsin = reinterpret_cast<const bf16*>(rope_sin);
   // Q and dO of every head
-  p.by_weight = by_weight(a, rows * 2 * HD * 2, 64, 512);
+  p.by_weight = by_weight(rows * 2 * HD * 2, a->softcap > 0.f ? 256 : 64);
   const int e = score_mode(a, [&](auto mode) {
     constexpr int MODE = decltype(mode)::value;
     return p.seg ? score_bwd_launch<true, MODE>(p, m, st) : score_bwd_launch<false, MODE>(p, m, st);

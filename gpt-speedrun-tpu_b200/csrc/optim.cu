@@ -344,8 +344,9 @@ __global__ void __launch_bounds__(1024) adamw_end_kernel(const double* __restric
 // its inputs. Moments enter the update unrounded; every operation up to the
 // codes is rounded by itself (no contraction), so that a restatement with
 // separate operations yields the same codes.
-// Bound by HBM: parameters, gradient, codes and the bf16 copy move 18.06 bytes
-// per parameter, where fp32 moments need 30.
+// Parameters, gradient, codes and the bf16 copy move 18.06 bytes per parameter,
+// where fp32 moments need 30: 344 us of HBM at 124.7 M parameters, of 507 measured
+// (685 with fp32 moments); the rest is instructions (below).
 constexpr int kQBlock = 64;
 
 // The finalizer of MurmurHash3 (32 bits; Appleby, public domain).
@@ -384,8 +385,8 @@ __device__ __forceinline__ uint32_t bytes4(const uint32_t* c) {
 
 // Eight lanes share a block, eight elements each: what a lane does once (group
 // lookup, addresses, exponents, shuffles) is spread over eight updates, since
-// the arithmetic, about 70 instructions an element, already fills two thirds of
-// the issue slots that the memory traffic leaves. The quotient m / r is the only
+// the arithmetic, 106 instructions an element, half of them integer, fills three
+// quarters of the issue slots of the whole run. The quotient m / r is the only
 // operation that is not rounded to nearest (its error, 2^-22 of the update, is
 // far below half a unit of the parameter).
 constexpr int kQLane = 8;
@@ -396,8 +397,8 @@ struct QuadGroup {
   float lr, eps, wd;
 };
 
-// Four blocks of 256 threads on an SM (64 registers), measured against 3 and 5 at
-// 124.7 M parameters: 531, 545 and 566 us.
+// Four blocks of 256 threads on an SM (64 registers): 507 us at 124.7 M parameters,
+// 4.4 TB/s; three blocks (80) and five (48, with spills) take 530 both.
 __global__ void __launch_bounds__(256, 4) adamw8_kernel(
     float* __restrict__ p, uint8_t* __restrict__ mq, uint8_t* __restrict__ me,
     uint8_t* __restrict__ vq, uint8_t* __restrict__ ve, const float* __restrict__ g, int64_t begin,
