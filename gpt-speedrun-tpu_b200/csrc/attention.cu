@@ -57,8 +57,8 @@
 // from O as stored (exact for one key tile); sums, maxima, lse, dQ's accumulator
 // and everything between are fp32.
 // What bounds them, 1 x 12 x 8192 (us, forward | backward):
-//    plain causal kernels 230 | 395; MODE without cap and bias 185 | 343; bias
-//    200 | 358; cap 258 | 428; both 259 | 453 (398 and 569 TFLOP/s).
+//    plain causal kernels 230 | 395; MODE without cap and bias 181 | 343; bias
+//    192 | 358; cap 238 | 429; both 259 | 454 (398 and 568 TFLOP/s).
 //  Forward: the latency of two softmax warps a scheduler. Without any arithmetic
 //  (raw scores packed as P) it takes 123 us; with it a warp spends 4,100 of 5,080
 //  clocks a block on its 64 pairs of scores a row, where the FMA pipe needs 1,024
@@ -240,10 +240,10 @@ GPTB200_DEV float fmax3_abs(float a, float b, float c) {
 template <int MODE>
 struct Score {
   static constexpr bool CAP = (MODE & kCap) != 0, BIAS = (MODE & kBias) != 0;
-  // A row keeps its maximum m until a score passes it by this many powers of
-  // two: bf16, the fp32 sums and O lose nothing below that, and exp2 is far
-  // from overflow.
-  static constexpr float kSlack = 40.f;
+  // A row keeps its maximum m until a block's probabilities against it add up to
+  // more than this: bf16, the fp32 sums and O lose nothing below that, and exp2 is
+  // far from overflow.
+  static constexpr float kSlack = 0x1p40f;
   float z_per_s;  // tanh's argument per raw score
   float out;      // s' log2(e) per tanh, or per raw score
   float slope2;   // slope * log2(e)
@@ -278,8 +278,8 @@ struct Score {
   // Without masks, keys before the query, against the maximum m: arithmetic (FMA
   // pipe) and exponentials (MUFU) of different columns overlap, with nothing to
   // wait for in between. 16 columns at a time; the callers have the next ones on
-  // their way from TMEM meanwhile. top and far collect the largest exponent and
-  // raw score squared; the caller discards the block if they do not do. The tanh's
+  // their way from TMEM meanwhile. far collects the largest raw score squared; the
+  // caller discards the block if it, or the sum of the probabilities, does not do. The tanh's
   // argument is not formed: its factor is in the coefficients (stream_coefs). The
   // bias, slope (key - query), with -m folded in, runs in four pairs that step by
   // eight keys: one addition for two scores. `at`: first key - query.
@@ -300,7 +300,7 @@ struct Score {
                     : both(-m);
   }
   GPTB200_DEV void stream(const uint32_t (&v)[16], const float2 (&k)[5], float2 (&off)[4],
-                          uint32_t* pk, float2 (&acc)[2], float& top, float& far) const {
+                          uint32_t* pk, float2 (&acc)[2], float& far) const {
 #pragma unroll
     for (int i = 0; i < 16; i += 8) {
       float2 s[4], y[4];
@@ -324,7 +324,6 @@ struct Score {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if (BIAS) off[q] = fadd2(off[q], both(8.f * slope2));
-        top = fmax3(top, y[q].x, y[q].y);
         y[q] = make_float2(ex2(y[q].x), ex2(y[q].y));
         acc[q & 1] = fadd2(acc[q & 1], y[q]);
         pk[i / 2 + q] = pack_bf16x2(y[q].x, y[q].y);
@@ -332,9 +331,9 @@ struct Score {
     }
   }
   // Whether a block that went through stream() has to be done in steps.
-  GPTB200_DEV bool discard(float top, float far) const {
+  GPTB200_DEV bool discard(float sum, float far) const {
     // (m = -inf lifts everything to +inf)
-    return __any_sync(0xffffffffu, !(top <= kSlack) || (CAP && !(far <= far_max)));
+    return __any_sync(0xffffffffu, !(sum <= kSlack) || (CAP && !(far <= far_max)));
   }
 
   // Modified scores in place of the raw ones, in log2, and their maximum; those
@@ -1137,7 +1136,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
         bool rescale = false;
         bool steps = diag || segmask || ahead;
         if (!steps) {
-          float top = -INFINITY, far = 0.f;
+          float far = 0.f;
           float2 k[5], off[4];
           if constexpr ((MODE & kCap) != 0) score.stream_coefs(k);
           uint32_t va[16], vb[16];
@@ -1147,16 +1146,17 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
             score.stream_bias(at0 + (float)(32 * w), m_used, off);
             tmem_wait_ld();
             tmem_ld16_nw(aS + 32 * w + 16, vb);
-            score.stream(va, k, off, pk, acc, top, far);
+            score.stream(va, k, off, pk, acc, far);
             tmem_wait_ld();
             if (w < 3) tmem_ld16_nw(aS + 32 * w + 32, va);
-            score.stream(vb, k, off, pk + 8, acc, top, far);
+            score.stream(vb, k, off, pk + 8, acc, far);
             if (w == 0 && !previous_done()) break;
             tmem_st8_nw(aP + 16 * w, pk);
             tmem_st8_nw(aP + 16 * w + 8, pk + 8);
           }
           if (!ok) break;
-          steps = score.discard(top, far);
+          const float2 both = fadd2(acc[0], acc[1]);
+          steps = score.discard(both.x + both.y, far);
         }
         if (steps) {
           // Masks, a new maximum or tanh's long form: modified scores go back
