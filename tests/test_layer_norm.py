@@ -111,6 +111,22 @@ def test_many_rows_accumulate(cuda):
     assert torch.equal(twice, once + once)  # fixed order: the second call adds the same bits
 
 
+# For every split of a row over lanes and warps, more rows than six turns of a full
+# grid take, and a last turn that is not full: rows in flight wrap around.
+TURNS = [(14301, 512), (11003, 768), (7201, 1024), (3601, 2048), (1801, 4096), (903, 8192), (701, 8200),
+         (14301, 129), (3603, 771), (1803, 1999), (901, 4095), (703, 6001), (451, 8193)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,d", TURNS)
+def test_many_turns_at_every_split(cuda, rows, d, dtype):
+    x, w, b, dy, res = _inputs(rows, d, dtype, seed=13)
+    for residual in (True, False):
+        r = res if residual else None
+        _check(_run(cuda, x, w, b, dy, r, cols=residual), _formula(x, w, b, dy, r), x, w, b, dy, dtype, r)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_rows_far_from_zero_and_constant_rows(cuda, dtype):
