@@ -70,9 +70,11 @@
 //  tile of 128 x 64; the MMAs' operands (88 KB), dS^T, the Q and dO tiles and dQ's
 //  way out are 152 KB a tile, 1,190 clocks at 128 bytes a clock.
 #include <algorithm>
-#include <atomic>
 #include <mutex>
+#include <new>
 #include <type_traits>
+#include <unordered_map>
+#include <vector>
 
 #include "common.cuh"
 
@@ -191,11 +193,11 @@ __device__ __forceinline__ int2 seg_range(const int2* tab, int nch, int c, int n
 // out head by head, heaviest first within a head, so the items in flight at
 // once cover a few heads whose K/V or Q/dO tiles come from DRAM about once and
 // are then served from L2, and a CTA that finishes early takes more work).
-// The counters live in a small device array of slots; each launch gets its own
-// slot (so launches that overlap on the GPU do not share one) and the last CTA
-// to finish puts the slot back to zero.
-constexpr int kSchedSlots = 64;
-__device__ unsigned g_attn_sched[2][kSchedSlots][2];
+// The counters live in a device array of slots. Launches that may overlap on the
+// GPU have different slots (sched_slot), and the last CTA of a launch to finish
+// puts its slot back to zero.
+constexpr int kSchedSlots = 1 << 16;
+__device__ unsigned g_attn_sched[kSchedSlots][2];
 
 // Called by the whole producer warp: the next item index (lane 0 fetches).
 __device__ __forceinline__ int next_item(unsigned* sched, int lane) {
@@ -2171,26 +2173,91 @@ int attention_read_error(int clear) {
 }
 
 // ------------------------------------------------------------------ host
-// A counter slot of g_attn_sched for one launch of kernel `which` (0 forward,
-// 1 backward) on the current device: slots rotate per device, so up to
-// kSchedSlots launches may be in flight at once.
-static unsigned* sched_slot(int which) {
-  static unsigned* base[64] = {};
-  static std::atomic<unsigned> next[64][2];
-  static std::mutex mu;
+// The counter slots of one device. Launches on a stream run one after the other,
+// so a stream keeps one slot for all of its launches; streams go by their ids,
+// which no two of a process have in common. A captured launch runs wherever its
+// graph is launched, beside any stream's launches and beside other branches of the
+// graph, so each has a slot to itself until the graph and everything instantiated
+// from it are gone (a graph does not run beside itself).
+struct SchedSlots {
+  std::mutex mu;
+  unsigned* base = nullptr;
+  int used = 0;                                // slots [0, used) have been handed out
+  std::vector<int> free;                       // of these, back from graphs
+  std::unordered_map<unsigned long long, int> of_stream;
+
+  int take() {  // -1: none is left
+    if (!free.empty()) {
+      const int k = free.back();
+      free.pop_back();
+      return k;
+    }
+    return used < kSchedSlots ? used++ : -1;
+  }
+};
+struct GraphSlot {
+  SchedSlots* owner;
+  int slot;
+};
+static void CUDART_CB return_slot(void* p) {  // a graph's last reference has gone
+  GraphSlot* g = reinterpret_cast<GraphSlot*>(p);
+  {
+    std::lock_guard<std::mutex> lock(g->owner->mu);
+    g->owner->free.push_back(g->slot);
+  }
+  delete g;
+}
+
+// The counter slot of a launch on `st`: 0, or an error (without a slot left:
+// 65,536 streams and captured launches at a time).
+static int sched_slot(cudaStream_t st, unsigned** slot) try {
+  static SchedSlots* const devices = new SchedSlots[64];  // graphs may outlive static objects
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 64) return nullptr;
-  if (!base[dev]) {
-    std::lock_guard<std::mutex> lock(mu);
-    if (!base[dev]) {
+  if (dev >= 64) return GPTB200_EUNSUPPORTED;
+  SchedSlots& d = devices[dev];
+  cudaStreamCaptureStatus status;
+  cudaGraph_t graph = nullptr;
+  unsigned long long id = 0;
+  cudaError_t e = cudaStreamGetCaptureInfo(st, &status, &id, &graph);
+  if (e == cudaSuccess && status != cudaStreamCaptureStatusActive) e = cudaStreamGetId(st, &id);
+  if (e != cudaSuccess) return -static_cast<int>(e);
+  int k;
+  {
+    std::lock_guard<std::mutex> lock(d.mu);
+    if (!d.base) {
       void* ptr = nullptr;
-      if (cudaGetSymbolAddress(&ptr, g_attn_sched) != cudaSuccess) return nullptr;
-      base[dev] = reinterpret_cast<unsigned*>(ptr);
+      e = cudaGetSymbolAddress(&ptr, g_attn_sched);
+      if (e != cudaSuccess) return -static_cast<int>(e);
+      d.free.reserve(kSchedSlots);  // return_slot has no way to report a failure
+      d.base = reinterpret_cast<unsigned*>(ptr);
+    }
+    if (status == cudaStreamCaptureStatusActive) {
+      k = d.take();
+    } else {
+      const auto known = d.of_stream.find(id);
+      k = known != d.of_stream.end() ? known->second : d.take();
+      if (k >= 0 && known == d.of_stream.end()) d.of_stream.emplace(id, k);
     }
   }
-  const unsigned k = next[dev][which].fetch_add(1) % kSchedSlots;
-  return base[dev] + ((size_t)which * kSchedSlots + k) * 2;
+  if (k < 0) return GPTB200_EUNSUPPORTED;
+  *slot = d.base + 2 * (size_t)k;
+  if (status != cudaStreamCaptureStatusActive) return 0;
+  GraphSlot* g = new GraphSlot{&d, k};
+  cudaUserObject_t kept;
+  e = cudaUserObjectCreate(&kept, g, return_slot, 1, cudaUserObjectNoDestructorSync);
+  if (e != cudaSuccess) {
+    return_slot(g);
+    return -static_cast<int>(e);
+  }
+  e = cudaGraphRetainUserObject(graph, kept, 1, cudaGraphUserObjectMove);
+  if (e != cudaSuccess) {
+    cudaUserObjectRelease(kept, 1);  // the last reference: returns the slot
+    return -static_cast<int>(e);
+  }
+  return 0;
+} catch (const std::bad_alloc&) {
+  return -static_cast<int>(cudaErrorMemoryAllocation);
 }
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -2295,8 +2362,9 @@ extern "C" int gptb200_attention_fwd(const void* q, const void* k, const void* v
   p.ost = o_stride_t;
   p.lse = lse;
   p.seg = segment_ids;
-  p.sched = sched_slot(0);
-  if (!p.sched) return GPTB200_EUNSUPPORTED;
+  auto st = reinterpret_cast<cudaStream_t>(stream);
+  const int no_slot = sched_slot(st, &p.sched);
+  if (no_slot) return no_slot;
   static bool cfg[64][2] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -2377,8 +2445,8 @@ extern "C" int gptb200_attention_bwd(const void* q, const void* k, const void* v
   p.rcos = reinterpret_cast<const bf16*>(rope_cos);
   p.rsin = reinterpret_cast<const bf16*>(rope_sin);
   p.seg = segment_ids;
-  p.sched = sched_slot(1);
-  if (!p.sched) return GPTB200_EUNSUPPORTED;
+  const int no_slot = sched_slot(st, &p.sched);
+  if (no_slot) return no_slot;
   static bool cfg[64][4] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -2531,8 +2599,8 @@ static int score_forward(const gptb200_score_attention* a, float* o32, cudaStrea
       !make_map4(&m.k, a->k, p.B, p.KVH, p.T, ks[0], ks[1], ks[2], FK) ||
       !make_map4(&m.v, a->v, p.B, p.KVH, p.T, ks[0], ks[1], ks[2], FK))
     return GPTB200_ESHAPE;
-  p.sched = sched_slot(0);
-  if (!p.sched) return GPTB200_EUNSUPPORTED;
+  const int no_slot = sched_slot(st, &p.sched);
+  if (no_slot) return no_slot;
   // K and V of every head
   p.by_weight = by_weight(a->batch * a->kv_heads * a->seq * 2 * HD * 2, 128);
   return score_mode(a, [&](auto mode) {
@@ -2586,9 +2654,9 @@ extern "C" int gptb200_score_attention_bwd(const gptb200_score_attention* a, con
       !make_map4(&m.g, dout, p.B, p.H, p.T, dout_stride[0], dout_stride[1], dout_stride[2], BQ) ||
       !make_dq_map(&m.dq, dq_acc, p.B * p.H, p.T))
     return GPTB200_ESHAPE;
-  p.sched = sched_slot(1);
-  if (!p.sched) return GPTB200_EUNSUPPORTED;
   auto st = reinterpret_cast<cudaStream_t>(stream);
+  const int no_slot = sched_slot(st, &p.sched);
+  if (no_slot) return no_slot;
   // delta = sum dO O from the stored O carries its rounding to bf16 (2^-9 |dO| |O|)
   // into dS = P (dP - delta) of the whole row. Where a row has few keys, one of
   // them tends to hold most of P, dP - delta is small for it and the rounding
