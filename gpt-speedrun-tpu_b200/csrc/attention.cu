@@ -242,10 +242,16 @@ GPTB200_DEV float fmax3_abs(float a, float b, float c) {
 template <int MODE>
 struct Score {
   static constexpr bool CAP = (MODE & kCap) != 0, BIAS = (MODE & kBias) != 0;
-  // A row keeps its maximum m until a block's probabilities against it add up to
-  // more than this: bf16, the fp32 sums and O lose nothing below that, and exp2 is
-  // far from overflow.
-  static constexpr float kSlack = 0x1p40f;
+  // A row keeps its reference m until a block's probabilities against it add up to
+  // more than this: 128 keys at the 2^8 that the plain kernels allow one. bf16 and
+  // the fp32 sums lose nothing below that. O before its division by l is at most the
+  // sum of the probabilities times max |v|: finite for |v| up to 2^113 / blocks.
+  static constexpr float kSlack = 0x1p15f;
+  // A reference is set this far (log2) above the maximum that asks for it, so that
+  // later keys seldom reach the limit: a row's first block is its diagonal one, and
+  // its first rows see few keys. Without it 10% more time at 8 x 12 x 1024 (general
+  // 45.0 us, with 6 41.7, 8 40.1, 10 and 12 39.7); smaller probabilities are as exact.
+  static constexpr float kRoom = 12.f;
   float z_per_s;  // tanh's argument per raw score
   float out;      // s' log2(e) per tanh, or per raw score
   float slope2;   // slope * log2(e)
@@ -277,7 +283,7 @@ struct Score {
     }
   }
 
-  // Without masks, keys before the query, against the maximum m: arithmetic (FMA
+  // Without masks, keys before the query, against the reference m: arithmetic (FMA
   // pipe) and exponentials (MUFU) of different columns overlap, with nothing to
   // wait for in between. 16 columns at a time; the callers have the next ones on
   // their way from TMEM meanwhile. far collects the largest raw score squared; the
@@ -1071,8 +1077,8 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
     }
   };
   // The same for modified scores: one streaming pass per block against the
-  // maximum that the rows have so far (Score::stream). Blocks with masked
-  // places, a row whose scores outgrow its maximum and scores past the short
+  // reference that the rows have so far (Score::stream). Blocks with masked
+  // places, a row whose scores outgrow its reference and scores past the short
   // form of tanh take steps instead, from the raw scores still in TMEM. The pass
   // is a loop over 32 keys and no longer code: all 128 keys unrolled (15 KB) or 64
   // take 268 to 283 us at 1 x 12 x 8192, this 259 (279 with TMEM loads that nothing
@@ -1186,7 +1192,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
           // whose max stays rescales by 1, one that has seen no key yet too.
           rescale = __any_sync(0xffffffffu, top > m_used + 8.0f);
           if (rescale) {
-            const float m_new = fmaxf(m_used, top);
+            const float m_new = top > m_used ? top + Score<MODE>::kRoom : m_used;
             alpha = m_new == -INFINITY ? 1.f : ex2(m_used - m_new);
             m_used = m_new;
           }

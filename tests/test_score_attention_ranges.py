@@ -1,0 +1,42 @@
+"""Score-modified attention at the ends of its inputs' ranges, against the formula in
+64 bits. Formula and elementwise tolerances are those of test_score_attention."""
+
+import pytest
+import torch
+
+from rig_b200 import kernels
+from test_score_attention import _check, _formula, _inputs, _run
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (0.0, True), (50.0, False), (50.0, True)])
+@pytest.mark.parametrize("power", [0, 108, -100])
+def test_far_keys_above_the_near_ones(cuda, cap, bias, power):
+    """Keys of the first tile whose scores lie 0 to 58 bits above those of a row's own
+    tile, which no mask reaches: the row's sums start against a reference that they
+    outgrow. Values of 2^108 and 2^-100 too, which the results can hold: an output is
+    at most max |v| < 2^111, so nothing on the way may reach 2^17 times it. The
+    incoming gradient moves against them (do.v has to be finite), and as everything
+    is linear in either, the results go back to the formula's by powers of two."""
+
+    t = 520
+    q, k, v, do = (x.to(cuda) for x in _inputs(1, 2, 1, t, 21, 1.0))
+    lift = torch.tensor([0.0, 1.0, 1.7, 2.6, 3.2, 4.0, 5.0], device=cuda)  # 8 nats each
+    row = torch.arange(t, device=cuda) // 32 % 7  # alike within a warp, which decides as one
+    q = (q.float() / 4 + lift[row][None, None, :, None]).bfloat16()
+    k = k.float() / 4
+    k[:, :, :128] += 1.0
+    k = k.bfloat16()
+    # small slopes: the bias is there, but does not undo the lift
+    slopes = torch.tensor([2.0 ** -9, 2.0 ** -7], device=cuda) if bias else None
+    want, tol, want_lse = _formula(q, k, v, do, 0.125, cap, slopes, None, None)
+    first, own = (torch.logsumexp((0.125 * q.double() @ k.double().transpose(-1, -2))[..., 256:, w], -1)
+                  for w in (slice(0, 128), slice(256, 384)))
+    assert (first - own).max() > 40 and (first - own).min() < 8  # nats
+    size, back = 2.0 ** power, 2.0 ** (-power // 4)
+    got, lse = _run(q, k, (v.double() * size).bfloat16(), (do.double() * back).bfloat16(), scale=0.125,
+                    softcap=cap, slopes=slopes)
+    got = {n: x.double() / (size if n == "o" else back if n == "dv" else size * back)
+           for n, x in got.items()}
+    assert all(torch.isfinite(x).all() for x in got.values())
+    _check(got, lse, want, tol, want_lse)
