@@ -42,8 +42,8 @@
 // gradients). What they add to the softmax warps:
 //  * tanh. The exponentials hold the MUFU pipe for 8 clocks a score (of a warp's
 //    32 rows), so tanh runs on the FMA pipe beside it, 8 clocks for a score too:
-//    z P(z^2) with five terms, relative error 7e-6, where a warp's scores have
-//    |z| <= 1; only a warp that holds a larger one takes 1 - 2 / (1 + e^(2z)),
+//    z P(z^2) with five terms, relative error 7e-6 (seven and 5e-8 for caps above
+//    kShortCap), where a warp's scores have |z| <= 1; only a warp that holds a larger one takes 1 - 2 / (1 + e^(2z)),
 //    two more MUFU operations per score.
 //  * the bias. Linear in the key up to the query, so it is one packed FMA for
 //    two scores; |i - j| itself only near the diagonal and in the prefix.
@@ -87,8 +87,14 @@ constexpr int HD = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Score modes of the kernels (bits of a MODE > kClassic: 1 general, 2 cap, 4 bias).
-enum { kClassic = 0, kGeneral = 1, kCap = 2, kBias = 4 };
+// Score modes of the kernels (bits of a MODE > kClassic: 1 general, 2 cap, 4 bias,
+// 8 a cap above kShortCap).
+enum { kClassic = 0, kGeneral = 1, kCap = 2, kBias = 4, kWide = 8 };
+// An error of tanh counts cap times in a score. Its five terms (7e-6 relative) are up
+// to 7e-4 of a probability at this cap, a third of the rounding to bf16; larger caps
+// take seven (5e-8). 1 x 12 x 8192 capped (us, forward | backward): 238 | 429 with
+// five, 278 | 443 with seven.
+constexpr float kShortCap = 128.f;
 
 struct AttnParams {
   int B, H, T;         // H: query heads
@@ -218,15 +224,27 @@ __device__ __forceinline__ void sched_finish(unsigned* sched) {
 }
 
 // ------------------------------------------------------------------ scores
-// tanh(z) / z in u = z^2 on |z| <= 1: minimax in relative error (7e-6) by
+// tanh(z) / z in u = z^2 on |z| <= 1: minimax in relative error (7e-6 and 5e-8) by
 // reweighted least squares over Chebyshev points.
 #define GPTB200_TANH_COEFS \
   {0.999993085861206f, -0.3329806327819824f, 0.13036808371543884f, -0.04481752589344978f, \
    0.009036410599946976f}
+#define GPTB200_TANH_WIDE_COEFS \
+  {0.9999999403953552f, -0.33332839608192444f, 0.13325203955173492f, -0.053457025438547134f, \
+   0.02028997428715229f, -0.006203373894095421f, 0.0010410209652036428f}
 
-// Any z: 1 - 2 / (1 + e^(2z)), an absolute error of a few 2^-24.
+// Any z: 1 - 2 / (1 + e^(2z)), an absolute error of a few 2^-24. WIDE: that on |z| > 1
+// only, the seven terms below, a few 2^-24 of the result.
+template <bool WIDE>
 GPTB200_DEV float tanh_any(float z) {
-  return fmaf(-2.f, __fdividef(1.f, 1.f + ex2(2.f * kLog2e * z)), 1.f);
+  const float far = fmaf(-2.f, __fdividef(1.f, 1.f + ex2(2.f * kLog2e * z)), 1.f);
+  if constexpr (!WIDE) return far;
+  constexpr float c[7] = GPTB200_TANH_WIDE_COEFS;
+  const float u = z * z;
+  float a = c[6];
+#pragma unroll
+  for (int e = 5; e >= 0; --e) a = fmaf(u, a, c[e]);
+  return u <= 1.f ? z * a : far;
 }
 
 GPTB200_DEV float fmax3_abs(float a, float b, float c) {
@@ -242,6 +260,8 @@ GPTB200_DEV float fmax3_abs(float a, float b, float c) {
 template <int MODE>
 struct Score {
   static constexpr bool CAP = (MODE & kCap) != 0, BIAS = (MODE & kBias) != 0;
+  static constexpr bool WIDE = (MODE & kWide) != 0;
+  static constexpr int TERMS = WIDE ? 7 : 5;
   // A row keeps its reference m until a block's probabilities against it add up to
   // more than this: 128 keys at the 2^8 that the plain kernels allow one. bf16 and
   // the fp32 sums lose nothing below that. O before its division by l is at most the
@@ -255,29 +275,29 @@ struct Score {
   float z_per_s;  // tanh's argument per raw score
   float out;      // s' log2(e) per tanh, or per raw score
   float slope2;   // slope * log2(e)
-  float far_max;  // the largest raw score squared with |z| <= 1
+  float far_max;  // the largest raw score squared (WIDE: z squared) with |z| <= 1
   GPTB200_DEV Score(const AttnParams& p, float slope2_) : slope2(slope2_) {
     z_per_s = CAP ? p.scale / p.cap : 1.f;
     out = (CAP ? p.cap : p.scale) * kLog2e;
     // below 2^-13 the ninth power in stream_coefs may underflow: never stream
-    far_max = z_per_s < 0x1p-13f ? -1.f : 1.f / (z_per_s * z_per_s);
+    far_max = WIDE ? 1.f : z_per_s < 0x1p-13f ? -1.f : 1.f / (z_per_s * z_per_s);
   }
   static GPTB200_DEV float2 both(float x) { return make_float2(x, x); }
   static GPTB200_DEV float2 pair(const uint32_t (&v)[32], int i) {
     return make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
   }
-  // The polynomial's coefficients times `out`.
-  GPTB200_DEV void coefs(float2 (&k)[5]) const {
-    constexpr float c[5] = GPTB200_TANH_COEFS;
+  // The polynomial's coefficients, times `by`.
+  static GPTB200_DEV void coefs(float2 (&k)[TERMS], float by) {
+    constexpr float c[5] = GPTB200_TANH_COEFS, w[7] = GPTB200_TANH_WIDE_COEFS;
 #pragma unroll
-    for (int u = 0; u < 5; ++u) k[u] = both(out * c[u]);
+    for (int u = 0; u < TERMS; ++u) k[u] = both(by * (WIDE ? w[u] : c[WIDE ? 0 : u]));
   }
   // Four pairs at a time, so that their dependent steps interleave.
-  static GPTB200_DEV void poly4(const float2 (&k)[5], const float2 (&u)[4], float2 (&a)[4]) {
+  static GPTB200_DEV void poly4(const float2 (&k)[TERMS], const float2 (&u)[4], float2 (&a)[4]) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) a[q] = ffma2(u[q], k[4], k[3]);
+    for (int q = 0; q < 4; ++q) a[q] = ffma2(u[q], k[TERMS - 1], k[TERMS - 2]);
 #pragma unroll
-    for (int e = 2; e >= 0; --e) {
+    for (int e = TERMS - 3; e >= 0; --e) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) a[q] = ffma2(u[q], a[q], k[e]);
     }
@@ -288,10 +308,12 @@ struct Score {
   // wait for in between. 16 columns at a time; the callers have the next ones on
   // their way from TMEM meanwhile. far collects the largest raw score squared; the
   // caller discards the block if it, or the sum of the probabilities, does not do. The tanh's
-  // argument is not formed: its factor is in the coefficients (stream_coefs). The
+  // argument is not formed: its factor is in the coefficients (stream_coefs; WIDE forms
+  // it, as the factor's powers would underflow). The
   // bias, slope (key - query), with -m folded in, runs in four pairs that step by
   // eight keys: one addition for two scores. `at`: first key - query.
-  GPTB200_DEV void stream_coefs(float2 (&k)[5]) const {
+  GPTB200_DEV void stream_coefs(float2 (&k)[TERMS]) const {
+    if constexpr (WIDE) return coefs(k, out);
     constexpr float c[5] = GPTB200_TANH_COEFS;
     float f = out * z_per_s;
 #pragma unroll
@@ -307,7 +329,7 @@ struct Score {
                                   fmaf(slope2, at + (float)(2 * q + 1), -m))
                     : both(-m);
   }
-  GPTB200_DEV void stream(const uint32_t (&v)[16], const float2 (&k)[5], float2 (&off)[4],
+  GPTB200_DEV void stream(const uint32_t (&v)[16], const float2 (&k)[TERMS], float2 (&off)[4],
                           uint32_t* pk, float2 (&acc)[2], float& far) const {
 #pragma unroll
     for (int i = 0; i < 16; i += 8) {
@@ -318,7 +340,10 @@ struct Score {
       if constexpr (CAP) {
         float2 u[4], a[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) u[q] = fmul2(s[q], s[q]);
+        for (int q = 0; q < 4; ++q) {
+          if constexpr (WIDE) s[q] = fmul2(s[q], both(z_per_s));
+          u[q] = fmul2(s[q], s[q]);
+        }
         poly4(k, u, a);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -359,10 +384,10 @@ struct Score {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
         v[i] = __float_as_uint(
-            biased(out * tanh_any(__uint_as_float(v[i]) * z_per_s), at + (float)i));
+            biased(out * tanh_any<WIDE>(__uint_as_float(v[i]) * z_per_s), at + (float)i));
     } else {
-      float2 k[5];
-      if constexpr (CAP) coefs(k);
+      float2 k[TERMS];
+      if constexpr (CAP) coefs(k, out);
 #pragma unroll
       for (int i = 0; i < 32; i += 8) {
         float2 y[4];
@@ -420,12 +445,8 @@ struct Score {
             fmax3_abs(far[(j >> 1) & 1], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
       large = __any_sync(0xffffffffu, fmaxf(far[0], far[1]) * z_per_s > 1.f);
     }
-    float2 k[5];
-    if constexpr (CAP) {
-      constexpr float c[5] = GPTB200_TANH_COEFS;
-#pragma unroll
-      for (int u = 0; u < 5; ++u) k[u] = both(c[u]);
-    }
+    float2 k[TERMS];
+    if constexpr (CAP) coefs(k, 1.f);
     float2 b = make_float2(slope2 * at, slope2 * (at - 1.f));  // the bias, key up to the query
 #pragma unroll
     for (int j = 0; j < 16; j += 8) {
@@ -438,7 +459,7 @@ struct Score {
         for (int q = 0; q < 4; ++q) t[q] = fmul2(t[q], both(z_per_s));
         if (large) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) t[q] = make_float2(tanh_any(t[q].x), tanh_any(t[q].y));
+          for (int q = 0; q < 4; ++q) t[q] = make_float2(tanh_any<WIDE>(t[q].x), tanh_any<WIDE>(t[q].y));
         } else {
           float2 u[4], a[4];
 #pragma unroll
@@ -1145,7 +1166,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
         bool steps = diag || segmask || ahead;
         if (!steps) {
           float far = 0.f;
-          float2 k[5], off[4];
+          float2 k[Score<MODE>::TERMS], off[4];
           if constexpr ((MODE & kCap) != 0) score.stream_coefs(k);
           uint32_t va[16], vb[16];
           tmem_ld16_nw(aS, va);
@@ -2588,6 +2609,9 @@ static int score_bwd_launch(const AttnParams& p, const ScoreMaps& m, cudaStream_
 // f<MODE>() for the call's cap and bias.
 template <typename F>
 static int score_mode(const gptb200_score_attention* a, F&& f) {
+  if (a->softcap > kShortCap)
+    return a->slopes ? f(std::integral_constant<int, kGeneral | kCap | kWide | kBias>())
+                     : f(std::integral_constant<int, kGeneral | kCap | kWide>());
   if (a->softcap > 0.f)
     return a->slopes ? f(std::integral_constant<int, kGeneral | kCap | kBias>())
                      : f(std::integral_constant<int, kGeneral | kCap>());

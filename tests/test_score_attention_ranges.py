@@ -40,3 +40,26 @@ def test_far_keys_above_the_near_ones(cuda, cap, bias, power):
            for n, x in got.items()}
     assert all(torch.isfinite(x).all() for x in got.values())
     _check(got, lse, want, tol, want_lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("cap,spread", [(200.0, 30.0), (200.0, 100.0), (1000.0, 150.0), (1000.0, 300.0),
+                                        (4000.0, 300.0), (65536.0, 300.0)])
+def test_large_caps(cuda, cap, spread, bias):
+    """Scores of hundreds under a cap of their size: an error of the tanh counts cap times
+    over. fp32 scores and tanh are a few roundings, so s' is off by at most 8 units of
+    2^-23 of its largest value, and the lse by that and its own roundings, 16 in all.
+    That is at most 0.0027 of a probability here. H + E of the formula holds 0.0049, of
+    which bf16 takes 0.0039: 1.2 times as much, 0.0059, has room for both."""
+
+    q, k, v, do = (x.to(cuda) for x in _inputs(1, 2, 2, 300, 17, spread))
+    slopes = kernels.distance_slopes(2, cuda) if bias else None
+    want, tol, want_lse = _formula(q, k, v, do, 0.125, cap, slopes, None, None)
+    s = 0.125 * q.double() @ k.double().transpose(-1, -2)
+    top = (cap * torch.tanh(s / cap)).abs().max().item()
+    assert top > 100
+    got, lse = _run(q, k, v, do, scale=0.125, softcap=cap, slopes=slopes)
+    assert (lse.double() - want_lse).abs().max() <= 16 * 2.0 ** -23 * top
+    for n in want:
+        assert ((got[n].double() - want[n]).abs() <= 1.2 * tol[n]).all(), n
