@@ -20,14 +20,20 @@
 // fitted. Each block writes one row of partials and a second launch adds them in a
 // fixed order: results repeat bit for bit. The arithmetic is two elements wide.
 //
-// Statistics are fp32 and the variance is taken about the mean, not from
-// sum(x^2): rows far from zero lose nothing. Outputs are rounded once.
+// Statistics are fp32, the variance is taken about the mean, and the mean is half a
+// unit of its last place off where the row lies far from zero: bf16 numbers of a size
+// have exact sums (8 bits, at most 2^14 of them), and the sum is divided by d, not just
+// multiplied by a rounded 1 / d; fp32 rows correct the mean by the sum of the distances
+// from it. So a constant row gives the bias, and as both passes form x - mean before
+// anything else, hat is off by |mean| rstd 2^-25 and no more. Outputs are rounded once.
 //
 // Measured (us and TB/s of the bytes named above; a copy moves 6.55): bf16
 // 131072 x 768 forward 67 and 6.0, backward with dx_in and all sums 130 and 6.2;
 // 8192 x 4096 forward 27 and 4.9 (a grid of 592 rows at a time: 14 turns); 65536 x
 // 768 fp32 66 and 6.1, 128 and 6.3. Rows without 16-byte accesses are bound by the
-// number of loads: bf16 65536 x 771 65 and 3.1, 126 and 3.2.
+// number of loads: bf16 65536 x 771 69 and 2.9, 132 and 3.1. Above 8192 the backward's
+// lanes hold 32 elements and spill: 8192 x 12288 81 and 5.0, 298 and 2.7 (bf16, with
+// dx_in and all sums), 216 and 3.7, 681 and 2.4 (fp32).
 #include <algorithm>
 
 #include "common.cuh"
@@ -205,7 +211,9 @@ __global__ void __launch_bounds__(32 * W * ln_fwd_rows<W>, ln_fwd_fit<T, VEC, W,
   using Raw = LnRaw<T, VEC>;
   // 128 bytes of a lane are enough in flight without the next row's
   constexpr bool AHEAD = ln_regs<T, VEC, NV> < 32;
-  __shared__ float red[2][W][1];
+  // fp32: the mean is corrected by the distances from it
+  constexpr bool CORRECT = sizeof(T) == 4;
+  __shared__ float red[2][W][1], red2[2][W][CORRECT ? 2 : 1];  // in turn: one barrier each
   int turn = 0;
   const int g = W == 1 ? threadIdx.x >> 5 : 0;
   const int t = W == 1 ? threadIdx.x & 31 : threadIdx.x;
@@ -243,28 +251,58 @@ __global__ void __launch_bounds__(32 * W * ln_fwd_rows<W>, ln_fwd_fit<T, VEC, W,
       w[i].stay();
       c[i].stay();
     }
-    float sum[1] = {0.f};
+    // chunks two elements wide; single ones would have to be brought together first
+    float2 add = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float v[VEC];
-      now[i].get(v);
+      if constexpr (VEC == 1) {
+        float v;
+        now[i].get(&v);
+        add.x += v;
+      } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) sum[0] += v[j];
-    }
-    ln_group_sums<W>(sum, red, turn, 0);
-    const float mean = sum[0] * inv_d;
-    float var[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float v[VEC];
-      now[i].get(v);
-      if (col(i) < p.d) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) var[0] = fmaf(v[j] - mean, v[j] - mean, var[0]);
+        for (int k = 0; k < VEC / 2; ++k) add = fadd2(add, now[i].pair(k));
       }
     }
-    ln_group_sums<W>(var, red, turn, 0);
-    const float rstd = rsqrtf(var[0] * inv_d + p.eps);
+    float sum[1] = {add.x + add.y};
+    ln_group_sums<W>(sum, red, turn, 0);
+    float mean;
+    if constexpr (VEC == 1) {  // the division costs these 78 us, this 69 (65536 x 771 bf16)
+      mean = sum[0] * inv_d;
+      mean = fmaf(fmaf(-mean, (float)p.d, sum[0]), inv_d, mean);  // and what that leaves of the sum
+    } else {  // 67 us so, 72 the other way (131072 x 768 bf16)
+      mean = sum[0] / (float)p.d;
+    }
+    float2 lean = make_float2(0.f, 0.f), square = lean;  // of the distances from it
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (col(i) < p.d) {
+        if constexpr (VEC == 1) {
+          float z;
+          now[i].get(&z);
+          z -= mean;
+          if constexpr (CORRECT) lean.x += z;
+          square.x = fmaf(z, z, square.x);
+        } else {
+#pragma unroll
+          for (int k = 0; k < VEC / 2; ++k) {
+            const float2 z = fadd2(now[i].pair(k), make_float2(-mean, -mean));
+            if constexpr (CORRECT) lean = fadd2(lean, z);
+            square = ffma2(z, z, square);
+          }
+        }
+      }
+    }
+    float dev[CORRECT ? 2 : 1] = {square.x + square.y};
+    if constexpr (CORRECT) dev[1] = lean.x + lean.y;
+    ln_group_sums<W>(dev, red2, turn, 0);
+    float var = dev[0] * inv_d;
+    if constexpr (CORRECT) {
+      const float off = dev[1] * inv_d;
+      mean += off;
+      var = fmaxf(fmaf(-off, off, var), 0.f);
+    }
+    const float rstd = rsqrtf(var + p.eps);
     if (t == 0) {
       p.mean[r] = mean;
       p.rstd[r] = rstd;
@@ -272,12 +310,23 @@ __global__ void __launch_bounds__(32 * W * ln_fwd_rows<W>, ln_fwd_fit<T, VEC, W,
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (col(i) < p.d) {
-        float v[VEC], a[VEC], b[VEC];
-        now[i].get(v);
-        w[i].get(a);
-        c[i].get(b);
+        float v[VEC];
+        if constexpr (VEC == 1) {
+          float a, b;
+          now[i].get(v);
+          w[i].get(&a);
+          c[i].get(&b);
+          v[0] = fmaf((v[0] - mean) * rstd, a, b);
+        } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = fmaf((v[j] - mean) * rstd, a[j], b[j]);
+          for (int k = 0; k < VEC / 2; ++k) {
+            const float2 z = fmul2(fadd2(now[i].pair(k), make_float2(-mean, -mean)),
+                                   make_float2(rstd, rstd));
+            const float2 o = ffma2(z, w[i].pair(k), c[i].pair(k));
+            v[2 * k] = o.x;
+            v[2 * k + 1] = o.y;
+          }
+        }
         Raw::store(y + r * p.ldy + col(i), v);
       }
     }
@@ -441,8 +490,7 @@ __global__ void __launch_bounds__(32 * W * ln_bwd_rows<VEC, W, NV>, 1) ln_bwd_ke
     float s[2 * R];
 #pragma unroll
     for (int u = 0; u < R; ++u) {
-      const float shift = -mean[u] * rstd[u];
-      const float2 m = make_float2(rstd[u], rstd[u]), b = make_float2(shift, shift);
+      const float2 m = make_float2(rstd[u], rstd[u]), b = make_float2(-mean[u], -mean[u]);
       float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll
       for (int i = 0; i < NV; i += C) {
@@ -457,7 +505,7 @@ __global__ void __launch_bounds__(32 * W * ln_bwd_rows<VEC, W, NV>, 1) ln_bwd_ke
         for (int j = 0; j < PAIRS; ++j) {  // columns past the width have dy = 0
           const int k = i * VEC / 2 + j;
           const float2 gy = ln_pair<T, VEC>(gs, j);
-          const float2 hat = ffma2(ln_pair<T, VEC>(xs, j), m, b);
+          const float2 hat = fmul2(fadd2(ln_pair<T, VEC>(xs, j), b), m);
           const float2 dn = fmul2(gy, ln_pair<T, VEC>(ws, j));
           ds[k] = ffma2(gy, hat, ds[k]);
           db[k] = fadd2(db[k], gy);
@@ -473,9 +521,9 @@ __global__ void __launch_bounds__(32 * W * ln_bwd_rows<VEC, W, NV>, 1) ln_bwd_ke
     for (int i = 0; i < (WIDE ? 0 : NV); ++i) w[i].stay();  // packed between the passes
 #pragma unroll
     for (int u = 0; u < R; ++u) {
-      const float shift = -mean[u] * rstd[u];
-      const float s0 = -s[2 * u] * inv_d, s1 = -s[2 * u + 1] * inv_d;
-      const float2 m = make_float2(rstd[u], rstd[u]), b = make_float2(shift, shift);
+      // per x - mean, not per hat: one operation less
+      const float s0 = -s[2 * u] * inv_d, s1 = -s[2 * u + 1] * inv_d * rstd[u];
+      const float2 m = make_float2(rstd[u], rstd[u]), b = make_float2(-mean[u], -mean[u]);
       const float2 m0 = make_float2(s0, s0), m1 = make_float2(s1, s1);
       T* to = dx + (r + u * step) * p.lddx;
       const bool in = R == 1 || r + u * step < p.rows;
@@ -492,9 +540,9 @@ __global__ void __launch_bounds__(32 * W * ln_bwd_rows<VEC, W, NV>, 1) ln_bwd_ke
         float v[C * VEC];
 #pragma unroll
         for (int j = 0; j < PAIRS; ++j) {  // past the width or the last row: not stored
-          const float2 hat = ffma2(ln_pair<T, VEC>(xs, j), m, b);
+          const float2 away = fadd2(ln_pair<T, VEC>(xs, j), b);
           const float2 dn = ffma2(ln_pair<T, VEC>(gs, j), ln_pair<T, VEC>(ws, j), m0);
-          float2 o = ffma2(hat, m1, dn);
+          float2 o = ffma2(away, m1, dn);
           if constexpr (RES)
             o = ffma2(o, m, ln_pair<T, VEC>(as, j));
           else
@@ -676,7 +724,8 @@ struct LnBackward {
   int launch() const {
     constexpr int rows = ln_bwd_rows<VEC, W, NV>;
     const int blocks = (int)ln_bwd_blocks(p.rows, rows);
-    size_t smem = rows > 1 ? sizeof(float) * rows * (size_t)p.d : 0;  // <= 16 KB
+    // 36 KB at most (12 rows of 768), which the slots of a staged variant cover
+    size_t smem = rows > 1 ? sizeof(float) * rows * (size_t)p.d : 0;
     auto kern = ln_bwd_kernel<T, VEC, W, NV, RES, COL>;
     if constexpr (ln_staged<T, VEC>) {
       constexpr int slots = ln_slots<W, NV, RES> * ln_slot<W, NV, RES>;
