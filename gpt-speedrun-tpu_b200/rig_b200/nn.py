@@ -65,7 +65,7 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, scale, bias, eps):
         shape = x.shape
         x2 = x.reshape(-1, shape[-1])
-        if x2.stride(1) != 1:
+        if x2.stride(1) != 1 or x2.stride(0) < x2.shape[1]:  # broadcast or overlapping rows too
             x2 = x2.contiguous()
         w = scale.to(x.dtype).contiguous()
         b = None if bias is None else bias.to(x.dtype).contiguous()
