@@ -57,9 +57,12 @@ def _validate(q, k, v) -> None:
         raise TypeError(f"q, k, and v must be bfloat16, got {q.dtype}, {k.dtype}, {v.dtype}")
 
 
+_MASKS = ("slopes", "segment_ids", "prefix_lens")
+
+
 class _ScoreAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, how, rope):
+    def forward(ctx, q, k, v, scale, softcap, rope, *masks):
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
         if rope is not None:  # rotate copies of q and k (BHSD viewed as BTHD)
             q, k = q.clone(), k.clone()
@@ -68,18 +71,23 @@ class _ScoreAttention(torch.autograd.Function):
         b, h, t, _ = q.shape
         o = torch.empty_like(q)
         lse = torch.empty(b, h, t, dtype=torch.float32, device=q.device)
-        ops.score_attention_fwd(q, k, v, o, lse, **how)
-        ctx.save_for_backward(q, k, v, o, lse)
+        how = dict(scale=scale, softcap=softcap)
+        ops.score_attention_fwd(q, k, v, o, lse, **how, **dict(zip(_MASKS, masks)))
+        # the masks may be the caller's own buffers: autograd notices if they are written to
+        # before the backward (tensors of inference mode have no versions, hence copies)
+        ctx.save_for_backward(q, k, v, o, lse, *(
+            m.clone() if m is not None and m.is_inference() else m for m in masks))
         ctx.how, ctx.rope = how, rope
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, o, lse = ctx.saved_tensors
+        q, k, v, o, lse, *masks = ctx.saved_tensors
         do = do.contiguous().to(torch.bfloat16)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-        ops.score_attention_bwd(q, k, v, o, do, lse, dq, dk, dv, rope=ctx.rope, **ctx.how)
-        return dq, dk, dv, None, None
+        ops.score_attention_bwd(q, k, v, o, do, lse, dq, dk, dv, rope=ctx.rope, **ctx.how,
+                                **dict(zip(_MASKS, masks)))
+        return dq, dk, dv, *[None] * (3 + len(masks))
 
 
 def make_score_attention(config: ScoreAttentionConfig = ScoreAttentionConfig(), *,
@@ -95,8 +103,7 @@ def make_score_attention(config: ScoreAttentionConfig = ScoreAttentionConfig(), 
             slopes = slopes.detach().to(device=q.device, dtype=torch.float32).contiguous()
         ints = [None if t is None else t.to(device=q.device, dtype=torch.int32).contiguous()
                 for t in (segment_ids, prefix_lens)]
-        how = dict(scale=float(scale), softcap=float(config.softcap), slopes=slopes,
-                   segment_ids=ints[0], prefix_lens=ints[1])
-        return _ScoreAttention.apply(q, k, v, how, rope_tables)
+        return _ScoreAttention.apply(q, k, v, float(scale), float(config.softcap), rope_tables,
+                                     slopes, *ints)
 
     return attention

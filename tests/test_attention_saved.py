@@ -1,0 +1,69 @@
+"""What the attention factories keep of a call for its backward: the caller may reuse
+its mask buffers for the next batch, and hears of it where that comes too early."""
+
+import pytest
+import torch
+
+from rig_b200 import kernels, ops
+
+B, H, KV, T = 2, 4, 2, 150
+
+
+def _inputs(dev):
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(B, H, T, 64, generator=g).bfloat16().to(dev)
+    k, v = (torch.randn(B, KV, T, 64, generator=g).bfloat16().to(dev) for _ in range(2))
+    do = torch.randn(B, H, T, 64, generator=g).bfloat16().to(dev)
+    masks = dict(slopes=kernels.distance_slopes(H, dev),
+                 segment_ids=(torch.arange(T, device=dev) // 40).int().expand(B, T).contiguous(),
+                 prefix_lens=torch.tensor([9, 70], dtype=torch.int32, device=dev))
+    return [x.requires_grad_(True) for x in (q, k, v)], do, masks
+
+
+def _reuse(name, t):
+    t.copy_(t * 2 if name == "slopes" else t + 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["slopes", "segment_ids", "prefix_lens"])
+def test_mask_overwritten_before_the_backward(cuda, name):
+    qkv, do, masks = _inputs(cuda)
+    attention = kernels.make_score_attention(kernels.ScoreAttentionConfig(softcap=30.0))
+    y = attention(*qkv, **masks)
+    _reuse(name, masks[name])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(do)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["slopes", "segment_ids", "prefix_lens"])
+@pytest.mark.parametrize("kind", ["converted", "inference"])
+def test_mask_that_was_copied_may_be_overwritten(cuda, name, kind):
+    """A mask of another type, which the call converts, and one without versions."""
+
+    qkv, do, masks = _inputs(cuda)
+    attention = kernels.make_score_attention(kernels.ScoreAttentionConfig(softcap=30.0))
+    y = attention(*qkv, **masks)
+    want = torch.autograd.grad(y, qkv, do)
+    if kind == "converted":
+        masks[name] = masks[name].double() if name == "slopes" else masks[name].long()
+    else:
+        with torch.inference_mode():
+            masks[name] = masks[name].clone()
+    y = attention(*qkv, **masks)
+    with torch.inference_mode():
+        _reuse(name, masks[name])
+    got = torch.autograd.grad(y, qkv, do)
+    assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+    assert (got[0].float() - want[0].float()).norm() <= 1e-3 * want[0].float().norm()
+
+
+@pytest.mark.gpu
+def test_gradients_twice_and_without_masks(cuda):
+    qkv, do, masks = _inputs(cuda)
+    for how in (masks, {}):
+        attention = kernels.make_score_attention(rope_tables=ops.rope_tables(T, 64, cuda))
+        y = attention(*qkv, **how)
+        first = torch.autograd.grad(y, qkv, do, retain_graph=True)
+        again = torch.autograd.grad(y, qkv, do)
+        assert torch.equal(first[1], again[1]) and torch.equal(first[2], again[2])
