@@ -93,13 +93,17 @@ class _ScoreAttention(torch.autograd.Function):
 def make_score_attention(config: ScoreAttentionConfig = ScoreAttentionConfig(), *,
                          rope_tables=None) -> Callable:
     """Returns attention(q, k, v, *, slopes, segment_ids, prefix_lens) over BHSD
-    bf16 tensors; k and v may have fewer heads than q. With `rope_tables` (from
+    bf16 tensors; k and v may have fewer heads than q. Slopes are constants: those
+    that require a gradient are refused. With `rope_tables` (from
     `ops.rope_tables`) q and k are rotated first, as in `make_causal_attention`."""
 
     def attention(q, k, v, *, slopes=None, segment_ids=None, prefix_lens=None):
         _validate(q, k, v)
         scale = config.softmax_scale if config.softmax_scale is not None else q.shape[-1] ** -0.5
         if slopes is not None:
+            if slopes.requires_grad and torch.is_grad_enabled():
+                raise ValueError("slopes are constants: the attention gives them no gradient "
+                                 "(pass slopes.detach())")
             slopes = slopes.detach().to(device=q.device, dtype=torch.float32).contiguous()
         ints = [None if t is None else t.to(device=q.device, dtype=torch.int32).contiguous()
                 for t in (segment_ids, prefix_lens)]

@@ -67,3 +67,28 @@ def test_gradients_twice_and_without_masks(cuda):
         first = torch.autograd.grad(y, qkv, do, retain_graph=True)
         again = torch.autograd.grad(y, qkv, do)
         assert torch.equal(first[1], again[1]) and torch.equal(first[2], again[2])
+
+
+def test_slopes_have_no_gradient():
+    """Learned slopes are refused (before anything runs), not left without a gradient."""
+
+    q, k, v = (torch.randn(1, 2, 8, 64).bfloat16() for _ in range(3))
+    attention = kernels.make_score_attention()
+    slopes = torch.zeros(2, requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        attention(q, k, v, slopes=slopes)
+    with pytest.raises(ValueError, match="gradient"):
+        attention(q, k, v, slopes=torch.exp(slopes))
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):  # as any CPU tensor
+        attention(q, k, v, slopes=slopes)
+
+
+@pytest.mark.gpu
+def test_slopes_that_require_a_gradient_without_one(cuda):
+    qkv, _, masks = _inputs(cuda)
+    attention = kernels.make_score_attention()
+    want = attention(*qkv, **masks)
+    learned = masks["slopes"].clone().requires_grad_(True)
+    with torch.no_grad():
+        got = attention(*qkv, **{**masks, "slopes": learned})
+    assert torch.equal(got, want)
