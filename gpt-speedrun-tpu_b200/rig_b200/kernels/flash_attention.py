@@ -63,17 +63,21 @@ class _Attention(torch.autograd.Function):
         o = torch.empty_like(q)
         lse = torch.empty(b, h, t, dtype=torch.float32, device=q.device)
         ops.attention_fwd(q, k, v, o, lse, scale=scale, segment_ids=segment_ids)
-        ctx.save_for_backward(q, k, v, o, lse)
-        ctx.scale, ctx.rope, ctx.segment_ids = scale, rope, segment_ids
+        # the ids may be the caller's own buffer: autograd notices if it is written to before
+        # the backward (a tensor of inference mode has no versions, hence a copy)
+        if segment_ids is not None and segment_ids.is_inference():
+            segment_ids = segment_ids.clone()
+        ctx.save_for_backward(q, k, v, o, lse, segment_ids)
+        ctx.scale, ctx.rope = scale, rope
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, o, lse = ctx.saved_tensors
+        q, k, v, o, lse, segment_ids = ctx.saved_tensors
         do = do.contiguous().to(torch.bfloat16)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         ops.attention_bwd(q, k, v, o, do, lse, dq, dk, dv, scale=ctx.scale, rope=ctx.rope,
-                          segment_ids=ctx.segment_ids)
+                          segment_ids=segment_ids)
         return dq, dk, dv, None, None, None
 
 

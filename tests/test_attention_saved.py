@@ -21,7 +21,7 @@ def _inputs(dev):
 
 
 def _reuse(name, t):
-    t.copy_(t * 2 if name == "slopes" else t + 1)
+    t.copy_(t * 2 if name == "slopes" else t // 2)
 
 
 @pytest.mark.gpu
@@ -92,3 +92,23 @@ def test_slopes_that_require_a_gradient_without_one(cuda):
     with torch.no_grad():
         got = attention(*qkv, **{**masks, "slopes": learned})
     assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_plain_attention_ids_overwritten_before_the_backward(cuda):
+    qkv, do, masks = _inputs(cuda)
+    q, k, v = (x.detach()[:, :KV].contiguous().requires_grad_(True) for x in qkv)
+    do, ids = do[:, :KV].contiguous(), masks["segment_ids"]
+    attention = kernels.make_causal_attention()
+    want = torch.autograd.grad(attention(q, k, v, ids), (q, k, v), do)
+    with torch.inference_mode():
+        other = ids.clone()
+    y = attention(q, k, v, other)
+    with torch.inference_mode():
+        _reuse("segment_ids", other)
+    got = torch.autograd.grad(y, (q, k, v), do)
+    assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+    y = attention(q, k, v, ids)
+    _reuse("segment_ids", ids)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(do)
