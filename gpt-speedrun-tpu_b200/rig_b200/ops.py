@@ -172,6 +172,23 @@ def matmul(x: torch.Tensor, w: torch.Tensor, *, bias=None, out=None, kind=_lib.E
                 residual=residual, aux=aux, rope=rope, rope_cols=rope_cols)
 
 
+def _rope_ptrs(rope, t: int, d: int) -> tuple[int | None, int | None]:
+    """Checks a (cos, sin) pair for t positions of head dimension d (the kernels read
+    row i for position i); returns the addresses."""
+
+    if rope is None:
+        return None, None
+    for name, r in zip(("cos", "sin"), rope):
+        if (not r.is_cuda or r.dtype is not BF16 or r.dim() != 2 or r.shape[1] != d // 2
+                or not r.is_contiguous()):
+            raise ValueError(f"rope {name} must be a contiguous CUDA tensor of {BF16} [seq, {d // 2}], got "
+                             f"{r.device} {r.dtype} {tuple(r.shape)}")
+        if r.shape[0] < t:
+            raise ValueError(f"rope tables of {r.shape[0]} positions do not cover {t}")
+    cos, sin = rope
+    return cos.data_ptr(), sin.data_ptr()
+
+
 def rope_apply(x: torch.Tensor, rope, *, inverse: bool = False) -> torch.Tensor:
     """In-place interleaved RoPE on a BTHD view (inverse: the transpose rotation)."""
 
@@ -180,7 +197,7 @@ def rope_apply(x: torch.Tensor, rope, *, inverse: bool = False) -> torch.Tensor:
         raise ValueError("rope_apply expects a [B, T, H, D] view with a contiguous head dim")
     b, t, h, d = x.shape
     call("gptb200_rope_apply", x.data_ptr(), x.stride(0), x.stride(1), x.stride(2), b, t, h, d,
-         rope[0].data_ptr(), rope[1].data_ptr(), int(inverse), _stream())
+         *_rope_ptrs(rope, t, d), int(inverse), _stream())
     return x
 
 
@@ -407,11 +424,11 @@ def attention_bwd(q, k, v, o, do, lse, dq, dk, dv, *, scale: float, layout="bhsd
         b, t, h, dh = q.shape
     if workspace is None:
         workspace = attention_workspace(b, h, t, q.device)
-    cos, sin = rope if rope is not None else (None, None)
+    cos, sin = _rope_ptrs(rope, t, dh)
     seg = _segments(segment_ids, b, t)
     call("gptb200_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), sb, sh, st,
          o.data_ptr(), do.data_ptr(), osb, osh, ost, lse.data_ptr(), dq.data_ptr(),
-         dk.data_ptr(), dv.data_ptr(), b, h, t, dh, float(scale), _ptr(cos), _ptr(sin),
+         dk.data_ptr(), dv.data_ptr(), b, h, t, dh, float(scale), cos, sin,
          _ptr(seg), workspace.data_ptr(), _stream())
     return dq, dk, dv
 
@@ -514,10 +531,10 @@ def score_attention_bwd(q, k, v, o, do, lse, dq, dk, dv, *, scale: float, layout
         workspace = _scratch(size, q.device)
     elif not workspace.is_cuda or workspace.numel() * workspace.element_size() < size:
         raise ValueError(f"the workspace needs {size} bytes on the device")
-    cos, sin = rope if rope is not None else (None, None)
+    cos, sin = _rope_ptrs(rope, t, d)
     call("gptb200_score_attention_bwd", c, do.data_ptr(), _view4("do", do, b, h, t, d, bthd),
          dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _view4("dq", dq, b, h, t, d, bthd), dkvs,
-         _ptr(cos), _ptr(sin), _ptr(workspace), _stream())
+         cos, sin, _ptr(workspace), _stream())
     return dq, dk, dv
 
 
