@@ -676,6 +676,17 @@ def _adamw8_flat(name: str, t: torch.Tensor | None, n: int, dtype) -> int | None
     return t.data_ptr()
 
 
+def _adamw8_plan(n: int, groups_dev: torch.Tensor, n_groups: int, workspace: torch.Tensor) -> None:
+    """Checks the group table and the workspace, which the kernels read and write in full."""
+
+    size = n_groups * ctypes.sizeof(_lib.TensorGroup)
+    if not groups_dev.is_cuda or not groups_dev.is_contiguous() or groups_dev.nbytes < size:
+        raise ValueError(f"{n_groups} tensor groups are {size} contiguous bytes on the device")
+    size = int(_lib.load().gptb200_adamw_workspace_size(n))
+    if not workspace.is_cuda or not workspace.is_contiguous() or workspace.nbytes < size:
+        raise ValueError(f"the workspace needs {size} bytes on the device")
+
+
 def adamw8_step(params, state, grads, groups_dev, n_groups, cfg, step, loss, history, params_bf16,
                 seed, workspace):
     """`adamw_step` with both moments in 8 bits (`adamw8_state`, updated in place).
@@ -683,9 +694,14 @@ def adamw8_step(params, state, grads, groups_dev, n_groups, cfg, step, loss, his
     The rounding of the new moments draws on (seed, step, element): the same
     inputs give the same codes. workspace: `adamw_workspace`."""
 
-    _cuda(groups_dev, step, loss, history, workspace)
     n = params.numel()
     q = _adamw8(state, n)
+    _adamw8_plan(n, groups_dev, n_groups, workspace)
+    for name, t, dtype in (("step", step, torch.int32), ("loss", loss, F32), ("history", history, F32)):
+        if t is not None:
+            _adamw8_flat(name, t, max(1, t.numel()), dtype)
+    if history is not None and (history.dim() != 2 or history.shape[1] != 3):
+        raise ValueError(f"history must have rows of 3 numbers, got {tuple(history.shape)}")
     call("gptb200_adamw8_step", _adamw8_flat("params", params, n, F32), q,
          _adamw8_flat("grads", grads, n, F32), n, groups_dev.data_ptr(), n_groups, cfg,
          step.data_ptr(), _ptr(loss), _ptr(history), _adamw8_flat("params_bf16", params_bf16, n, BF16),
@@ -696,9 +712,9 @@ def adamw8_update_range(params, state, grads, begin, end, groups_dev, n_groups, 
                         params_bf16, seed, workspace):
     """`adamw_update_range` with 8-bit moments; begin and end are multiples of 64."""
 
-    _cuda(groups_dev, workspace)
     n = params.numel()
     q = _adamw8(state, n)
+    _adamw8_plan(n, groups_dev, n_groups, workspace)
     if not 0 <= begin < end <= state[0].numel():
         raise ValueError(f"[{begin}, {end}) is outside the {state[0].numel()} elements")
     call("gptb200_adamw8_update_range", _adamw8_flat("params", params, n, F32), q,
