@@ -33,8 +33,9 @@
 // Every mbarrier wait is bounded (common.cuh). Semantics follow
 // rig/kernels/tpu_flash_attention.py:171-207 (fp32 statistics, bf16 P).
 //
-// Both kernels take a MODE. kClassic is the plain causal attention above; the
-// others run the score-modified attention (gptb200_score_attention_fwd/bwd),
+// Score-modified attention (gptb200_score_attention_fwd/bwd) has a forward of its own,
+// score_fwd_tc, and shares the backward, whose MODE kClassic is the plain causal
+// attention above:
 //   s'_ij = cap tanh(scale q_i.k_j / cap) - slope_h |i - j|,
 // with key/value heads shared by heads / kv_heads query heads, a per-sequence
 // prefix whose keys every query sees, and segment ids whose negative values
@@ -43,21 +44,21 @@
 //  * tanh. The exponentials hold the MUFU pipe for 8 clocks a score (of a warp's
 //    32 rows), so tanh runs on the FMA pipe beside it, 8 clocks for a score too:
 //    z P(z^2) with five terms, relative error 7e-6 (seven and 5e-8 for caps above
-//    kShortCap), where a warp's scores have |z| <= 1; only a warp that holds a larger one takes 1 - 2 / (1 + e^(2z)),
-//    two more MUFU operations per score.
+//    kShortCap), where a warp's scores have |z| <= 1; only a warp that holds a larger
+//    one takes 1 - 2 / (1 + e^(2z)), two more MUFU operations per score.
 //  * the bias. Linear in the key up to the query, so it is one packed FMA for
 //    two scores; |i - j| itself only near the diagonal and in the prefix.
 // Masks are words of 32 keys, made once per block and warp; blocks that no mask
 // reaches run code without them (tests that are predicated off still take issue
-// slots). The forward's rows go through one streaming pass against the maximum
-// they have so far, the diagonal block first (softmax_general). In the backward an
+// slots). The forward's rows go through one streaming pass against the reference
+// they have so far, the diagonal block first. In the backward an
 // item is a key tile of a key/value head: it walks the query tiles of every query
 // head that shares it, so dK and dV of the group add up in TMEM, in a fixed order.
 // Roundings: P to bf16 before P.V and P^T dO, dS to bf16 before dK and dQ, delta
 // from O as stored (exact for one key tile); sums, maxima, lse, dQ's accumulator
 // and everything between are fp32.
 // What bounds them, 1 x 12 x 8192 (us, forward | backward):
-//    plain causal kernels 230 | 395; MODE without cap and bias 181 | 343; bias
+//    plain causal kernels 230 | 395; without cap and bias 181 | 343; bias
 //    192 | 358; cap 238 | 429; both 259 | 454 (398 and 568 TFLOP/s).
 //  Forward: the latency of two softmax warps a scheduler. Without any arithmetic
 //  (raw scores packed as P) it takes 123 us; with it a warp spends 4,100 of 5,080
@@ -87,8 +88,8 @@ constexpr int HD = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Score modes of the kernels (bits of a MODE > kClassic: 1 general, 2 cap, 4 bias,
-// 8 a cap above kShortCap).
+// Modes of the score-modified kernels (bits: 1 always, 2 cap, 4 bias, 8 a cap above
+// kShortCap); kClassic is the plain attention's backward.
 enum { kClassic = 0, kGeneral = 1, kCap = 2, kBias = 4, kWide = 8 };
 // An error of tanh counts cap times in a score. Its five terms (7e-6 relative) are up
 // to 7e-4 of a probability at this cap, a third of the rounding to bf16; larger caps
@@ -98,20 +99,20 @@ constexpr float kShortCap = 128.f;
 
 struct AttnParams {
   int B, H, T;         // H: query heads
-  int KVH, group;      // key/value heads, query heads per key/value head (MODE > kClassic)
+  int KVH, group;      // key/value heads, query heads per key/value head (score-modified)
   float scale;
   float cap;           // tanh cap of the scaled scores (kCap)
   const float* slopes; // [H] distance slopes (kBias)
-  const int* prefix;   // [B] keys every query sees, or null (MODE > kClassic)
-  int by_weight;       // items of all heads by falling weight (MODE > kClassic)
+  const int* prefix;   // [B] keys every query sees, or null (score-modified)
+  int by_weight;       // items of all heads by falling weight (score-modified)
   // output / saved tensors
   bf16* o;
   int64_t osb, osh, ost;
-  float* o32;          // [B, H, T, 64] fp32 instead of o and lse, or null (MODE > kClassic)
+  float* o32;          // [B, H, T, 64] fp32 instead of o and lse, or null (score-modified)
   float* lse;          // [B, H, T], natural log
   const bf16* dout;
-  const float* delta;  // [B, H, T] (MODE > kClassic: negated)
-  const float* neg_lse2;  // [B, H, T] -lse log2(e) (MODE > kClassic)
+  const float* delta;  // [B, H, T] (score-modified: negated)
+  const float* neg_lse2;  // [B, H, T] -lse log2(e) (score-modified)
   float* dq_acc;       // [B, H, T, 64] fp32
   bf16* dk;
   bf16* dv;
@@ -582,7 +583,7 @@ constexpr int KV_BYTES = FK * 128;      // 128 rows x 64 bf16
 constexpr int kKvStages = 4;
 constexpr int kFwdMma1Warp = 10;       // MMA thread of tile 1 (warp 1 serves tile 0)
 constexpr int kFwdThreads = 32 * 11;
-// MODE > kClassic: whole warpgroups, so that registers can move from the one
+// score_fwd_tc: whole warpgroups, so that registers can move from the one
 // that loads and issues (warps 0-3, the last one idle) to the two softmax ones
 // (4-7: tile 0, 8-11: tile 1), which keep a block's raw scores beside its
 // probabilities. The shares add up to what the launch gives.
@@ -595,8 +596,8 @@ constexpr int kFwdItemUsers = 2 + 8;   // both MMA threads, the 8 softmax warps
 // visits (tile 0 the first n0 of them), whether tile 1 lies inside the sequence.
 struct FwdItem {
   int pr, bh, nkv, n0, has1;
-  int nch;     // chunks of the segment table (MODE > kClassic)
-  int prefix;  // keys every query sees (MODE > kClassic)
+  int nch;     // chunks of the segment table (score_fwd_tc)
+  int prefix;  // keys every query sees (score_fwd_tc)
   int pad;
 };
 
@@ -616,12 +617,11 @@ struct FwdSmem {
   static constexpr int TOTAL = BAR + 256;
 };
 
-template <bool SEG, int MODE>
-__global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralThreads, 1)
+template <bool SEG>
+__global__ void __launch_bounds__(kFwdThreads, 1)
     attn_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const AttnParams p) {
   using L = FwdSmem<SEG>;
-  constexpr bool GENERAL = MODE != kClassic;
   extern __shared__ __align__(1024) uint8_t smem_fwd[];
   uint8_t* sm = smem_fwd;
   if (smem_u32(sm) & 1023) {  // the layout needs 1024-byte aligned tiles: give up, flagged
@@ -647,8 +647,6 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   FwdItem* items = reinterpret_cast<FwdItem*>(sm + L::ITEM);
 
-  constexpr int kMma1Warp = GENERAL ? 2 : kFwdMma1Warp;
-  constexpr int kSoftmaxWarp = GENERAL ? 4 : 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int BH = p.B * p.H;
   const int npair = (p.T + 2 * FQ - 1) / (2 * FQ);
@@ -657,11 +655,8 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
   auto segtab_of = [&](int slot) {
     return reinterpret_cast<int2*>(sm + L::SEGTAB) + slot * kMaxSegChunks;
   };
-  // Key block of list entry j of the item in `slot` (nkv entries). MODE >
-  // kClassic walks the list from its end: the diagonal comes first and sets the
-  // rows' maxima, which a bias that falls with the distance then never raises.
-  auto kblock = [&](int slot, int j, int nkv) -> int {
-    if constexpr (GENERAL) j = nkv - 1 - j;
+  // key block of list entry j of the item in `slot`
+  auto kblock = [&](int slot, int j) -> int {
     if constexpr (SEG)
       return reinterpret_cast<const int*>(sm + L::BLOCKS)[slot * (kMaxSegChunks / 2) + j];
     else
@@ -700,7 +695,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
   auto tO = [&](int x) { return tmem + 256 + 64 * x; };
   auto tP = [&](int x) { return tmem + 384 + 64 * x; };
 
-  auto produce = [&]() {
+  if (warp == 0) {
     // Item producer: publishes each item's slot (with segment ids also the
     // chunk ranges and the key-block list), then loads its two Q tiles and its
     // K/V blocks into the ring.
@@ -717,11 +712,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
         }
         break;
       }
-      int bh = item / npair, pr = npair - 1 - (item - bh * npair);
-      if (GENERAL && p.by_weight) {
-        pr = npair - 1 - item / BH;
-        bh = item % BH;
-      }
+      const int bh = item / npair, pr = npair - 1 - (item - bh * npair);
       const int b = bh / p.H, h = bh - b * p.H;
       const int q0 = pr * 2 * FQ;
       // tile x's diagonal key block is d0 + x; tile 1 of the last pair may lie
@@ -730,57 +721,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
       const int has1 = q0 + FQ < p.T;
       const int dmax = has1 ? d0 + 1 : d0;
       int nkv = dmax + 1, n0 = d0 + 1;
-      int hk = h, pf = 0, nch = 0;
-      if constexpr (GENERAL) {
-        hk = h / p.group;
-        if (p.prefix) {  // the prefix's blocks are seen by both tiles
-          pf = min(max(p.prefix[b], 0), p.T);
-          nkv = max(nkv, (pf + FK - 1) / FK);
-          n0 = max(n0, (pf + FK - 1) / FK);
-        }
-      }
-      if constexpr (SEG && GENERAL) {
-        // As below, over the blocks up to the diagonal or the prefix's end. A
-        // tile's diagonal block stays in the list even if nothing meets there
-        // (padding alone), so that every tile has a block and writes its rows.
-        const int* segrow = p.seg + (int64_t)b * p.T;
-        int2* tab = segtab_of(slot);
-        nch = min((p.T + kSegChunk - 1) / kSegChunk, 2 * nkv);
-        for (int c = 0; c < nch; ++c) {
-          int mn = INT_MAX, mx = INT_MIN;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int t = c * kSegChunk + u * 32 + lane;
-            if (t < p.T) {
-              const int v = segrow[t];
-              mn = min(mn, v);
-              mx = max(mx, v);
-            }
-          }
-          mn = __reduce_min_sync(0xffffffffu, mn);
-          mx = __reduce_max_sync(0xffffffffu, mx);
-          if (lane == 0) tab[c] = seg_chunk(mn, mx);
-        }
-        __syncwarp();
-        if (lane == 0) {
-          int* bl = reinterpret_cast<int*>(sm + L::BLOCKS) + slot * (kMaxSegChunks / 2);
-          const int2 qr0 = seg_range(tab, nch, 2 * d0, 2);
-          const int2 qr1 = seg_range(tab, nch, 2 * d0 + 2, 2);
-          int n = 0, n_le0 = 0;
-          for (int j = 0; j < nkv; ++j) {
-            const int2 kr = seg_range(tab, nch, 2 * j, 2);
-            if (j == d0 || j == dmax || (j < n0 && seg_meet(kr, qr0)) ||
-                (has1 && seg_meet(kr, qr1))) {
-              bl[n++] = j;
-              if (j < n0) ++n_le0;
-            }
-          }
-          nkv = n;
-          n0 = n_le0;
-        }
-        nkv = __shfl_sync(0xffffffffu, nkv, 0);
-        n0 = __shfl_sync(0xffffffffu, n0, 0);
-      } else if constexpr (SEG) {
+      if constexpr (SEG) {
         // The key blocks 0..dmax either query tile can see, in order. Both
         // tiles walk this one list (tile 0 its prefix up to d0); a block only
         // the other tile needs is fully masked for a tile, at most costing its
@@ -826,7 +767,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
         n0 = __shfl_sync(0xffffffffu, n0, 0);
       }
       if (lane == 0) {
-        items[slot] = FwdItem{pr, bh, nkv, n0, has1, nch, pf, 0};
+        items[slot] = FwdItem{pr, bh, nkv, n0, has1, 0, 0, 0};
         mbar_arrive(&item_full[slot]);
         if ((ok = mbar_wait(&q_empty[slot], ((ii >> 1) & 1) ^ 1, abort_flag, err))) {
           uint8_t* qd = sm + L::Q + slot * 2 * Q_BYTES;
@@ -838,15 +779,14 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
           const int s = gk % kKvStages;
           if (!(ok = mbar_wait(&kv_empty[s], ((gk / kKvStages) & 1) ^ 1, abort_flag, err))) break;
           mbar_arrive_expect_tx(&kv_full[s], 2 * KV_BYTES);
-          const int key0 = kblock(slot, j, nkv) * FK;
-          tma_load_4d(sm + L::K + s * KV_BYTES, &tmK, &kv_full[s], 0, key0, hk, b);
-          tma_load_4d(sm + L::V + s * KV_BYTES, &tmV, &kv_full[s], 0, key0, hk, b);
+          const int key0 = kblock(slot, j) * FK;
+          tma_load_4d(sm + L::K + s * KV_BYTES, &tmK, &kv_full[s], 0, key0, h, b);
+          tma_load_4d(sm + L::V + s * KV_BYTES, &tmV, &kv_full[s], 0, key0, h, b);
         }
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
-  };
-  auto issue = [&]() {
+  } else if (warp == 1 || warp == kFwdMma1Warp) {
     // One MMA thread per tile: S_x = Q_x K_j^T (128 x 128 fp32) for the next
     // block as soon as the softmax holds S_x in registers, O_x += P_x V_j
     // once P_x is in TMEM. The two tiles progress independently; each walks
@@ -863,8 +803,6 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
         const FwdItem inf = items[slot];
         if (inf.nkv < 0) break;  // no more items
         const int nb = x == 0 ? inf.n0 : (inf.has1 ? inf.nkv : 0);
-        // the tile's blocks are list entries [j0, j0 + nb)
-        const int j0 = GENERAL && x == 0 ? inf.nkv - nb : 0;
         const uint32_t sQ = smem_u32(sm + L::Q + (slot * 2 + x) * Q_BYTES);
         auto issue_s = [&](int s) {
           const uint32_t sK = smem_u32(sm + L::K + s * KV_BYTES);
@@ -874,34 +812,25 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
                       umma_smem_desc(sK + k * 32, 16, 1024), idS, k > 0);
           umma_commit(&s_full[x]);
         };
-        // a block this tile skips: release it once it has arrived
-        auto skip = [&](int j) {
-          const int s = (gk + j) % kKvStages;
-          if (!mbar_wait(&kv_full[s], ((gk + j) / kKvStages) & 1, abort_flag, err)) return false;
-          mbar_arrive(&kv_empty[s]);
-          return true;
-        };
-        for (int j = 0; ok && j < j0; ++j) ok = skip(j);
-        if (!ok) break;
         if (nb > 0) {
           // S of the item's first block: Q loaded, the block loaded, and the
           // previous item's last S taken out of TMEM by the softmax
-          const int s0 = (gk + j0) % kKvStages;
           ok = mbar_wait(&q_full[slot], (ii >> 1) & 1, abort_flag, err) &&
-               mbar_wait(&kv_full[s0], ((gk + j0) / kKvStages) & 1, abort_flag, err) &&
+               mbar_wait(&kv_full[gk % kKvStages], (gk / kKvStages) & 1, abort_flag, err) &&
                (jx == 0 || mbar_wait(&s_free[x], (jx - 1) & 1, abort_flag, err));
           if (!ok) break;
           tc_fence_after();
-          issue_s(s0);
+          issue_s(gk % kKvStages);
         }
-        for (int j = j0; ok && j < inf.nkv; ++j) {
+        for (int j = 0; ok && j < inf.nkv; ++j) {
           const int s = (gk + j) % kKvStages;
-          if (j >= j0 + nb) {
-            ok = skip(j);
+          if (j >= nb) {  // a block this tile skips: release it once it has arrived
+            if (!(ok = mbar_wait(&kv_full[s], ((gk + j) / kKvStages) & 1, abort_flag, err))) break;
+            mbar_arrive(&kv_empty[s]);
             continue;
           }
-          const int jj = jx + j - j0;  // running block index of this tile
-          if (j + 1 < j0 + nb) {
+          const int jj = jx + j;  // running block index of this tile
+          if (j + 1 < nb) {
             const int s1 = (gk + j + 1) % kKvStages;
             if (!(ok = mbar_wait(&kv_full[s1], ((gk + j + 1) / kKvStages) & 1, abort_flag, err)) ||
                 !(ok = mbar_wait(&s_free[x], jj & 1, abort_flag, err)))
@@ -916,7 +845,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
 #pragma unroll
           for (int k = 0; k < FK / 16; ++k)
             umma_bf16_ts(tO(x), tP(x) + k * 8, umma_smem_desc(sV + k * 2048, KV_BYTES, 1024), idO,
-                         (j > j0 || k > 0));
+                         (j > 0 || k > 0));
           umma_commit(&pv_done[x]);
           umma_commit(&kv_empty[s]);
         }
@@ -931,8 +860,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
         jx += nb;
       }
     }
-  };
-  [[maybe_unused]] auto softmax = [&]() {
+  } else if (warp < kFwdMma1Warp) {
     // Softmax warpgroup x (warps 2-5: tile 0, 6-9: tile 1); thread = query
     // row r of the tile (TMEM lane r). Per block: the S row into registers,
     // its max, then exp + row sum + P, with a running max that is only raised
@@ -968,7 +896,7 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
         const int jj = jx + j;
         if (!(ok = mbar_wait(&s_full[x], jj & 1, abort_flag, err))) break;
         tc_fence_after();
-        const int jb = kblock(slot, j, inf.nkv);
+        const int jb = kblock(slot, j);
         const bool diag = (jb == d0 + x);  // keys past the query (and past T) are masked
         // Per-element segment test unless keys and queries all share one id;
         // the block's key ids then come through shared memory (double-buffered,
@@ -1096,15 +1024,293 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
       if (lane == 0) mbar_arrive(&item_empty[slot]);
       jx += nb;
     }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (threadIdx.x == 0) sched_finish(p.sched);
+}
+
+// The forward of the score-modified attention. A kernel of its own: with the roles of
+// both as functions of one template, the plain kernel took 1 to 2.7% more time.
+template <bool SEG, int MODE>
+__global__ void __launch_bounds__(kFwdGeneralThreads, 1)
+    score_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                 const __grid_constant__ CUtensorMap tmV, const AttnParams p) {
+  using L = FwdSmem<SEG>;
+  extern __shared__ __align__(1024) uint8_t smem_fwd[];
+  uint8_t* sm = smem_fwd;
+  if (smem_u32(sm) & 1023) {  // the layout needs 1024-byte aligned tiles: give up, flagged
+    if (threadIdx.x == 0) {
+      atomicCAS(&g_attn_error, 0, kErrSmemAlign);
+      sched_finish(p.sched);
+    }
+    return;
+  }
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::BAR);
+  uint64_t* q_full = bars + 0;                 // [2 item slots]
+  uint64_t* q_empty = bars + 2;                // [2]
+  uint64_t* kv_full = bars + 4;                // [kKvStages]
+  uint64_t* kv_empty = kv_full + kKvStages;    // [kKvStages]
+  uint64_t* s_full = kv_empty + kKvStages;     // [2 tiles]: S of the current block is in TMEM
+  uint64_t* p_full = s_full + 2;               // [2]: P written to TMEM
+  uint64_t* pv_done = p_full + 2;              // [2]: the tile's P.V MMA has completed
+  uint64_t* s_free = pv_done + 2;              // [2]: S has been loaded into registers
+  uint64_t* item_full = s_free + 2;            // [2]
+  uint64_t* item_empty = item_full + 2;        // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(item_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  FwdItem* items = reinterpret_cast<FwdItem*>(sm + L::ITEM);
+
+  constexpr int kMma1Warp = 2;  // MMA thread of tile 1 (warp 1 serves tile 0)
+  constexpr int kSoftmaxWarp = 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int BH = p.B * p.H;
+  const int npair = (p.T + 2 * FQ - 1) / (2 * FQ);
+  const int n_items = npair * BH;  // item = bh * npair + (npair - 1 - pair)
+  int* err = &g_attn_error;
+  auto segtab_of = [&](int slot) {
+    return reinterpret_cast<int2*>(sm + L::SEGTAB) + slot * kMaxSegChunks;
   };
-  // The same for modified scores: one streaming pass per block against the
-  // reference that the rows have so far (Score::stream). Blocks with masked
-  // places, a row whose scores outgrow its reference and scores past the short
-  // form of tanh take steps instead, from the raw scores still in TMEM. The pass
-  // is a loop over 32 keys and no longer code: all 128 keys unrolled (15 KB) or 64
+  // Key block of list entry j of the item in `slot` (nkv entries). The list is walked
+  // from its end: the diagonal comes first and sets the rows' maxima, which a bias
+  // that falls with the distance then never raises.
+  auto kblock = [&](int slot, int j, int nkv) -> int {
+    j = nkv - 1 - j;
+    if constexpr (SEG)
+      return reinterpret_cast<const int*>(sm + L::BLOCKS)[slot * (kMaxSegChunks / 2) + j];
+    else
+      return j;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 2);  // released by each tile's MMA thread
+      mbar_init(&item_full[s], 1);
+      mbar_init(&item_empty[s], kFwdItemUsers);
+    }
+    for (int s = 0; s < kKvStages; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 2);  // released by each tile's MMA thread
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x], 4);
+      mbar_init(&pv_done[x], 1);
+      mbar_init(&s_free[x], 4);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // TMEM columns: S[2] (128 fp32 each) | O[2] (64 fp32) | P[2] (128 keys as bf16 pairs)
+  const uint32_t tmem = *tmem_slot;
+  auto tS = [&](int x) { return tmem + 128 * x; };
+  auto tO = [&](int x) { return tmem + 256 + 64 * x; };
+  auto tP = [&](int x) { return tmem + 384 + 64 * x; };
+
+  auto produce = [&]() {
+    // Item producer: publishes each item's slot (with segment ids also the
+    // chunk ranges and the key-block list), then loads its two Q tiles and its
+    // K/V blocks into the ring.
+    bool ok = true;
+    int gk = 0;
+    for (int ii = 0; ok; ++ii) {
+      const int slot = ii & 1;
+      const int item = next_item(p.sched, lane);
+      if (!(ok = mbar_wait(&item_empty[slot], ((ii >> 1) & 1) ^ 1, abort_flag, err))) break;
+      if (item >= n_items) {  // no more work: an empty slot ends every role's loop
+        if (lane == 0) {
+          items[slot].nkv = -1;
+          mbar_arrive(&item_full[slot]);
+        }
+        break;
+      }
+      int bh = item / npair, pr = npair - 1 - (item - bh * npair);
+      if (p.by_weight) {
+        pr = npair - 1 - item / BH;
+        bh = item % BH;
+      }
+      const int b = bh / p.H, h = bh - b * p.H;
+      const int q0 = pr * 2 * FQ;
+      // tile x's diagonal key block is d0 + x; tile 1 of the last pair may lie
+      // wholly past the sequence end
+      const int d0 = q0 / FK;
+      const int has1 = q0 + FQ < p.T;
+      const int dmax = has1 ? d0 + 1 : d0;
+      int nkv = dmax + 1, n0 = d0 + 1;
+      const int hk = h / p.group;
+      int pf = 0, nch = 0;
+      if (p.prefix) {  // the prefix's blocks are seen by both tiles
+        pf = min(max(p.prefix[b], 0), p.T);
+        nkv = max(nkv, (pf + FK - 1) / FK);
+        n0 = max(n0, (pf + FK - 1) / FK);
+      }
+      if constexpr (SEG) {
+        // The key blocks up to the diagonal or the prefix's end that either query
+        // tile can see, in order; both tiles walk this one list (tile 0 the first n0).
+        // A tile's diagonal block stays in it even if nothing meets there (padding
+        // alone), so that every tile has a block and writes its rows.
+        const int* segrow = p.seg + (int64_t)b * p.T;
+        int2* tab = segtab_of(slot);
+        nch = min((p.T + kSegChunk - 1) / kSegChunk, 2 * nkv);
+        for (int c = 0; c < nch; ++c) {
+          int mn = INT_MAX, mx = INT_MIN;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int t = c * kSegChunk + u * 32 + lane;
+            if (t < p.T) {
+              const int v = segrow[t];
+              mn = min(mn, v);
+              mx = max(mx, v);
+            }
+          }
+          mn = __reduce_min_sync(0xffffffffu, mn);
+          mx = __reduce_max_sync(0xffffffffu, mx);
+          if (lane == 0) tab[c] = seg_chunk(mn, mx);
+        }
+        __syncwarp();
+        if (lane == 0) {
+          int* bl = reinterpret_cast<int*>(sm + L::BLOCKS) + slot * (kMaxSegChunks / 2);
+          const int2 qr0 = seg_range(tab, nch, 2 * d0, 2);
+          const int2 qr1 = seg_range(tab, nch, 2 * d0 + 2, 2);
+          int n = 0, n_le0 = 0;
+          for (int j = 0; j < nkv; ++j) {
+            const int2 kr = seg_range(tab, nch, 2 * j, 2);
+            if (j == d0 || j == dmax || (j < n0 && seg_meet(kr, qr0)) ||
+                (has1 && seg_meet(kr, qr1))) {
+              bl[n++] = j;
+              if (j < n0) ++n_le0;
+            }
+          }
+          nkv = n;
+          n0 = n_le0;
+        }
+        nkv = __shfl_sync(0xffffffffu, nkv, 0);
+        n0 = __shfl_sync(0xffffffffu, n0, 0);
+      }
+      if (lane == 0) {
+        items[slot] = FwdItem{pr, bh, nkv, n0, has1, nch, pf, 0};
+        mbar_arrive(&item_full[slot]);
+        if ((ok = mbar_wait(&q_empty[slot], ((ii >> 1) & 1) ^ 1, abort_flag, err))) {
+          uint8_t* qd = sm + L::Q + slot * 2 * Q_BYTES;
+          mbar_arrive_expect_tx(&q_full[slot], 2 * Q_BYTES);
+          tma_load_4d(qd, &tmQ, &q_full[slot], 0, q0, h, b);
+          tma_load_4d(qd + Q_BYTES, &tmQ, &q_full[slot], 0, q0 + FQ, h, b);
+        }
+        for (int j = 0; ok && j < nkv; ++j, ++gk) {
+          const int s = gk % kKvStages;
+          if (!(ok = mbar_wait(&kv_empty[s], ((gk / kKvStages) & 1) ^ 1, abort_flag, err))) break;
+          mbar_arrive_expect_tx(&kv_full[s], 2 * KV_BYTES);
+          const int key0 = kblock(slot, j, nkv) * FK;
+          tma_load_4d(sm + L::K + s * KV_BYTES, &tmK, &kv_full[s], 0, key0, hk, b);
+          tma_load_4d(sm + L::V + s * KV_BYTES, &tmV, &kv_full[s], 0, key0, hk, b);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+    }
+  };
+  auto issue = [&]() {
+    // One MMA thread per tile: S_x = Q_x K_j^T (128 x 128 fp32) for the next
+    // block as soon as the softmax holds S_x in registers, O_x += P_x V_j
+    // once P_x is in TMEM. The two tiles progress independently; each walks
+    // every block of the item's list and releases the ones it does not use.
+    const int x = warp == 1 ? 0 : 1;
+    if (lane == 0) {
+      constexpr uint32_t idS = umma_idesc_bf16(128, FK, 0, 0);
+      constexpr uint32_t idO = umma_idesc_bf16(128, HD, 0, 1);  // A = P in TMEM, B = V MN-major
+      bool ok = true;
+      int gk = 0, jx = 0, ii = 0;  // ring block, this tile's running block, item
+      for (; ok; ++ii) {
+        const int slot = ii & 1;
+        if (!(ok = mbar_wait(&item_full[slot], (ii >> 1) & 1, abort_flag, err))) break;
+        const FwdItem inf = items[slot];
+        if (inf.nkv < 0) break;  // no more items
+        const int nb = x == 0 ? inf.n0 : (inf.has1 ? inf.nkv : 0);
+        // the tile's blocks are list entries [j0, j0 + nb)
+        const int j0 = x == 0 ? inf.nkv - nb : 0;
+        const uint32_t sQ = smem_u32(sm + L::Q + (slot * 2 + x) * Q_BYTES);
+        auto issue_s = [&](int s) {
+          const uint32_t sK = smem_u32(sm + L::K + s * KV_BYTES);
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k)
+            umma_bf16(tS(x), umma_smem_desc(sQ + k * 32, 16, 1024),
+                      umma_smem_desc(sK + k * 32, 16, 1024), idS, k > 0);
+          umma_commit(&s_full[x]);
+        };
+        // a block this tile skips: release it once it has arrived
+        auto skip = [&](int j) {
+          const int s = (gk + j) % kKvStages;
+          if (!mbar_wait(&kv_full[s], ((gk + j) / kKvStages) & 1, abort_flag, err)) return false;
+          mbar_arrive(&kv_empty[s]);
+          return true;
+        };
+        for (int j = 0; ok && j < j0; ++j) ok = skip(j);
+        if (!ok) break;
+        if (nb > 0) {
+          // S of the item's first block: Q loaded, the block loaded, and the
+          // previous item's last S taken out of TMEM by the softmax
+          const int s0 = (gk + j0) % kKvStages;
+          ok = mbar_wait(&q_full[slot], (ii >> 1) & 1, abort_flag, err) &&
+               mbar_wait(&kv_full[s0], ((gk + j0) / kKvStages) & 1, abort_flag, err) &&
+               (jx == 0 || mbar_wait(&s_free[x], (jx - 1) & 1, abort_flag, err));
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(s0);
+        }
+        for (int j = j0; ok && j < inf.nkv; ++j) {
+          const int s = (gk + j) % kKvStages;
+          if (j >= j0 + nb) {
+            ok = skip(j);
+            continue;
+          }
+          const int jj = jx + j - j0;  // running block index of this tile
+          if (j + 1 < j0 + nb) {
+            const int s1 = (gk + j + 1) % kKvStages;
+            if (!(ok = mbar_wait(&kv_full[s1], ((gk + j + 1) / kKvStages) & 1, abort_flag, err)) ||
+                !(ok = mbar_wait(&s_free[x], jj & 1, abort_flag, err)))
+              break;
+            tc_fence_after();
+            issue_s(s1);
+          }
+          if (!(ok = mbar_wait(&p_full[x], jj & 1, abort_flag, err))) break;
+          tc_fence_after();
+          const uint32_t sV = smem_u32(sm + L::V + s * KV_BYTES);
+          // O_x += P_x V_j, P read from TMEM (keys 16k..16k+15 at column 8k)
+#pragma unroll
+          for (int k = 0; k < FK / 16; ++k)
+            umma_bf16_ts(tO(x), tP(x) + k * 8, umma_smem_desc(sV + k * 2048, KV_BYTES, 1024), idO,
+                         (j > j0 || k > 0));
+          umma_commit(&pv_done[x]);
+          umma_commit(&kv_empty[s]);
+        }
+        if (!ok) break;
+        // the item's Q tile is free once its last S MMA has completed
+        if (nb > 0)
+          umma_commit(&q_empty[slot]);
+        else
+          mbar_arrive(&q_empty[slot]);
+        mbar_arrive(&item_empty[slot]);
+        gk += inf.nkv;
+        jx += nb;
+      }
+    }
+  };
+  // Softmax warpgroup x; thread = query row r of the tile (TMEM lane r). One streaming
+  // pass per block against the reference that the rows have so far (Score::stream).
+  // Blocks with masked places, a row whose scores outgrow its reference and scores past
+  // the short form of tanh take steps instead, from the raw scores still in TMEM. The
+  // pass is a loop over 32 keys and no longer code: all 128 keys unrolled (15 KB) or 64
   // take 268 to 283 us at 1 x 12 x 8192, this 259 (279 with TMEM loads that nothing
   // covers).
-  [[maybe_unused]] auto softmax_general = [&]() {
+  auto softmax = [&]() {
     const int x = (warp - kSoftmaxWarp) >> 2;
     const int quad = warp & 3;
     const int r = quad * 32 + lane;
@@ -1292,23 +1498,15 @@ __global__ void __launch_bounds__(MODE == kClassic ? kFwdThreads : kFwdGeneralTh
       jx += nb;
     }
   };
-  if constexpr (GENERAL) {
-    if (warp < kSoftmaxWarp) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFwdRegsIssue));
-      if (warp == 0) {
-        produce();
-      } else if (warp <= kMma1Warp) {
-        issue();
-      }
-    } else {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFwdRegsSoftmax));
-      softmax_general();
+  if (warp < kSoftmaxWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFwdRegsIssue));
+    if (warp == 0) {
+      produce();
+    } else if (warp <= kMma1Warp) {
+      issue();
     }
-  } else if (warp == 0) {
-    produce();
-  } else if (warp == 1 || warp == kMma1Warp) {
-    issue();
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFwdRegsSoftmax));
     softmax();
   }
   tc_fence_before();
@@ -2396,7 +2594,7 @@ extern "C" int gptb200_attention_fwd(const void* q, const void* k, const void* v
   int dev = 0;
   cudaGetDevice(&dev);
   const int seg = segment_ids != nullptr;
-  auto kern = seg ? attn_fwd_tc<true, kClassic> : attn_fwd_tc<false, kClassic>;
+  auto kern = seg ? attn_fwd_tc<true> : attn_fwd_tc<false>;
   const int smem = seg ? FwdSmem<true>::TOTAL : FwdSmem<false>::TOTAL;
   int sms = 148;
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -2594,7 +2792,7 @@ template <bool SEG, int MODE>
 static int score_fwd_launch(const AttnParams& p, const ScoreMaps& m, cudaStream_t st) {
   static bool done[64] = {};
   const int64_t items = (int64_t)((p.T + 2 * FQ - 1) / (2 * FQ)) * p.B * p.H;
-  return launch_persistent(attn_fwd_tc<SEG, MODE>, done, items, kFwdGeneralThreads,
+  return launch_persistent(score_fwd_tc<SEG, MODE>, done, items, kFwdGeneralThreads,
                            FwdSmem<SEG>::TOTAL, st, m.q, m.k, m.v, p);
 }
 
