@@ -682,7 +682,7 @@ def _adamw8_plan(n: int, groups_dev: torch.Tensor, n_groups: int, workspace: tor
     size = n_groups * ctypes.sizeof(_lib.TensorGroup)
     if not groups_dev.is_cuda or not groups_dev.is_contiguous() or groups_dev.nbytes < size:
         raise ValueError(f"{n_groups} tensor groups are {size} contiguous bytes on the device")
-    size = int(_lib.load().gptb200_adamw_workspace_size(n))
+    size = _lib.load().gptb200_adamw_workspace_size(n)
     if not workspace.is_cuda or not workspace.is_contiguous() or workspace.nbytes < size:
         raise ValueError(f"the workspace needs {size} bytes on the device")
 
@@ -697,11 +697,14 @@ def adamw8_step(params, state, grads, groups_dev, n_groups, cfg, step, loss, his
     n = params.numel()
     q = _adamw8(state, n)
     _adamw8_plan(n, groups_dev, n_groups, workspace)
-    for name, t, dtype in (("step", step, torch.int32), ("loss", loss, F32), ("history", history, F32)):
-        if t is not None:
-            _adamw8_flat(name, t, max(1, t.numel()), dtype)
-    if history is not None and (history.dim() != 2 or history.shape[1] != 3):
-        raise ValueError(f"history must have rows of 3 numbers, got {tuple(history.shape)}")
+    if not step.is_cuda or step.dtype is not torch.int32 or not step.numel():
+        raise ValueError(f"step must be a CUDA tensor of int32, got {step.device} {step.dtype}")
+    if loss is not None and (not loss.is_cuda or loss.dtype is not F32 or not loss.numel()):
+        raise ValueError(f"loss must be a CUDA tensor of {F32}, got {loss.device} {loss.dtype}")
+    if history is not None and (not history.is_cuda or history.dtype is not F32 or history.dim() != 2
+                                or history.shape[1] != 3 or not history.is_contiguous()):
+        raise ValueError(f"history must be a contiguous CUDA tensor of {F32} [steps, 3], got "
+                         f"{history.device} {history.dtype} {tuple(history.shape)}")
     call("gptb200_adamw8_step", _adamw8_flat("params", params, n, F32), q,
          _adamw8_flat("grads", grads, n, F32), n, groups_dev.data_ptr(), n_groups, cfg,
          step.data_ptr(), _ptr(loss), _ptr(history), _adamw8_flat("params_bf16", params_bf16, n, BF16),
