@@ -73,6 +73,7 @@
 #include <algorithm>
 #include <mutex>
 #include <new>
+#include <shared_mutex>
 #include <type_traits>
 #include <unordered_map>
 #include <vector>
@@ -201,7 +202,7 @@ __device__ __forceinline__ int2 seg_range(const int2* tab, int nch, int c, int n
 // once cover a few heads whose K/V or Q/dO tiles come from DRAM about once and
 // are then served from L2, and a CTA that finishes early takes more work).
 // The counters live in a device array of slots. Launches that may overlap on the
-// GPU have different slots (sched_slot), and the last CTA of a launch to finish
+// GPU have different slots (SchedSlot), and the last CTA of a launch to finish
 // puts its slot back to zero.
 constexpr int kSchedSlots = 1 << 16;
 __device__ unsigned g_attn_sched[kSchedSlots][2];
@@ -2405,10 +2406,11 @@ int attention_read_error(int clear) {
 // graph, so each has a slot to itself until the graph and everything instantiated
 // from it are gone (a graph does not run beside itself).
 struct SchedSlots {
-  std::mutex mu;
+  std::shared_mutex launching;  // shared: from the choice of a slot to the launch
+  std::mutex mu;                // the fields below
   unsigned* base = nullptr;
   int used = 0;                                // slots [0, used) have been handed out
-  std::vector<int> free;                       // of these, back from graphs
+  std::vector<int> free;                       // of these, those that nothing holds
   std::unordered_map<unsigned long long, int> of_stream;
 
   int take() {  // -1: none is left
@@ -2418,6 +2420,17 @@ struct SchedSlots {
       return k;
     }
     return used < kSchedSlots ? used++ : -1;
+  }
+  // A program that has used as many streams as there are slots: once the device is
+  // idle, and no thread between its choice and its launch, no stream needs its slot.
+  cudaError_t forget_streams() {
+    std::unique_lock<std::shared_mutex> none(launching);
+    const cudaError_t e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(mu);
+    for (const auto& s : of_stream) free.push_back(s.second);
+    of_stream.clear();
+    return cudaSuccess;
   }
 };
 struct GraphSlot {
@@ -2433,57 +2446,75 @@ static void CUDART_CB return_slot(void* p) {  // a graph's last reference has go
   delete g;
 }
 
-// The counter slot of a launch on `st`: 0, or an error (without a slot left:
-// 65,536 streams and captured launches at a time).
-static int sched_slot(cudaStream_t st, unsigned** slot) try {
-  static SchedSlots* const devices = new SchedSlots[64];  // graphs may outlive static objects
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 64) return GPTB200_EUNSUPPORTED;
-  SchedSlots& d = devices[dev];
-  cudaStreamCaptureStatus status;
-  cudaGraph_t graph = nullptr;
-  unsigned long long id = 0;
-  cudaError_t e = cudaStreamGetCaptureInfo(st, &status, &id, &graph);
-  if (e == cudaSuccess && status != cudaStreamCaptureStatusActive) e = cudaStreamGetId(st, &id);
-  if (e != cudaSuccess) return -static_cast<int>(e);
-  int k;
-  {
-    std::lock_guard<std::mutex> lock(d.mu);
-    if (!d.base) {
-      void* ptr = nullptr;
-      e = cudaGetSymbolAddress(&ptr, g_attn_sched);
+// The counter slot of a launch on `st`; kept until the launch has been made. status:
+// 0, or an error (65,536 captured launches at a time leave no slot).
+struct SchedSlot {
+  int status;
+  unsigned* counter = nullptr;
+  explicit SchedSlot(cudaStream_t st) {
+    try {
+      status = choose(st);
+    } catch (const std::bad_alloc&) {
+      status = -static_cast<int>(cudaErrorMemoryAllocation);
+    }
+  }
+
+ private:
+  std::shared_lock<std::shared_mutex> launching_;
+
+  int choose(cudaStream_t st) {
+    static SchedSlots* const devices = new SchedSlots[64];  // graphs may outlive static objects
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64) return GPTB200_EUNSUPPORTED;
+    SchedSlots& d = devices[dev];
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    cudaGraph_t graph = nullptr;
+    unsigned long long id = 0;
+    cudaError_t e = cudaStreamGetCaptureInfo(st, &capture, &id, &graph);
+    const bool captured = capture == cudaStreamCaptureStatusActive;
+    if (e == cudaSuccess && !captured) e = cudaStreamGetId(st, &id);
+    if (e != cudaSuccess) return -static_cast<int>(e);
+    int k = -1;
+    for (int tries = 0; k < 0; ++tries) {
+      launching_ = std::shared_lock<std::shared_mutex>(d.launching);
+      {
+        std::lock_guard<std::mutex> lock(d.mu);
+        if (!d.base) {
+          void* ptr = nullptr;
+          e = cudaGetSymbolAddress(&ptr, g_attn_sched);
+          if (e != cudaSuccess) return -static_cast<int>(e);
+          d.free.reserve(kSchedSlots);  // return_slot has no way to report a failure
+          d.base = reinterpret_cast<unsigned*>(ptr);
+        }
+        const auto known = captured ? d.of_stream.end() : d.of_stream.find(id);
+        k = known != d.of_stream.end() ? known->second : d.take();
+        if (!captured && k >= 0) d.of_stream.emplace(id, k);
+      }
+      if (k >= 0) break;
+      launching_.unlock();
+      if (captured || tries) return GPTB200_EUNSUPPORTED;
+      e = d.forget_streams();
       if (e != cudaSuccess) return -static_cast<int>(e);
-      d.free.reserve(kSchedSlots);  // return_slot has no way to report a failure
-      d.base = reinterpret_cast<unsigned*>(ptr);
     }
-    if (status == cudaStreamCaptureStatusActive) {
-      k = d.take();
-    } else {
-      const auto known = d.of_stream.find(id);
-      k = known != d.of_stream.end() ? known->second : d.take();
-      if (k >= 0 && known == d.of_stream.end()) d.of_stream.emplace(id, k);
+    if (captured) {
+      GraphSlot* g = new GraphSlot{&d, k};
+      cudaUserObject_t kept;
+      e = cudaUserObjectCreate(&kept, g, return_slot, 1, cudaUserObjectNoDestructorSync);
+      if (e != cudaSuccess) {
+        return_slot(g);
+        return -static_cast<int>(e);
+      }
+      e = cudaGraphRetainUserObject(graph, kept, 1, cudaGraphUserObjectMove);
+      if (e != cudaSuccess) {
+        cudaUserObjectRelease(kept, 1);  // the last reference: returns the slot
+        return -static_cast<int>(e);
+      }
     }
+    counter = d.base + 2 * (size_t)k;
+    return 0;
   }
-  if (k < 0) return GPTB200_EUNSUPPORTED;
-  *slot = d.base + 2 * (size_t)k;
-  if (status != cudaStreamCaptureStatusActive) return 0;
-  GraphSlot* g = new GraphSlot{&d, k};
-  cudaUserObject_t kept;
-  e = cudaUserObjectCreate(&kept, g, return_slot, 1, cudaUserObjectNoDestructorSync);
-  if (e != cudaSuccess) {
-    return_slot(g);
-    return -static_cast<int>(e);
-  }
-  e = cudaGraphRetainUserObject(graph, kept, 1, cudaGraphUserObjectMove);
-  if (e != cudaSuccess) {
-    cudaUserObjectRelease(kept, 1);  // the last reference: returns the slot
-    return -static_cast<int>(e);
-  }
-  return 0;
-} catch (const std::bad_alloc&) {
-  return -static_cast<int>(cudaErrorMemoryAllocation);
-}
+};
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -2588,8 +2619,9 @@ extern "C" int gptb200_attention_fwd(const void* q, const void* k, const void* v
   p.lse = lse;
   p.seg = segment_ids;
   auto st = reinterpret_cast<cudaStream_t>(stream);
-  const int no_slot = sched_slot(st, &p.sched);
-  if (no_slot) return no_slot;
+  const SchedSlot slot(st);
+  if (slot.status) return slot.status;
+  p.sched = slot.counter;
   static bool cfg[64][2] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -2670,8 +2702,9 @@ extern "C" int gptb200_attention_bwd(const void* q, const void* k, const void* v
   p.rcos = reinterpret_cast<const bf16*>(rope_cos);
   p.rsin = reinterpret_cast<const bf16*>(rope_sin);
   p.seg = segment_ids;
-  const int no_slot = sched_slot(st, &p.sched);
-  if (no_slot) return no_slot;
+  const SchedSlot slot(st);
+  if (slot.status) return slot.status;
+  p.sched = slot.counter;
   static bool cfg[64][4] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -2827,8 +2860,9 @@ static int score_forward(const gptb200_score_attention* a, float* o32, cudaStrea
       !make_map4(&m.k, a->k, p.B, p.KVH, p.T, ks[0], ks[1], ks[2], FK) ||
       !make_map4(&m.v, a->v, p.B, p.KVH, p.T, ks[0], ks[1], ks[2], FK))
     return GPTB200_ESHAPE;
-  const int no_slot = sched_slot(st, &p.sched);
-  if (no_slot) return no_slot;
+  const SchedSlot slot(st);
+  if (slot.status) return slot.status;
+  p.sched = slot.counter;
   // K and V of every head
   p.by_weight = by_weight(a->batch * a->kv_heads * a->seq * 2 * HD * 2, 128);
   return score_mode(a, [&](auto mode) {
@@ -2883,8 +2917,6 @@ extern "C" int gptb200_score_attention_bwd(const gptb200_score_attention* a, con
       !make_dq_map(&m.dq, dq_acc, p.B * p.H, p.T))
     return GPTB200_ESHAPE;
   auto st = reinterpret_cast<cudaStream_t>(stream);
-  const int no_slot = sched_slot(st, &p.sched);
-  if (no_slot) return no_slot;
   // delta = sum dO O from the stored O carries its rounding to bf16 (2^-9 |dO| |O|)
   // into dS = P (dP - delta) of the whole row. Where a row has few keys, one of
   // them tends to hold most of P, dP - delta is small for it and the rounding
@@ -2901,6 +2933,9 @@ extern "C" int gptb200_score_attention_bwd(const gptb200_score_attention* a, con
       p.o, reinterpret_cast<const bf16*>(dout), p.osb, p.osh, p.ost, dout_stride[0], dout_stride[1],
       dout_stride[2], p.B, p.H, p.T, delta, dq_acc, a->lse, neg_lse2, short_rows);
   GPTB200_CHECK_LAUNCH();
+  const SchedSlot slot(st);
+  if (slot.status) return slot.status;
+  p.sched = slot.counter;
   p.delta = delta;
   p.neg_lse2 = neg_lse2;
   p.dq_acc = dq_acc;

@@ -2,6 +2,8 @@
 graphs beside them. Each hands out its work items from a counter that no other
 launch in flight may draw from; a shared one leaves rows unwritten."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -86,4 +88,28 @@ def test_counters_of_graphs_come_back(cuda):
     run()
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(out[1:], want[1:]))
+    assert ops.device_error() == 0
+
+
+@pytest.mark.gpu
+def test_more_streams_than_counters(cuda):
+    """A launch on each of more streams than there are counters, none of them used before."""
+
+    q = torch.randn(2, 2, 300, 64, device=cuda).bfloat16()
+    want, o, lse = torch.empty_like(q), torch.empty_like(q), torch.empty(2, 2, 300, device=cuda)
+    ops.score_attention_fwd(q, q, q, want, lse, scale=0.125, softcap=30.0)
+    cudart, raw = torch.cuda.cudart(), ctypes.c_void_p()
+    for i in range(66000):
+        assert int(cudart.cudaStreamCreate(ctypes.addressof(raw))) == 0
+        look = i % 3000 == 2999
+        if look:
+            torch.cuda.synchronize()
+            o.zero_()
+            torch.cuda.synchronize()
+        with torch.cuda.stream(torch.cuda.ExternalStream(raw.value)):
+            ops.score_attention_fwd(q, q, q, o, lse, scale=0.125, softcap=30.0)
+        assert int(cudart.cudaStreamDestroy(raw.value)) == 0
+        if look:
+            torch.cuda.synchronize()
+            assert torch.equal(o, want)
     assert ops.device_error() == 0
