@@ -279,7 +279,8 @@ struct Score {
   float slope2;   // slope * log2(e)
   float far_max;  // the largest raw score squared (WIDE: z squared) with |z| <= 1
   GPTB200_DEV Score(const AttnParams& p, float slope2_) : slope2(slope2_) {
-    z_per_s = CAP ? p.scale / p.cap : 1.f;
+    // (finite for the smallest caps too: a score of 0 stays 0)
+    z_per_s = CAP ? fminf(p.scale / p.cap, 0x1p100f) : 1.f;
     out = (CAP ? p.cap : p.scale) * kLog2e;
     // below 2^-13 the ninth power in stream_coefs may underflow: never stream
     far_max = WIDE ? 1.f : z_per_s < 0x1p-13f ? -1.f : 1.f / (z_per_s * z_per_s);

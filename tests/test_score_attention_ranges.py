@@ -63,3 +63,17 @@ def test_large_caps(cuda, cap, spread, bias):
     assert (lse.double() - want_lse).abs().max() <= 16 * 2.0 ** -23 * top
     for n in want:
         assert ((got[n].double() - want[n]).abs() <= 1.2 * tol[n]).all(), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [1e-40, 1e-38, 1e-20, 1e-6])
+def test_tiny_caps(cuda, cap):
+    """Next to nothing is left of any score, scores of exactly 0 among them: the mean of
+    the values. (Without a bias; 1e-40 is a denormal number, scale / cap overflows.)"""
+
+    q, k, v, do = (x.to(cuda) for x in _inputs(1, 2, 1, 300, 23))
+    q[:, :, ::5] = 0
+    k[:, :, 7::11] = 0
+    want, tol, want_lse = _formula(q, k, v, do, 0.125, cap, None, None, None)
+    got, lse = _run(q, k, v, do, scale=0.125, softcap=cap)
+    _check(got, lse, want, tol, want_lse)
