@@ -2789,7 +2789,9 @@ static AttnParams score_params(const gptb200_score_attention* a) {
 // head by head. By weight the last items are light and every SM ends at about
 // the same time; head by head the tiles that the items of a head share stay in
 // L2. So: by weight while the shared tiles of all heads (`bytes`) fit, and in the
-// backward longer for capped scores, which compute more per byte. Measured at 12
+// backward longer for capped scores, which compute more per byte. One limit cannot tell
+// many short sequences from few long ones: the capped backward of 128 x 1024 is past it
+// and 8% slower for that, 16 x 8192 20% faster. Measured at 12
 // heads (us, by weight / head by head; MB of shared tiles), capped and biased |
 // without either:
 //   forward  25 MB (1 x 8192): 260 / 331 | 185 / 235;  101 MB (4 x 8192): 945 / 1011
@@ -2921,10 +2923,13 @@ extern "C" int gptb200_score_attention_bwd(const gptb200_score_attention* a, con
   // delta = sum dO O from the stored O carries its rounding to bf16 (2^-9 |dO| |O|)
   // into dS = P (dP - delta) of the whole row. Where a row has few keys, one of
   // them tends to hold most of P, dP - delta is small for it and the rounding
-  // weighs more: dq and dk are 0.0046 off at 33 keys, 0.0037 at 64 to 256 and
-  // 0.0030 at 1,024 (relative; 0.0024 with an exact delta). So sequences of one
-  // key tile compute O again, in fp32 and into the accumulator that delta's
-  // kernel clears: one more launch for a forward of one block a tile.
+  // weighs more. Off by (dq, relative): rows of up to 8 keys 0.0046, 16 0.0041, 33
+  // 0.0038, 64 0.0036, 300 0.0035, 1,024 0.0034; with an exact delta 0.0025 at any
+  // length. So sequences of one key tile compute O again, in fp32 and into the
+  // accumulator that delta's kernel clears (O as stored is not read then): one more
+  // launch of one block a tile, 3 us. Longer ones would pay a whole forward (1 x 12 x
+  // 8192: 454 us and 259 more), so short documents in them keep the errors above, as
+  // they have them in the plain attention.
   const bool short_rows = p.T <= FK;
   if (short_rows) {
     const int f = score_forward(a, dq_acc, st);

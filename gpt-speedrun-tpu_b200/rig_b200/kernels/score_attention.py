@@ -7,7 +7,8 @@ forward/backward kernels:
 
 with optional key/value heads shared by several query heads, segment ids
 (negative: padding) and a per-sequence prefix that every query sees. A query
-that sees no key gives zeros. The reference has no counterpart.
+that sees no key gives zeros. What the masks hide must still be finite numbers
+(0 * NaN is NaN in the products). The reference has no counterpart.
 """
 
 from __future__ import annotations

@@ -140,7 +140,8 @@ int gptb200_rms_norm_bwd(const void* x, const void* scale, const float* rstd, co
 
 /* ------------------------------------------------------------------ layer norm
  * y = (x - mean) * rstd * scale + bias, rstd = 1 / sqrt(var + eps), statistics
- * in fp32 (the variance about the mean), one rounding at the end. x, y, scale
+ * in fp32 (the mean to half a unit of its last place, the variance about it; a
+ * constant row gives the bias), one rounding at the end. x, y, scale
  * and bias have element type `dtype`; bias may be NULL; rows have unit inner
  * stride and row strides of x_stride / y_stride elements (>= d). mean, rstd:
  * fp32 [rows], saved for the backward. Any d from 1 to 16384; rows of 8-element
@@ -216,6 +217,9 @@ int gptb200_document_segments(const int32_t* tokens, int64_t batch, int64_t seq,
  * documents on top of the causal mask, reference_causal_attention's
  * segment_ids); key blocks whose id range misses a query tile's are skipped.
  * With segment ids, seq <= 65536 (GPTB200_EUNSUPPORTED otherwise).
+ * Launches on different streams and in captured graphs may overlap; 65,536
+ * captured launches at a time, counting forwards and backwards of this and the
+ * score-modified attention, are the most (GPTB200_EUNSUPPORTED beyond).
  * Replaces rig/kernels/tpu_flash_attention.py:236-348 (forward kernel) behind
  * make_causal_attention (:962-1164); semantics of reference_causal_attention
  * (:171-207).
@@ -245,7 +249,8 @@ int gptb200_attention_bwd(const void* q, const void* k, const void* v, int64_t s
  * Causal attention whose scores are capped and biased before the softmax (no
  * reference counterpart):
  *   s'_ij = softcap * tanh(softmax_scale q_i.k_j / softcap) - slopes[h] |i - j|
- * softcap 0: no cap; slopes NULL: no bias (finite fp32 [heads] otherwise; they
+ * The tanh is off by 7e-6 of itself, for caps above 128 by 2e-7. softcap 0: no cap;
+ * slopes NULL: no bias (finite fp32 [heads] otherwise; they
  * are constants, no gradient). heads is a multiple of kv_heads: query head h
  * reads key/value head h / (heads / kv_heads), whose dk and dv sum over its
  * query heads. Query i sees key j if
