@@ -163,32 +163,6 @@ __device__ __forceinline__ bool rng_single(int2 a, int2 b) {
   return a.x == a.y && b.x == b.y && a.x == b.x;
 }
 
-// tab[c - c0] = (min, max) id of positions [64c, 64c + 64) of seg_row for
-// chunks c0 <= c < c1; positions past T are ignored (an empty chunk is
-// (INT_MAX, INT_MIN)). Every thread of the CTA takes part.
-__device__ void seg_chunk_ranges(const int* __restrict__ seg_row, int T, int c0, int c1,
-                                 int2* tab) {
-  const int warps = blockDim.x >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int c = c0 + w; c < c1; c += warps) {
-    int mn = INT_MAX, mx = INT_MIN;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int t = c * kSegChunk + u * 32 + lane;
-      if (t < T) {
-        const int v = seg_row[t];
-        mn = min(mn, v);
-        mx = max(mx, v);
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      mn = min(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    }
-    if (lane == 0) tab[c - c0] = make_int2(mn, mx);
-  }
-}
-
 // Range of the ids in table entries [c, c + n) (entries at or past nch are empty).
 __device__ __forceinline__ int2 seg_range(const int2* tab, int nch, int c, int n) {
   int2 r = make_int2(INT_MAX, INT_MIN);
